@@ -1,0 +1,384 @@
+"""What is measured of three operators: the AdamW step over many tensors (states in 32 or in 8 bits), the product of
+8-bit rows (a scale for each token and channel) and the fold that ends a stride-2 transposed convolution made as such a
+product.  `run` computes a case in its plain form, or (`own`) through pgan_hip.HipOps."""
+import math
+import os
+import random
+import sys
+
+import torch
+import torch.nn.functional as F
+
+own = False
+
+DEV = "cuda"
+LR, B1, B2, EPS, DECAY = 5e-5, 0.5, 0.999, 1e-8, 0.01      # the trainer's rates; the decay is AdamW's usual one
+STEP = 37                                                    # steps made before the first one that is run
+SEED8 = 12345                                                # seed of the 8-bit states' rounding
+BLOCK = 256                                                  # elements of a state that share a scale
+M32 = 0xFFFFFFFF
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+
+# elements of the parameter tensors of the two networks (64 x 64 alignments, latent size 128)
+CRITIC = ([1024, 64, 64, 131072, 128, 128, 524288, 256, 256, 2097152, 512, 512]
+          + [64, 16, 16, 16, 2048, 32, 32, 32, 8192, 64, 64, 64] + [11712, 1])
+GENERATOR = ([1048576, 512, 512, 2097152, 256, 256, 524288, 128, 128, 131072, 64, 64, 1024]
+             + [32768, 64, 64, 8192, 32, 32, 2048, 16, 16, 512, 8, 8, 32])
+
+
+def listed():
+    adam = dict(op="adamw", tensors=0, least=0, most=0, shapes=0)
+    prod = dict(op="product", bias=True, lrelu=False, gap=0)
+    return [
+        # the two optimizer steps of a training iteration: 26 tensors, most of them tiny
+        dict(adam, name="adamw critic", net="critic", p="fp32", g="fp32", bits=32),
+        dict(adam, name="adamw generator 8", net="generator", p="fp32", g="fp32", bits=8),
+        # networks past the caches: 32 bits throughout, and parameters and gradients in bf16 with states in 8
+        dict(adam, name="adamw large", net="", tensors=24, least=100000, most=9000000, shapes=7, p="fp32", g="fp32", bits=32),
+        dict(adam, name="adamw large bf16 8", net="", tensors=24, least=100000, most=9000000, shapes=8, p="bf16", g="bf16", bits=8),
+        # one alignment drawn from a generator: the latent vector's product, where latency is what counts
+        dict(prod, name="product one token", T=1, K=128, N=8192, x="fp32", y="bf16"),
+        # its second stage: 16 pixels
+        dict(prod, name="product 16 tokens", T=16, K=512, N=4096, x="bf16", y="bf16", lrelu=True),
+        # the second stage of a thousand alignments: bound by what it writes
+        dict(prod, name="product 1000 alignments", T=16000, K=512, N=4096, x="bf16", y="bf16", lrelu=True),
+        # a long inner axis, where the matrix cores are what counts
+        dict(prod, name="product square", T=4096, K=4096, N=4096, x="bf16", y="bf16"),
+        # nothing a multiple of anything, rows that are part of wider ones
+        dict(prod, name="product odd", T=777, K=1001, N=1234, x="fp32", y="fp32", gap=5),
+        # the end of a generator stage: one alignment, and a thousand
+        dict(name="fold one", op="fold", B=1, H=8, W=8, C=128, y="bf16", out="q8"),
+        dict(name="fold 1000 alignments", op="fold", B=1000, H=16, W=16, C=64, y="bf16", out="q8"),
+        # the generator's last stage: a single channel and the sigmoid
+        dict(name="fold sites", op="fold", B=1000, H=32, W=32, C=1, y="bf16", out="sites"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(("adamw", "adamw", "product", "product", "product", "fold"))
+    types = ("fp32", "bf16", "fp16")
+    if kind == "adamw":
+        n, most = _log(rng, 1, 40), _log(rng, 300, 4000000)
+        return dict(op="adamw", net="", tensors=n, least=1, most=most, shapes=rng.randrange(1 << 20), p=rng.choice(types),
+                    g=rng.choice(types), bits=rng.choice((8, 32)))
+    if kind == "product":
+        K, N = _log(rng, 16, 4096), _log(rng, 16, 8192)
+        T = min(_log(rng, 1, 65536), (1 << 36) // (K * N), (1 << 26) // N)
+        if rng.random() < 0.5:
+            K, N = -(-K // 16) * 16, -(-N // 16) * 16
+        return dict(op="product", T=max(T, 1), K=K, N=N, x=rng.choice(types), y=rng.choice(types), bias=rng.random() < 0.7,
+                    lrelu=rng.random() < 0.4, gap=rng.choice((0, 0, 1, 24)))
+    H, W, C = rng.choice((4, 8, 16, rng.randint(1, 33))), rng.choice((4, 8, 16, rng.randint(1, 33))), _log(rng, 1, 512)
+    out = rng.choice(("q8", "q8", "sites", "tanh", "linear"))
+    B = min(_log(rng, 1, 1000), max(1, (1 << 27) // (16 * C * H * W)))
+    return dict(op="fold", B=B, H=H, W=W, C=C, y=rng.choice(types), out=out)
+
+
+# ---- what a program has in hand ------------------------------------------------------------------------------------
+def _sizes(case):
+    if case["net"]:
+        return CRITIC if case["net"] == "critic" else GENERATOR
+    rng = random.Random(case["shapes"])
+    return [_log(rng, case["least"], case["most"]) for _ in range(case["tensors"])]
+
+
+def _rows(T, K, dtype, gap=0):
+    """A [T, K] buffer whose rows start on multiples of 16 elements (gap: of any number, `gap` more than K)."""
+    return torch.empty(T, K + gap if gap else -(-K // 16) * 16, dtype=dtype, device=DEV)[:, :K]
+
+
+def prepare(case, seed):
+    gen = torch.Generator(DEV)
+    gen.manual_seed(seed * 7919 + 11)
+    randn = lambda *s: torch.randn(*s, generator=gen, device=DEV)   # noqa: E731
+    if case["op"] == "adamw":
+        sizes = _sizes(case)
+        held = [-(-n // BLOCK) * BLOCK for n in sizes]          # a state's slice starts on a block of its own
+        at, total = [], 0
+        for h in held:
+            at.append(total)
+            total += h
+        inside = torch.cat([torch.arange(h, device=DEV) < n for n, h in zip(sizes, held)])
+        m, v = randn(total) * 1e-3 * inside, (randn(total) * 1e-3 * inside).square()
+        s = dict(case=case, step=STEP, sizes=sizes, at=at, total=total,
+                 p=[(randn(n) * 0.05).to(DTYPES[case["p"]]) for n in sizes],
+                 g=[(randn(n) * 1e-3 * torch.exp(randn(n))).to(DTYPES[case["g"]]) for n in sizes])
+        if case["bits"] == 8:
+            first = torch.cat([torch.arange(0, h, BLOCK, device=DEV) for h in held])
+            which = torch.cat([torch.full((h // BLOCK,), i, dtype=torch.int64, device=DEV) for i, h in enumerate(held)])
+            s["first"], s["which"] = first, which               # a block's first element, and its tensor's number
+            r = v.sqrt()
+            s["ms"], s["rs"] = _scales(m.view(-1, BLOCK), v.view(-1, BLOCK))
+            s["m"] = (m.view(-1, BLOCK) / s["ms"][:, None]).to(torch.float8_e4m3fn).view(-1)
+            s["v"] = (r.view(-1, BLOCK) / s["rs"][:, None]).to(torch.float8_e4m3fn).view(-1)
+            s["mss"] = [s["ms"][a // BLOCK:(a + h) // BLOCK] for a, h in zip(at, held)]
+            s["rss"] = [s["rs"][a // BLOCK:(a + h) // BLOCK] for a, h in zip(at, held)]
+        else:
+            s["m"], s["v"] = m, v
+        s["m_of"] = [s["m"][a:a + n] for a, n in zip(at, sizes)]
+        s["v_of"] = [s["v"][a:a + n] for a, n in zip(at, sizes)]
+        return s
+    if case["op"] == "product":
+        T, K, N = case["T"], case["K"], case["N"]
+        x = _rows(T, K, DTYPES[case["x"]], case["gap"])
+        x.copy_(randn(T, K) * torch.exp(0.5 * randn(T, 1)))
+        w = randn(N, K) * 0.05                                  # the channels' weights, held in 8 bits
+        amax = w.abs().amax(dim=1).clamp_min(2.0 ** -100)
+        w8 = _rows(N, K, torch.int8)
+        w8.copy_(torch.round(w / amax[:, None] * 127))
+        return dict(case=case, x=x, w=w8, ws=amax / 127, bias=randn(N) * 0.1 if case["bias"] else None,
+                    q=_rows(T, K, torch.int8), qs=torch.empty(T, device=DEV), y=torch.empty(T, N, dtype=DTYPES[case["y"]], device=DEV))
+    B, H, W, C = case["B"], case["H"], case["W"], case["C"]
+    s = dict(case=case, y=randn(B, H, W, 16 * C).to(DTYPES[case["y"]]), shift=randn(C) * 0.3)
+    if case["out"] == "q8":
+        s.update(q=_rows(B * H * W * 4, C, torch.int8), qs=torch.empty(B * H * W * 4, device=DEV))
+    else:
+        s["out"] = torch.empty(B, 2 * H, 2 * W, C, device=DEV)
+    return s
+
+
+# ---- the plain forms -----------------------------------------------------------------------------------------------
+def _mix(x):
+    x = (x ^ (x >> 16)) * 0x6A09E667 & M32
+    x = (x ^ (x >> 15)) * 0xBB67AE85 & M32
+    return x ^ (x >> 16)
+
+
+def _dither(s):
+    """16 random bits for each element's first state and 16 for its second, from seed, step, tensor and place."""
+    key = _mix((SEED8 + s["step"] * 0xA54FF53B + s["which"] * 0x3C6EF373) & M32)
+    h = _mix(key[:, None] ^ ((s["first"][:, None] + torch.arange(BLOCK, device=DEV)) & M32))
+    return h & 0xFFFF, h >> 16
+
+
+def _exponent(x):
+    return (x.view(torch.int32) >> 23) - 127
+
+
+def _scales(m, v):
+    """Powers of two that bring a block's largest magnitudes into [128, 256); the second state is held as its root."""
+    em = _exponent(m.abs().amax(dim=1)).clamp_min(-100)
+    er = _exponent(v.amax(dim=1)).clamp_min(-126) >> 1
+    one = torch.ones(1, device=DEV)
+    return torch.ldexp(one, em - 7), torch.ldexp(one, er - 7)
+
+
+def _encode(y, u16):
+    """Codes of y in [0, 256): four exponent bits, three of mantissa; u16 (16 random bits) decides the rounding."""
+    small = y < 2.0 ** -6
+    bits = torch.where(small, y + 2.0 ** -6, y).view(torch.int32).to(torch.int64)
+    return ((bits + (u16 << 4) + 8) >> 20) - 960 - 8 * small
+
+
+def _flat(ts):
+    return torch.cat([F.pad(t.reshape(-1).float(), (0, -t.numel() % BLOCK)) for t in ts])
+
+
+def _adamw(s):
+    case = s["case"]
+    s["step"] += 1
+    p, g = _flat(s["p"]), _flat(s["g"])
+    if case["bits"] == 8:
+        m = (s["m"].float().view(-1, BLOCK) * s["ms"][:, None]).view(-1)
+        r = (s["v"].float().view(-1, BLOCK) * s["rs"][:, None]).view(-1)
+        v = r * r
+    else:
+        m, v = s["m"], s["v"]
+    m = m * B1 + g * (1 - B1)
+    v = v * B2 + (g * g) * (1 - B2)
+    root = v.sqrt()
+    size, inv = LR / (1 - B1 ** s["step"]), 1 / math.sqrt(1 - B2 ** s["step"])
+    p = p * (1 - LR * DECAY) - (m * size) / (root * inv + EPS)
+    if case["bits"] == 8:
+        um, ur = _dither(s)
+        mb, rb = m.view(-1, BLOCK), root.view(-1, BLOCK)
+        ms, rs = _scales(mb, v.view(-1, BLOCK))
+        cm = _encode(mb.abs() / ms[:, None], um) + 128 * (mb < 0)
+        cr = torch.maximum(_encode(rb / rs[:, None], ur), (v.view(-1, BLOCK) > 0).to(torch.int64))
+        s["m"].copy_(cm.to(torch.uint8).view(-1).view(torch.float8_e4m3fn))
+        s["v"].copy_(cr.to(torch.uint8).view(-1).view(torch.float8_e4m3fn))
+        s["ms"].copy_(ms)
+        s["rs"].copy_(rs)
+    else:
+        s["m"].copy_(m)
+        s["v"].copy_(v)
+    torch._foreach_copy_(s["p"], [p[a:a + n] for a, n in zip(s["at"], s["sizes"])])
+
+
+def _codes(x):
+    """Rows of fp32 values as whole numbers in [-127, 127] and their scales; a row that holds no finite maximum gets the
+    scale NaN."""
+    amax = x.abs().amax(dim=-1).clamp_min(2.0 ** -100)
+    fine = torch.isfinite(amax)
+    inv = torch.full_like(amax, 127.0) / amax
+    q = torch.where(fine[..., None], torch.round(x * inv[..., None]), 0.0)
+    return q, torch.where(fine, amax * (1 / 127), math.nan)
+
+
+def _lrelu(x):
+    return torch.where(x > 0, x, x * 0.1)
+
+
+def _product(s):
+    x = s["x"].float()
+    q, qs = _codes(_lrelu(x) if s["case"]["lrelu"] else x)
+    y = (q @ s["w"].float().t()) * (qs[:, None] * s["ws"][None])
+    s["y"].copy_(y if s["bias"] is None else y + s["bias"])
+
+
+def _fold(s):
+    """Rows first: an even output row takes taps 1 (its own input row) and 3 (the one before), an odd one 2 and 0 (the
+    one after); then the same along the columns."""
+    case = s["case"]
+    B, H, W, C = case["B"], case["H"], case["W"], case["C"]
+    t = s["y"].float().view(B, H, W, 4, 4, C)
+    down = lambda a: F.pad(a, (0, 0, 0, 0, 0, 0, 1, 0))[:, :H]                  # noqa: E731
+    up = lambda a: F.pad(a, (0, 0, 0, 0, 0, 0, 0, 1))[:, 1:]                    # noqa: E731
+    rows = torch.stack([t[:, :, :, 1] + down(t[:, :, :, 3]), t[:, :, :, 2] + up(t[:, :, :, 0])], dim=2)   # B H 2 W 4 C
+    right = lambda a: F.pad(a, (0, 0, 1, 0))[..., :W, :]                        # noqa: E731
+    left = lambda a: F.pad(a, (0, 0, 0, 1))[..., 1:, :]                         # noqa: E731
+    o = torch.stack([rows[..., 1, :] + right(rows[..., 3, :]), rows[..., 2, :] + left(rows[..., 0, :])], dim=4)
+    o = o.reshape(B, 2 * H, 2 * W, C) + s["shift"]
+    if case["out"] == "q8":
+        q, qs = _codes(_lrelu(o).view(-1, C))
+        s["q"].copy_(q)
+        s["qs"].copy_(qs)
+    else:
+        s["out"].copy_(torch.sigmoid(o) if case["out"] == "sites" else torch.tanh(o) if case["out"] == "tanh" else o)
+
+
+# ---- the framework's calls -----------------------------------------------------------------------------------------
+_OPS = []
+
+
+def _ops():
+    if not _OPS:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pg-alignments-gan_amd"))
+        from pgan_hip import HipOps
+        _OPS.append(HipOps(torch.device(DEV, torch.cuda.current_device()), ws_floats=4, max_samples=1))
+    return _OPS[0]
+
+
+def run(s):
+    case = s["case"]
+    if case["op"] == "adamw":
+        if own:
+            s["step"] += 1
+            _ops().adamw(s["p"], s["g"], s["m_of"], s["v_of"], s["step"], LR, B1, B2, EPS, DECAY,
+                         scales=(s["mss"], s["rss"]) if case["bits"] == 8 else None, seed=SEED8)
+        else:
+            _adamw(s)
+        out = dict(p=s["p"], m=s["m"], v=s["v"])
+        if case["bits"] == 8:
+            out.update(ms=s["ms"], rs=s["rs"])
+        return out
+    if case["op"] == "product":
+        if own:
+            _ops().linear_q8(s["x"], s["w"], s["ws"], s["y"], s["q"], s["qs"], bias=s["bias"], lrelu=case["lrelu"])
+        else:
+            _product(s)
+        return dict(y=s["y"])
+    if case["out"] == "q8":
+        if own:
+            _ops().up_fold_q8(s["y"], s["shift"], s["q"], s["qs"])
+        else:
+            _fold(s)
+        return dict(q=s["q"], qs=s["qs"])
+    if own:
+        _ops().up_fold(s["y"], s["shift"], s["out"], {"linear": 0, "sites": 1, "tanh": 2}[case["out"]])
+    else:
+        _fold(s)
+    return dict(out=s["out"])
+
+
+def work(case):
+    if case["op"] == "adamw":
+        n = sum(_sizes(case))
+        state = 16 if case["bits"] == 32 else 4 + 16 / BLOCK
+        return {"bytes": n * (2 * BYTES[case["p"]] + BYTES[case["g"]] + state), "flops": 15 * n}
+    if case["op"] == "product":
+        T, K, N = case["T"], case["K"], case["N"]
+        return {"bytes": T * K * BYTES[case["x"]] + N * K + 4 * N * (2 if case["bias"] else 1) + T * N * BYTES[case["y"]],
+                "flops": 2 * T * K * N}
+    n, C = case["B"] * case["H"] * case["W"], case["C"]
+    out = 4 * n * (C + 4) if case["out"] == "q8" else 16 * n * C
+    return {"bytes": 16 * n * C * BYTES[case["y"]] + 4 * C + out, "flops": 24 * n * C}
+
+
+# ---- the definitions in 64 bits ------------------------------------------------------------------------------------
+def _exact_adamw(case, s):
+    step = STEP + 1
+    out = dict(p=[], m=[], v=[], ms=None, rs=None)
+    for i, (p, g, a, n) in enumerate(zip(s["p"], s["g"], s["at"], s["sizes"])):
+        h = -(-n // BLOCK) * BLOCK
+        p, g = p.double(), F.pad(g.double(), (0, h - n))
+        m, v = s["m"][a:a + h].double(), s["v"][a:a + h].double()
+        if case["bits"] == 8:
+            b = slice(a // BLOCK, (a + h) // BLOCK)
+            m = (m.view(-1, BLOCK) * s["ms"][b, None].double()).view(-1)
+            v = (v.view(-1, BLOCK) * s["rs"][b, None].double()).view(-1).square()
+        m, v = B1 * m + (1 - B1) * g, B2 * v + (1 - B2) * g * g
+        mhat, vhat = m / (1 - B1 ** step), v / (1 - B2 ** step)
+        out["p"].append(p - LR * DECAY * p - LR * (mhat / (vhat.sqrt() + EPS))[:n])
+        if case["bits"] == 8:
+            number = lambda x: ((x ^ (x >> 16)) * 0x6A09E667) & M32             # noqa: E731
+            second = lambda x: ((x ^ (x >> 15)) * 0xBB67AE85) & M32             # noqa: E731
+            mix = lambda x: (lambda z: z ^ (z >> 16))(second(number(x)))        # noqa: E731
+            key = mix(torch.tensor((SEED8 + step * 0xA54FF53B + i * 0x3C6EF373) & M32, device=DEV))
+            bits = mix(key ^ torch.arange(h, device=DEV))
+
+            def rounded(x, top, low, u, least):
+                """x / 2^e held with three bits of mantissa and a smallest step of 2^-9, rounded up where the rest
+                exceeds 1 - u."""
+                e = torch.floor(torch.log2(top.clamp_min(2.0 ** -1000))).clamp_min(low) - 7
+                z = x.abs().view(-1, BLOCK) / torch.exp2(e)[:, None]
+                q = torch.exp2(torch.floor(torch.log2(z.clamp_min(2.0 ** -6))) - 3)
+                k = torch.maximum(torch.floor(z / q + (u.view(-1, BLOCK).double() + 0.5) / 65536) * q, least * 2.0 ** -9)
+                return (torch.sign(x).view(-1, BLOCK) * k).view(-1)
+            out["m"].append(rounded(m, m.abs().view(-1, BLOCK).amax(1), -100, bits & 0xFFFF, 0.0 * m.view(-1, BLOCK)))
+            r = v.sqrt()
+            out["v"].append(rounded(r, r.view(-1, BLOCK).amax(1), -63, bits >> 16, (v > 0).double().view(-1, BLOCK)))
+        else:
+            out["m"].append(m)
+            out["v"].append(v)
+    out["m"], out["v"] = torch.cat(out["m"]), torch.cat(out["v"])
+    if case["bits"] == 32:
+        del out["ms"], out["rs"]
+    return out
+
+
+def _exact_codes(x):
+    """The codes by their definition: the fp32 quotient 127 / maximum times the fp32 value, rounded to fp32 and then to the
+    nearest whole number."""
+    top = x.abs().max(dim=1).values.clamp_min(2.0 ** -100)
+    inv = (127.0 / top).float().double()
+    return torch.round((x * inv[:, None]).float().double()), top * (1 / 127)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "adamw":
+        return _exact_adamw(case, s)
+    if case["op"] == "product":
+        x = s["x"].double()
+        if case["lrelu"]:
+            x = torch.where(x > 0, x, (x * float(torch.tensor(0.1))).float().double())
+        q, qs = _exact_codes(x)
+        y = torch.einsum("tk,nk->tn", q, s["w"].double()) * qs[:, None] * s["ws"].double()
+        return dict(y=y if s["bias"] is None else y + s["bias"].double())
+    B, H, W, C = case["B"], case["H"], case["W"], case["C"]
+    wide = torch.zeros(B, 2 * H + 2, 2 * W + 2, C, dtype=torch.float64, device=DEV)     # a border takes what falls outside
+    t = s["y"].double().view(B, H, W, 4, 4, C)
+    for kh in range(4):
+        for kw in range(4):
+            wide[:, kh:kh + 2 * H:2, kw:kw + 2 * W:2] += t[:, :, :, kh, kw]
+    o = wide[:, 1:-1, 1:-1] + s["shift"].double()
+    if case["out"] != "q8":
+        return dict(out=1 / (1 + torch.exp(-o)) if case["out"] == "sites" else torch.tanh(o) if case["out"] == "tanh" else o)
+    o = torch.where(o > 0, o, o * 0.1).reshape(-1, C)
+    return dict(q=None, qs=o.abs().max(dim=1).values.clamp_min(2.0 ** -100) / 127)

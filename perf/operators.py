@@ -122,6 +122,8 @@ def prepare(case, seed):
             s["m"], s["v"] = m, v
         s["m_of"] = [s["m"][a:a + n] for a, n in zip(at, sizes)]
         s["v_of"] = [s["v"][a:a + n] for a, n in zip(at, sizes)]
+        if own:                                                 # the handle that an optimizer keeps
+            s["plan"] = _ops().adamw_plan(s["p"], s["m_of"], s["v_of"], scales=(s["mss"], s["rss"]) if case["bits"] == 8 else None)
         return s
     if case["op"] == "product":
         T, K, N = case["T"], case["K"], case["N"]
@@ -269,8 +271,7 @@ def run(s):
     if case["op"] == "adamw":
         if own:
             s["step"] += 1
-            _ops().adamw(s["p"], s["g"], s["m_of"], s["v_of"], s["step"], LR, B1, B2, EPS, DECAY,
-                         scales=(s["mss"], s["rss"]) if case["bits"] == 8 else None, seed=SEED8)
+            s["plan"].step(s["g"], s["step"], LR, B1, B2, EPS, DECAY, seed=SEED8)
         else:
             _adamw(s)
         out = dict(p=s["p"], m=s["m"], v=s["v"])

@@ -259,6 +259,20 @@ int pgan_zero_multi(void* const* bufs, const long long* bytes, int n, hipStream_
 int pgan_adam(float* p, const float* g, float* m, float* v, long long n, float lr, float b1, float b2, float eps,
               float grad_scale, int* step_dev, int step, hipStream_t st);
 
+/* torch.optim.AdamW step over n tensors (host arrays of n device pointers and n values each; tensors of no elements are
+ * passed over): per tensor its elements, its types (type of p + 3 * type of g; 0 fp32, 1 bf16, 2 fp16), learning rate and
+ * weight decay.  bits 32: m and v are fp32.  bits 8: m and v hold e4m3 codes of m and of sqrt(v), one byte an element, and
+ * m_scale / r_scale one power of two for every 256 elements (codes and scales of zeros are a fresh state); codes are rounded
+ * stochastically from a hash of (seed, step, tensor's number, element).  Elements past a tensor's last one are left alone.
+ * Refused (-1): two written buffers that share memory, pointers that are not aligned to their element.
+ * step_dev: NULL (step >= 1 is the number of this step), or 4 device ints: [0] is incremented and used, [1] and [2] get the
+ * corrections 1 / (1 - b1^t) and 1 / sqrt(1 - b2^t) as fp32 -- a captured graph then counts on every replay.
+ * grad_scale as in pgan_adam.  (src/train_wgan_v2.py:489-490,612,634 step torch.optim.Adam.) */
+int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
+                     float* const* r_scale, const long long* numel, const int* types, const double* lr,
+                     const double* decay, int n, int bits, double b1, double b2, float eps, float grad_scale, int seed,
+                     int* step_dev, int step, hipStream_t st);
+
 /* Philox4x32-10 draws replacing torch.randn (src/train_wgan_v2.py:534,621) and np.random.random
  * (src/layers.py:37).  state: 4 uint32 on the device (seed lo, hi, offset lo, hi), advanced by the call. */
 int pgan_philox(float* out, long long n, unsigned int* state, int normal, hipStream_t st);
@@ -324,6 +338,31 @@ int pgan_ct1d_wgrad(const float* ya, const float* x, float* dw, int N, int Cs, i
  * ConvTranspose layers on a 1x1 / length-1 input (src/layers.py:92,117) and their weight gradients. */
 int pgan_gemm(const float* A, const float* B, float* C, int M, int N, int K, int transa, hipStream_t st);
 
+/* ---- products of 8-bit rows with a scale for each token and channel, for drawing alignments from a trained generator
+ * (its ConvTranspose2d stacks, src/layers.py:91-147, in evaluation; no backward).  Types: 0 fp32, 1 bf16, 2 fp16; strides
+ * in elements; no rows (T, rows, B = 0): nothing is launched.
+ * pgan_quant_rows: q[r][k] = rint(x[r][k] * 127 / max_k |x[r][k]|), scale[r] = max / 127, after LeakyReLU(0.1) of x when
+ *   lrelu is set; bytes past K of a row of q are left alone.  A row with an infinity or a NaN: codes 0, scale NaN.
+ * pgan_gemm_q8: y[t][n] = q_scale[t] w_scale[n] sum_k q[t][k] w[n][k] + bias[n] (bias may be NULL), K <= 131072.  Rows of q
+ *   and w start on 16-byte borders (base and stride) and are readable up to the next multiple of 16 past K; what stands
+ *   there does not matter.
+ * pgan_linear_q8: both, through the caller's q (T rows of stride ldq) and q_scale.
+ * pgan_up_fold_q8 / pgan_up_fold: the end of ConvTranspose2d(k 4, stride 2, padding 1) (src/layers.py:97-115) made as a
+ *   product whose channels are (kh, kw, c): y[B][H][W][4][4][C] -> [B][2H][2W][C] = sum of the up to four taps + shift[c]
+ *   (NULL: none); then LeakyReLU(0.1) and pgan_quant_rows' codes (one row a pixel), or fp32 through act 0 none, 1 sigmoid,
+ *   2 tanh. */
+int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long ldq, float* scale, long long rows, int K,
+                    int lrelu, hipStream_t st);
+int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
+                 const float* bias, void* y, int y_type, long long ldy, long long T, int N, int K, hipStream_t st);
+int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long ldq, float* q_scale, const void* w,
+                   long long ldw, const float* w_scale, const float* bias, void* y, int y_type, long long ldy, long long T,
+                   int N, int K, int lrelu, hipStream_t st);
+int pgan_up_fold_q8(const void* y, int y_type, const float* shift, void* q, long long ldq, float* scale, int B, int H, int W,
+                    int C, hipStream_t st);
+int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int B, int H, int W, int C, int act,
+                 hipStream_t st);
+
 /* ---- input pipeline: the reference's alignment files (`<n>_sites.csv`, 64 lines of 64 comma-separated 0/1,
  * src/sim_conversion/convert_ms.py:39; `<n>_pos.csv`, 64 lines of one float, convert_ms.py:28-29) parsed natively into
  * bit-packed form (replaces the two np.loadtxt calls per alignment of DataGeneratorDisk.get_batch,
@@ -384,7 +423,7 @@ int pgan_stream_edge(void* ev, hipStream_t from, hipStream_t to);
 /* ---- launch tape: one iteration's enqueue calls (the loop body of src/train_wgan_v2.py:516-634, which the reference
  * drives op by op from Python) noted once and replayed by one call.  pgan_tape_append notes a call of the named entry
  * point of this header (enqueue entry points only) with one 64-bit word per argument in declaration order: integers
- * sign-extended, pointers as addresses, floats as their 32 bits in the low half; host arrays an argument points to
+ * sign-extended, pointers as addresses, floats as their 32 bits in the low half, doubles as their 64; host arrays an argument points to
  * must stay alive as long as the tape.  pgan_tape_replay makes the calls in order; it stops at the first one that does
  * not return 0, stores its index in *failed_at (may be NULL) and returns that call's code.  pgan_tape_arg_count: words
  * the named entry point takes, -1 if it cannot be noted. */

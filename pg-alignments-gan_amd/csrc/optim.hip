@@ -1,0 +1,388 @@
+// AdamW over many tensors in one launch, its two states in 32 or in 8 bits (torch.optim.AdamW semantics; the reference
+// steps its networks with torch.optim.Adam, src/train_wgan_v2.py:489-490,612,634).
+//
+//   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// States in 8 bits: blocks of 256 elements of a tensor, each with two power-of-two scales that bring the block's largest
+// magnitudes into [128, 256); m and sqrt(v) are held as e4m3 codes (four exponent bits, three of mantissa) of the scaled
+// value.  A power of two costs nothing of a floating code's relative precision and makes scaling exact.  Codes are rounded
+// stochastically: at b2 = 0.999 a step changes v by 0.1 % or less while neighbouring codes are 6 to 12 % apart, so rounding
+// to the nearest would leave v where it is for ever.  The random bits are a hash of (seed, step, tensor, place): a step is
+// reproducible and nothing depends on the launch's shape.  A root that is not zero never becomes zero (its code is at least
+// 1): a zero denominator beside an m that survived its own rounding would throw the parameter off by m / eps.  A state that
+// is not finite is held as NaN, as it would poison the element in 32 bits too; it does not touch its block's scale.
+//
+// Bound by HBM: 28 bytes an element with fp32 states, 16 with 8-bit ones.
+#include <algorithm>
+#include <vector>
+
+#include "../../include/pgan_hip.h"
+#include "pgan_common.h"
+
+// Products and sums are rounded one by one, as the formulas are written: a code's rounding is then the same wherever the
+// formulas are evaluated in fp32.  The kernels wait for memory either way.
+#pragma clang fp contract(off)
+
+namespace {
+
+constexpr int AW_MAX = 40;          // tensors per launch: what fits the kernel arguments (4 KiB)
+constexpr int AW_CHUNK = 2048;      // elements of a tensor per block of 256 threads
+constexpr int AW_BLOCK = 256;       // elements that share a scale
+constexpr long long AW_MOST = 0xffffff;      // blocks per launch (fewer than 2^32 threads)
+
+struct AwTensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;
+    float* rs;
+    long long n;
+    float size;                     // lr / (1 - b1^t); lr alone where the step count lives on the device
+    float keep;                     // 1 - lr wd
+    int types;                      // p type + 3 * g type, + 16 where every pointer allows vector accesses
+    int index;                      // number of the tensor in the caller's list
+};
+struct AwArgs {
+    AwTensor t[AW_MAX];
+    unsigned first[AW_MAX];         // first chunk of each tensor
+    const int* step_dev;
+    int n, step;
+    float b1, c1, b2, c2, eps, gs, inv2;
+    unsigned seed;
+};
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x6A09E667u;
+    x = (x ^ (x >> 15)) * 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ float from16(uint16_t u, int type) {
+    return type == 1 ? __builtin_bit_cast(float, (uint32_t)u << 16) : (float)__builtin_bit_cast(_Float16, u);
+}
+__device__ __forceinline__ uint16_t to16(float x, int type) {
+    if (type == 1) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        return x != x ? (uint16_t)((u >> 16) | 0x40u) : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+    }
+    return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// four elements of a tensor from i on; VEC: one access, else those below n one by one
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load4(const void* src, long long i, long long n, float (&o)[4]) {
+    if constexpr (TYPE == 0) {
+        const float* s = static_cast<const float*>(src);
+        if constexpr (VEC) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(s + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = x[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = i + e < n ? s[i + e] : 0.f;
+        }
+    } else {
+        const uint16_t* s = static_cast<const uint16_t*>(src);
+        if constexpr (VEC) {
+            const uint2 x = *reinterpret_cast<const uint2*>(s + i);
+            o[0] = from16((uint16_t)x.x, TYPE);
+            o[1] = from16((uint16_t)(x.x >> 16), TYPE);
+            o[2] = from16((uint16_t)x.y, TYPE);
+            o[3] = from16((uint16_t)(x.y >> 16), TYPE);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = i + e < n ? from16(s[i + e], TYPE) : 0.f;
+        }
+    }
+}
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void store4(void* dst, long long i, long long n, const float (&o)[4]) {
+    if constexpr (TYPE == 0) {
+        float* d = static_cast<float*>(dst);
+        if constexpr (VEC) {
+            *reinterpret_cast<f32x4*>(d + i) = f32x4{o[0], o[1], o[2], o[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) d[i + e] = o[e];
+        }
+    } else {
+        uint16_t* d = static_cast<uint16_t*>(dst);
+        if constexpr (VEC) {
+            uint2 x;
+            x.x = (uint32_t)to16(o[0], TYPE) | (uint32_t)to16(o[1], TYPE) << 16;
+            x.y = (uint32_t)to16(o[2], TYPE) | (uint32_t)to16(o[3], TYPE) << 16;
+            *reinterpret_cast<uint2*>(d + i) = x;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) d[i + e] = to16(o[e], TYPE);
+        }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ uint32_t load_codes(const void* src, long long i, long long n) {
+    const uint8_t* s = static_cast<const uint8_t*>(src);
+    if constexpr (VEC) return *reinterpret_cast<const uint32_t*>(s + i);
+    uint32_t u = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) u |= (uint32_t)s[i + e] << (8 * e);
+    return u;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_codes(void* dst, long long i, long long n, uint32_t u) {
+    uint8_t* d = static_cast<uint8_t*>(dst);
+    if constexpr (VEC) {
+        *reinterpret_cast<uint32_t*>(d + i) = u;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) d[i + e] = (uint8_t)(u >> (8 * e));
+    }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = __builtin_fmaxf(v, dpp_move<0xB1>(v));
+    v = __builtin_fmaxf(v, dpp_move<0x4E>(v));
+    v = __builtin_fmaxf(v, dpp_move<0x141>(v));
+    v = __builtin_fmaxf(v, dpp_move<0x140>(v));
+    v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
+    return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127; }
+__device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) != 0x7f800000u; }
+
+// e4m3 code of y in [0, 256), u in [0, 2^16): the low 20 bits of the fp32 pattern are the part of a step that is decided by
+// the random bits.  Below the smallest normal code the steps are even: adding 2^-6 there gives the pattern the same form.
+__device__ __forceinline__ uint32_t encode(float y, uint32_t u) {
+    const bool small = y < 0x1p-6f;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, small ? y + 0x1p-6f : y);
+    return ((bits + (u << 4) + 8u) >> 20) - (small ? 968u : 960u);
+}
+
+struct AwStep {
+    float size, keep, b1, c1, b2, c2, eps, gs, inv2;
+};
+__device__ __forceinline__ void update(const AwStep& s, float& p, float g, float& m, float& v, float& root) {
+    g = g * s.gs;
+    m = m * s.b1 + g * s.c1;
+    v = v * s.b2 + (g * g) * s.c2;
+    root = sqrtf(v);
+    p = p * s.keep - (m * s.size) / (root * s.inv2 + s.eps);
+}
+
+template <int PT, int GT, bool VEC>
+__device__ __forceinline__ void body32(const AwTensor& t, const AwStep& s, long long i) {
+    float p[4], g[4], m[4], v[4], root;
+    load4<PT, VEC>(t.p, i, t.n, p);
+    load4<GT, VEC>(t.g, i, t.n, g);
+    load4<0, VEC>(t.m, i, t.n, m);
+    load4<0, VEC>(t.v, i, t.n, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) update(s, p[e], g[e], m[e], v[e], root);
+    store4<PT, VEC>(t.p, i, t.n, p);
+    store4<0, VEC>(t.m, i, t.n, m);
+    store4<0, VEC>(t.v, i, t.n, v);
+}
+
+// one block of 256 elements by one wave, four elements a lane; i: the lane's first element
+template <int PT, int GT, bool VEC>
+__device__ __forceinline__ void body8(const AwTensor& t, const AwStep& s, long long i, uint32_t key) {
+    const long long blk = i / AW_BLOCK;
+    float p[4], g[4], m[4], v[4], r[4];
+    load4<PT, VEC>(t.p, i, t.n, p);
+    load4<GT, VEC>(t.g, i, t.n, g);
+    const uint32_t cm = load_codes<VEC>(t.m, i, t.n), cv = load_codes<VEC>(t.v, i, t.n);
+    const float ms = t.ms[blk], rs = t.rs[blk];
+    m[0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0) * ms;
+    m[1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1) * ms;
+    m[2] = __builtin_amdgcn_cvt_f32_fp8(cm, 2) * ms;
+    m[3] = __builtin_amdgcn_cvt_f32_fp8(cm, 3) * ms;
+    v[0] = __builtin_amdgcn_cvt_f32_fp8(cv, 0) * rs;
+    v[1] = __builtin_amdgcn_cvt_f32_fp8(cv, 1) * rs;
+    v[2] = __builtin_amdgcn_cvt_f32_fp8(cv, 2) * rs;
+    v[3] = __builtin_amdgcn_cvt_f32_fp8(cv, 3) * rs;
+    float mmax = 0.f, vmax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = v[e] * v[e];
+        update(s, p[e], g[e], m[e], v[e], r[e]);
+        if (finite(m[e])) mmax = __builtin_fmaxf(mmax, __builtin_fabsf(m[e]));
+        if (finite(v[e])) vmax = __builtin_fmaxf(vmax, v[e]);
+    }
+    store4<PT, VEC>(t.p, i, t.n, p);
+    mmax = wave_max(mmax);
+    vmax = wave_max(vmax);
+    const int em = max(exponent(mmax), -100) - 7, er = (max(exponent(vmax), -126) >> 1) - 7;
+    const float im = pow2(-em), ir = pow2(-er);
+    uint32_t nm = 0, nr = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t h = mix(key ^ (uint32_t)(i + e));
+        uint32_t a = encode(__builtin_fabsf(m[e]) * im, h & 0xffffu);
+        uint32_t b = encode(r[e] * ir, h >> 16);
+        b = (v[e] > 0.f && b == 0) ? 1u : b;
+        a = finite(m[e]) ? a : 0x7fu;
+        b = finite(v[e]) ? b : 0x7fu;
+        nm |= (a | (__builtin_bit_cast(uint32_t, m[e]) >> 31) << 7) << (8 * e);
+        nr |= b << (8 * e);
+    }
+    store_codes<VEC>(t.m, i, t.n, nm);
+    store_codes<VEC>(t.v, i, t.n, nr);
+    if ((threadIdx.x & 63) == 0) {
+        t.ms[blk] = pow2(em);
+        t.rs[blk] = pow2(er);
+    }
+}
+
+template <int BITS, int PT, int GT>
+__device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long long at, bool vec, uint32_t key) {
+    if constexpr (BITS == 32) {
+#pragma unroll
+        for (int u = 0; u < AW_CHUNK / 1024; ++u) {
+            const long long i = at + u * 1024 + threadIdx.x * 4;
+            if (i >= t.n) continue;
+            if (vec && i + 4 <= t.n) body32<PT, GT, true>(t, s, i);
+            else body32<PT, GT, false>(t, s, i);
+        }
+    } else {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < AW_CHUNK / 1024; ++u) {
+            const long long b = at + u * 1024 + wave * AW_BLOCK;        // the same for all lanes of the wave
+            if (b >= t.n) continue;
+            if (vec && b + AW_BLOCK <= t.n) body8<PT, GT, true>(t, s, b + lane * 4, key);
+            else body8<PT, GT, false>(t, s, b + lane * 4, key);
+        }
+    }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const AwArgs a) {
+    int k = 0;
+    for (int i = 1; i < a.n; ++i) k = blockIdx.x >= a.first[i] ? i : k;
+    const AwTensor& t = a.t[k];
+    const long long at = (long long)(blockIdx.x - a.first[k]) * AW_CHUNK;
+    AwStep s{t.size, t.keep, a.b1, a.c1, a.b2, a.c2, a.eps, a.gs, a.inv2};
+    uint32_t step = (uint32_t)a.step;
+    if (a.step_dev) {
+        step = (uint32_t)a.step_dev[0];
+        s.size = t.size * __builtin_bit_cast(float, a.step_dev[1]);
+        s.inv2 = __builtin_bit_cast(float, a.step_dev[2]);
+    }
+    const uint32_t key = BITS == 8 ? mix(a.seed + step * 0xA54FF53Bu + (uint32_t)t.index * 0x3C6EF373u) : 0u;
+    const bool vec = t.types >= 16;
+    switch (t.types & 15) {
+        case 0: chunk<BITS, 0, 0>(t, s, at, vec, key); break;
+        case 1: chunk<BITS, 1, 0>(t, s, at, vec, key); break;
+        case 2: chunk<BITS, 2, 0>(t, s, at, vec, key); break;
+        case 3: chunk<BITS, 0, 1>(t, s, at, vec, key); break;
+        case 4: chunk<BITS, 1, 1>(t, s, at, vec, key); break;
+        case 5: chunk<BITS, 2, 1>(t, s, at, vec, key); break;
+        case 6: chunk<BITS, 0, 2>(t, s, at, vec, key); break;
+        case 7: chunk<BITS, 1, 2>(t, s, at, vec, key); break;
+        default: chunk<BITS, 2, 2>(t, s, at, vec, key); break;
+    }
+}
+
+// counter[0] += 1; counter[1], [2] = 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) as fp32 patterns
+__global__ void adamw_tick_kernel(int* counter, double b1, double b2) {
+    const int t = counter[0] + 1;
+    counter[0] = t;
+    counter[1] = __builtin_bit_cast(int, (float)(1.0 / (1.0 - pow(b1, (double)t))));
+    counter[2] = __builtin_bit_cast(int, (float)(1.0 / sqrt(1.0 - pow(b2, (double)t))));
+}
+
+inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+struct Span {
+    uintptr_t lo, hi;
+};
+
+}  // namespace
+
+extern "C" {
+
+int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
+                     float* const* r_scale, const long long* numel, const int* types, const double* lr,
+                     const double* decay, int n, int bits, double b1, double b2, float eps, float grad_scale, int seed,
+                     int* step_dev, int step, hipStream_t st) {
+    if (n < 0 || (bits != 32 && bits != 8) || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1) || !(eps >= 0)) return PGAN_EINVAL;
+    if (!step_dev && step < 1) return PGAN_EINVAL;
+    if (n > 0 && (!p || !g || !m || !v || !numel || !types || !lr || !decay)) return PGAN_EINVAL;
+    if (bits == 8 && n > 0 && (!m_scale || !r_scale)) return PGAN_EINVAL;
+    const int size_of[3] = {4, 2, 2};
+    try {
+        // what is written: no two of these may share memory (the same tensor twice in the lists, a state for two of them)
+        std::vector<Span> out;
+        out.reserve((size_t)n * 5);
+        for (int i = 0; i < n; ++i) {
+            if (numel[i] < 0 || numel[i] > AW_MOST * AW_CHUNK || types[i] < 0 || types[i] > 8) return PGAN_EINVAL;
+            if (numel[i] == 0) continue;
+            if (!p[i] || !g[i] || !m[i] || !v[i] || (bits == 8 && (!m_scale[i] || !r_scale[i]))) return PGAN_EINVAL;
+            const int ps = size_of[types[i] % 3], gsz = size_of[types[i] / 3];
+            if (!aligned(p[i], ps) || !aligned(g[i], gsz)) return PGAN_EINVAL;
+            if (bits == 32 && (!aligned(m[i], 4) || !aligned(v[i], 4))) return PGAN_EINVAL;
+            const auto add = [&out](const void* q, long long bytes) {
+                const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
+                out.push_back(Span{lo, lo + (uintptr_t)bytes});
+            };
+            add(p[i], numel[i] * ps);
+            add(m[i], numel[i] * (bits / 8));
+            add(v[i], numel[i] * (bits / 8));
+            if (bits == 8) {
+                const long long nb = (numel[i] + AW_BLOCK - 1) / AW_BLOCK * 4;
+                add(m_scale[i], nb);
+                add(r_scale[i], nb);
+            }
+        }
+        std::sort(out.begin(), out.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
+        for (size_t i = 1; i < out.size(); ++i)
+            if (out[i].lo < out[i - 1].hi) return PGAN_EINVAL;
+    } catch (...) {
+        return PGAN_EINVAL;
+    }
+    if (step_dev) adamw_tick_kernel<<<1, 1, 0, st>>>(step_dev, b1, b2);
+    AwArgs a;
+    a.step_dev = step_dev;
+    a.step = step;
+    a.b1 = (float)b1;
+    a.c1 = (float)(1.0 - b1);
+    a.b2 = (float)b2;
+    a.c2 = (float)(1.0 - b2);
+    a.eps = eps;
+    a.gs = grad_scale;
+    a.seed = (unsigned)seed;
+    const double bc1 = step_dev ? 1.0 : 1.0 - pow(b1, (double)step);
+    a.inv2 = step_dev ? 1.f : (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
+    int i = 0;
+    while (i < n) {
+        a.n = 0;
+        long long chunks = 0;
+        for (; i < n && a.n < AW_MAX; ++i) {
+            if (numel[i] == 0) continue;
+            const long long c = (numel[i] + AW_CHUNK - 1) / AW_CHUNK;
+            if (chunks + c > AW_MOST) break;
+            const int pt = types[i] % 3, gt = types[i] / 3;
+            const bool vec = aligned(p[i], 4 * size_of[pt]) && aligned(g[i], 4 * size_of[gt])
+                             && aligned(m[i], bits / 2) && aligned(v[i], bits / 2);
+            a.first[a.n] = (unsigned)chunks;
+            a.t[a.n] = AwTensor{p[i], g[i], m[i], v[i], bits == 8 ? m_scale[i] : nullptr, bits == 8 ? r_scale[i] : nullptr,
+                                numel[i], (float)(lr[i] / bc1), (float)(1.0 - lr[i] * decay[i]), types[i] + (vec ? 16 : 0), i};
+            chunks += c;
+            ++a.n;
+        }
+        if (a.n == 0) break;
+        if (bits == 32) adamw_kernel<32><<<(unsigned)chunks, 256, 0, st>>>(a);
+        else adamw_kernel<8><<<(unsigned)chunks, 256, 0, st>>>(a);
+    }
+    return pgan_launch_status();
+}
+
+}  // extern "C"

@@ -24,7 +24,7 @@ namespace {
 std::atomic<long long> g_events_created{0};
 
 // ---- calling an entry point from an array of 64-bit words -------------------------------------------------------
-// One word per argument: integers sign-extended, pointers as addresses, floats as their 32 bits in the low half.
+// One word per argument: integers sign-extended, pointers as addresses, floats as their 32 bits in the low half, doubles as their 64.
 template <class T>
 inline T word_as(uint64_t w) {
     if constexpr (std::is_pointer_v<T>) {
@@ -34,6 +34,10 @@ inline T word_as(uint64_t w) {
         float f;
         std::memcpy(&f, &b, 4);
         return f;
+    } else if constexpr (std::is_same_v<T, double>) {
+        double d;
+        std::memcpy(&d, &w, 8);
+        return d;
     } else {
         static_assert(std::is_integral_v<T>, "argument kind");
         return static_cast<T>(static_cast<int64_t>(w));
@@ -72,6 +76,8 @@ const Entry ENTRIES[] = {
     PGAN_ENTRY(pgan_head_fwd), PGAN_ENTRY(pgan_head_seed), PGAN_ENTRY(pgan_head_wgrad),
     PGAN_ENTRY(pgan_interpolate), PGAN_ENTRY(pgan_gp_penalty), PGAN_ENTRY(pgan_div_penalty), PGAN_ENTRY(pgan_critic_loss),
     PGAN_ENTRY(pgan_sum_scale), PGAN_ENTRY(pgan_act_bwd), PGAN_ENTRY(pgan_affine), PGAN_ENTRY(pgan_zero_multi), PGAN_ENTRY(pgan_adam),
+    PGAN_ENTRY(pgan_adamw_multi), PGAN_ENTRY(pgan_quant_rows), PGAN_ENTRY(pgan_gemm_q8), PGAN_ENTRY(pgan_linear_q8),
+    PGAN_ENTRY(pgan_up_fold_q8), PGAN_ENTRY(pgan_up_fold),
     PGAN_ENTRY(pgan_philox), PGAN_ENTRY(pgan_philox_slice), PGAN_ENTRY(pgan_take_batch), PGAN_ENTRY(pgan_take_batch_slice),
     PGAN_ENTRY(pgan_label_smooth), PGAN_ENTRY(pgan_mono_switch),
     PGAN_ENTRY(pgan_d1d_fwd), PGAN_ENTRY(pgan_d1d_bwd), PGAN_ENTRY(pgan_d1d_fwd_len), PGAN_ENTRY(pgan_d1d_bwd_len),

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 from typing import List, Optional, Sequence
 
 import torch
@@ -43,7 +43,7 @@ def _load() -> ctypes.CDLL:
 
 _lib = _load()
 
-P, I, L, F = c_void_p, c_int, c_longlong, c_float
+P, I, L, F, D = c_void_p, c_int, c_longlong, c_float, c_double
 _SIGS = {
     "pgan_conv_down": [P, P, P, I, I, I, I, P],
     "pgan_conv_down_gn_sums": [P, P, P, I, I, I, I, P, L, P],
@@ -93,6 +93,12 @@ _SIGS = {
     "pgan_act_bwd": [P, P, P, L, I, P],
     "pgan_affine": [P, P, L, F, F, P],
     "pgan_adam": [P, P, P, P, L, F, F, F, F, F, P, I, P],
+    "pgan_adamw_multi": [P, P, P, P, P, P, P, P, P, P, I, I, D, D, F, F, I, P, I, P],
+    "pgan_quant_rows": [P, I, L, P, L, P, L, I, I, P],
+    "pgan_gemm_q8": [P, L, P, P, L, P, P, P, I, L, L, I, I, P],
+    "pgan_linear_q8": [P, I, L, P, L, P, P, L, P, P, P, I, L, L, I, I, I, P],
+    "pgan_up_fold_q8": [P, I, P, P, L, P, I, I, I, I, P],
+    "pgan_up_fold": [P, I, P, P, I, I, I, I, I, P],
     "pgan_philox": [P, L, P, I, P],
     "pgan_philox_slice": [P, L, L, L, P, I, P],
     "pgan_take_batch": [P, P, P, P, P, I, I, I, I, P],
@@ -250,6 +256,9 @@ def _arg_word(kind, v) -> int:
     if kind is c_float:
         import struct
         return struct.unpack("<I", struct.pack("<f", float(v)))[0]
+    if kind is c_double:
+        import struct
+        return struct.unpack("<Q", struct.pack("<d", float(v)))[0]
     if kind is c_void_p:
         if v is None:
             return 0
@@ -403,6 +412,96 @@ def _hw(t: torch.Tensor) -> int:
     return n
 
 
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # type codes of the C-ABI
+ADAMW_BLOCK = 256      # elements of an 8-bit AdamW state that share a scale
+
+
+def rows8(rows: int, cols: int, device) -> torch.Tensor:
+    """[rows, cols] int8 buffer for the codes of quant_rows / gemm_q8: rows start on 16-byte borders."""
+    return torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :cols]
+
+
+class AdamWPlan:
+    """What HipOps.adamw_plan returns: parameters and states of an AdamW step, checked once; step() makes one."""
+
+    def __init__(self, ops, params, m, v, scales):
+        n = len(params)
+        if len(m) != n or len(v) != n:
+            raise PganError(f"adamw: {n} parameters, {len(m)} and {len(v)} states")
+        self.bits = 32 if scales is None else 8
+        if scales is not None and (len(scales) != 2 or len(scales[0]) != n or len(scales[1]) != n):
+            raise PganError("adamw: states in 8 bits need two lists of scales, one tensor for each parameter")
+        held = torch.float32 if scales is None else torch.float8_e4m3fn
+        self.ops, self.n, ptypes = ops, n, []
+        for i, p in enumerate(params):
+            k = p.numel()
+            if p.dtype not in ELEMENT_TYPES:
+                raise PganError(f"adamw: parameters are float32, bfloat16 or float16, got {p.dtype}")
+            ops._here(p, f"adamw: parameter {i}")
+            if not p.is_contiguous():
+                raise PganError(f"adamw: parameter {i} is not contiguous")
+            for s in (m[i], v[i]):
+                ops._here(s, f"adamw: state {i}")
+                if s.dtype != held or s.numel() != k or not s.is_contiguous():
+                    raise PganError(f"adamw: state {i} must be a contiguous {held} tensor of {k} elements")
+            for s in () if scales is None else (scales[0][i], scales[1][i]):
+                ops._here(s, f"adamw: scale {i}")
+                if s.dtype != torch.float32 or s.numel() != -(-k // ADAMW_BLOCK) or not s.is_contiguous():
+                    raise PganError(f"adamw: scales {i} must be a contiguous float32 tensor of {-(-k // ADAMW_BLOCK)} elements")
+            ptypes.append(ELEMENT_TYPES[p.dtype])
+        alive = lambda ts: [t.detach() for t in ts]      # the plan keeps the memory that its pointers refer to
+        self.params, self.m, self.v = alive(params), alive(m), alive(v)
+        self.scales = None if scales is None else (alive(scales[0]), alive(scales[1]))
+        self.sizes, self._ptypes = [p.numel() for p in params], ptypes
+        self._pt, self._dt, self._it = c_void_p * n, c_double * n, c_int * n
+        ptrs = lambda ts: self._pt(*[t.data_ptr() for t in ts])
+        self._p, self._m, self._v = ptrs(params), ptrs(m), ptrs(v)
+        self._ms, self._rs = (None, None) if scales is None else (ptrs(scales[0]), ptrs(scales[1]))
+        self._numel = (c_longlong * n)(*self.sizes)
+        self._rates = (None, None, None, None)
+        self._types = (None, None)
+
+    def _per_tensor(self, x, what):
+        if isinstance(x, (int, float)):
+            return self._dt(*[x] * self.n)
+        if len(x) != self.n:
+            raise PganError(f"adamw: {len(x)} values of {what} for {self.n} tensors")
+        return self._dt(*x)
+
+    def step(self, grads, step, lr, b1, b2, eps, weight_decay=0.0, seed=0, step_dev=None, grad_scale=1.0) -> None:
+        """One step with `grads` (one for each parameter, float32, bfloat16 or float16), the step's number counted from
+        1 -- or step_dev, an int32[4] device tensor that counts by itself ([0] holds the steps made).  lr and
+        weight_decay: a number, or one for each tensor.  seed: of the rounding of 8-bit states."""
+        ops = self.ops
+        if len(grads) != self.n:
+            raise PganError(f"adamw: {len(grads)} gradients for {self.n} parameters")
+        dev, kinds, gp = ops._device, [], []
+        for g, k in zip(grads, self.sizes):
+            if g.device != dev or g.numel() != k or not g.is_contiguous():
+                raise PganError(f"adamw: a gradient must be a contiguous tensor of its parameter's {k} elements on {dev}, got "
+                                f"{tuple(g.shape)} on {g.device}, contiguous: {g.is_contiguous()}")
+            kinds.append(g.dtype)
+            gp.append(g.data_ptr())
+        if kinds != self._types[0]:
+            try:
+                self._types = (kinds, self._it(*[p + 3 * ELEMENT_TYPES[k] for p, k in zip(self._ptypes, kinds)]))
+            except KeyError as e:
+                raise PganError(f"adamw: gradients are float32, bfloat16 or float16, got {e}") from None
+        if self._rates[0] is None or self._rates[0] != lr or self._rates[1] != weight_decay:
+            self._rates = (lr, weight_decay, self._per_tensor(lr, "lr"), self._per_tensor(weight_decay, "weight_decay"))
+        sd = None
+        if step_dev is not None:
+            if step_dev.device != dev or step_dev.dtype != torch.int32 or step_dev.numel() < 4 or not step_dev.is_contiguous():
+                raise PganError("adamw: step_dev must be a contiguous int32 tensor of 4 elements on the device")
+            sd = step_dev.data_ptr()
+        elif step < 1:
+            raise PganError(f"adamw: steps count from 1, got {step}")
+        _check(_lib.pgan_adamw_multi(self._p, self._pt(*gp), self._m, self._v, self._ms, self._rs, self._numel, self._types[1],
+                                     self._rates[2], self._rates[3], self.n, self.bits, b1, b2, eps, grad_scale,
+                                     (seed + (1 << 31)) % (1 << 32) - (1 << 31), sd, int(step), ops._own_stream()),
+               "pgan_adamw_multi")
+
+
 D1_PACKED = (64, 16, 16, 16, 2048, 32, 32, 32, 8192, 64, 64, 64)   # cw cb gw gb per 1-D stage
 
 
@@ -417,6 +516,8 @@ class HipOps:
             raise PganError("HipOps needs a GPU")
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         _DEVICE_INDEX[0] = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self._index = _DEVICE_INDEX[0]
+        self._device = torch.device("cuda", self._index)
         self.ws = torch.empty(ws_floats, dtype=torch.float32, device=self.device)
         self.ws_small = torch.empty(4096, dtype=torch.float32, device=self.device)
         self.d1_part = torch.zeros(max_samples * 16384, dtype=torch.float32, device=self.device)  # gaps stay 0
@@ -887,6 +988,29 @@ class HipOps:
         _check(_lib.pgan_adam(_ptr(p), _ptr(g), _ptr(m), _ptr(v), p.numel(), lr, b1, b2, eps, float(grad_scale), sd,
                               int(step), _stream()), "pgan_adam")
 
+    def _own_stream(self):
+        """The current stream of this backend's device, which has to be the current device: a kernel for another
+        device's stream cannot be launched."""
+        if torch.cuda.current_device() != self._index:
+            raise PganError(f"the current device is cuda:{torch.cuda.current_device()}, this backend works on {self._device}")
+        return _raw_stream(self._index) if _raw_stream is not None else torch.cuda.current_stream(self._index).cuda_stream
+
+    def _here(self, t, what):
+        if t.device != self._device:
+            raise PganError(f"{what} is on {t.device}, this backend works on {self._device}")
+
+    def adamw_plan(self, params, m, v, scales=None) -> AdamWPlan:
+        """AdamW over many tensors in one launch: contiguous parameters (float32, bfloat16 or float16, mixed as they come)
+        and their states -- float32, or with scales = (list, list) in 8 bits: m[i] and v[i] float8_e4m3fn codes of m and of
+        sqrt(v), scales[0][i] and scales[1][i] float32 with one entry for every ADAMW_BLOCK elements; zeros are a fresh
+        state.  The plan is kept as long as the tensors are; its step() takes the gradients."""
+        return AdamWPlan(self, list(params), list(m), list(v), scales)
+
+    def adamw(self, params, grads, m, v, step, lr, b1, b2, eps, weight_decay=0.0, scales=None, seed=0, step_dev=None,
+              grad_scale=1.0) -> None:
+        """One AdamW step without a plan (see adamw_plan, which saves the checks of every later step)."""
+        self.adamw_plan(params, m, v, scales).step(grads, step, lr, b1, b2, eps, weight_decay, seed, step_dev, grad_scale)
+
     def philox(self, out, state, normal: bool, skip: int = 0, total: Optional[int] = None):
         """out = values [skip, skip + out.numel()) of a draw of `total` values (default: the whole draw); the state
         advances by the whole draw."""
@@ -1012,6 +1136,142 @@ class HipOps:
         N = b.shape[1]
         assert b.shape[0] == K and tuple(c.shape) == (M, N)
         _check(_lib.pgan_gemm(_ptr(a), _ptr(b), _ptr(c), M, N, K, 1, _stream()), "pgan_gemm")
+
+    # ---------------- products of 8-bit rows (evaluation only: no backward) ----------------
+    def _float_rows(self, t, what):
+        """(pointer, type code, row stride) of a 2-D view with contiguous rows."""
+        self._here(t, what)
+        if t.dtype not in ELEMENT_TYPES or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise PganError(f"{what}: expected a 2-D float32, bfloat16 or float16 tensor with contiguous rows, got "
+                            f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+        if ld < t.shape[1]:
+            raise PganError(f"{what}: rows overlap (stride {ld} for {t.shape[1]} columns)")
+        return t.data_ptr(), ELEMENT_TYPES[t.dtype], ld
+
+    def _code_rows(self, t, what, rows, cols):
+        """(pointer, row stride) of 8-bit rows: on 16-byte borders, readable up to a multiple of 16."""
+        self._here(t, what)
+        if t.dtype != torch.int8 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
+            raise PganError(f"{what}: expected int8 rows [{rows}, {cols}], got {t.dtype} {tuple(t.shape)} with strides "
+                            f"{t.stride()}")
+        wide = (cols + 15) // 16 * 16
+        ld = t.stride(0) if t.shape[0] > 1 else wide
+        if t.data_ptr() % 16 or ld % 16 or ld < cols:
+            raise PganError(f"{what}: rows must start on 16-byte borders (pgan_hip.rows8 makes such a buffer)")
+        if rows and t.storage_offset() + (rows - 1) * ld + wide > t.untyped_storage().nbytes():
+            raise PganError(f"{what}: the last row is not readable up to a multiple of 16 bytes")
+        return t.data_ptr(), ld
+
+    def _scales(self, t, what, n):
+        self._here(t, what)
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+            raise PganError(f"{what}: expected a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
+        return t.data_ptr()
+
+    @staticmethod
+    def _apart(*named):
+        """Refuses outputs that share memory with another operand."""
+        spans = []
+        for what, t, written in named:
+            if t is not None and t.numel():
+                lo = t.data_ptr()
+                last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+                spans.append((lo, lo + (last + 1) * t.element_size(), written, what))
+        spans.sort()
+        top = (0, 0, False, "")
+        for s in spans:
+            if s[0] < top[1] and (s[2] or top[2]):
+                raise PganError(f"{top[3]} and {s[3]} share memory")
+            if s[1] > top[1]:
+                top = s
+
+    def quant_rows(self, x, q, scale, lrelu: bool = False) -> None:
+        """Codes and scale of each row of x [T, K] (after LeakyReLU(0.1) if lrelu): q int8 [T, K], scale float32 [T] with
+        x ~ q * scale.  A row that holds an infinity or a NaN gets codes 0 and the scale NaN."""
+        xp, xt, ldx = self._float_rows(x, "quant_rows: x")
+        T, K = x.shape
+        if K < 1:
+            raise PganError("quant_rows: rows without elements have no scale")
+        qp, ldq = self._code_rows(q, "quant_rows: q", T, K)
+        sp = self._scales(scale, "quant_rows: scale", T)
+        self._apart(("x", x, False), ("q", q, True), ("scale", scale, True))
+        _check(_lib.pgan_quant_rows(xp, xt, ldx, qp, ldq, sp, T, K, int(bool(lrelu)), self._own_stream()), "pgan_quant_rows")
+
+    def _product_args(self, what, K, w, w_scale, y, bias):
+        yp, yt, ldy = self._float_rows(y, f"{what}: y")
+        T, N = y.shape
+        wp, ldw = self._code_rows(w, f"{what}: w", N, K)
+        if w.shape[0] != N or (bias is not None and bias.numel() != N) or K < 1 or N < 1:
+            raise PganError(f"{what}: w {tuple(w.shape)} and bias do not fit y {tuple(y.shape)} and {K} inner elements")
+        return T, N, wp, ldw, self._scales(w_scale, f"{what}: w_scale", N), \
+            None if bias is None else self._scales(bias, f"{what}: bias", N), yp, yt, ldy
+
+    def gemm_q8(self, q, q_scale, w, w_scale, y, bias=None) -> None:
+        """y [T, N] = q_scale[t] w_scale[n] sum_k q[t, k] w[n, k] + bias[n]: q int8 [T, K], w int8 [N, K], y float32, bfloat16
+        or float16; the sum is exact (K <= 131072)."""
+        K = q.shape[1]
+        T, N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("gemm_q8", K, w, w_scale, y, bias)
+        if q.shape[0] != T:
+            raise PganError(f"gemm_q8: {q.shape[0]} rows of q for {T} of y")
+        qp, ldq = self._code_rows(q, "gemm_q8: q", T, K)
+        qs = self._scales(q_scale, "gemm_q8: q_scale", T)
+        self._apart(("y", y, True), ("q", q, False), ("q_scale", q_scale, False), ("w", w, False), ("w_scale", w_scale, False),
+                    ("bias", bias, False))
+        _check(_lib.pgan_gemm_q8(qp, ldq, qs, wp, ldw, ws, bp, yp, yt, ldy, T, N, K, self._own_stream()), "pgan_gemm_q8")
+
+    def linear_q8(self, x, w, w_scale, y, q, q_scale, bias=None, lrelu: bool = False) -> None:
+        """quant_rows(x) and gemm_q8 in one call.  q int8 [at least T, K] and q_scale [at least T] are scratch of the caller:
+        what they hold afterwards is not part of the result (few tokens skip them)."""
+        xp, xt, ldx = self._float_rows(x, "linear_q8: x")
+        K = x.shape[1]
+        T, N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("linear_q8", K, w, w_scale, y, bias)
+        if x.shape[0] != T:
+            raise PganError(f"linear_q8: {x.shape[0]} rows of x for {T} of y")
+        qp, ldq = self._code_rows(q, "linear_q8: q", T, K)
+        qs = self._scales(q_scale, "linear_q8: q_scale", T)
+        self._apart(("y", y, True), ("q", q, True), ("q_scale", q_scale, True), ("x", x, False), ("w", w, False),
+                    ("w_scale", w_scale, False), ("bias", bias, False))
+        _check(_lib.pgan_linear_q8(xp, xt, ldx, qp, ldq, qs, wp, ldw, ws, bp, yp, yt, ldy, T, N, K, int(bool(lrelu)),
+                                   self._own_stream()), "pgan_linear_q8")
+
+    def _fold_args(self, what, y, shift, C):
+        self._here(y, f"{what}: y")
+        if y.dtype not in ELEMENT_TYPES or y.dim() != 4 or not y.is_contiguous() or y.shape[3] != 16 * C or C < 1:
+            raise PganError(f"{what}: y must be a contiguous [B, H, W, 16 * {C}] tensor of float32, bfloat16 or float16, got "
+                            f"{y.dtype} {tuple(y.shape)}")
+        if shift is not None and shift.numel() != C:
+            raise PganError(f"{what}: {shift.numel()} shifts for {C} channels")
+        return y.data_ptr(), ELEMENT_TYPES[y.dtype], None if shift is None else self._scales(shift, f"{what}: shift", C)
+
+    def up_fold_q8(self, y, shift, q, scale) -> None:
+        """y [B, H, W, (kh, kw, c)]: the taps of ConvTranspose2d(kernel 4, stride 2, padding 1) made as a product.  Sums the
+        taps of each output pixel, adds shift[c] (or None), applies LeakyReLU(0.1) and writes the pixel's codes: q int8
+        [B * 2H * 2W, C], scale [B * 2H * 2W]."""
+        C = q.shape[1]
+        yp, yt, hp = self._fold_args("up_fold_q8", y, shift, C)
+        B, H, W = y.shape[:3]
+        if q.shape[0] != 4 * B * H * W:
+            raise PganError(f"up_fold_q8: q has {q.shape[0]} rows for {4 * B * H * W} pixels")
+        qp, ldq = self._code_rows(q, "up_fold_q8: q", 4 * B * H * W, C)
+        sp = self._scales(scale, "up_fold_q8: scale", 4 * B * H * W)
+        self._apart(("q", q, True), ("scale", scale, True), ("y", y, False), ("shift", shift, False))
+        _check(_lib.pgan_up_fold_q8(yp, yt, hp, qp, ldq, sp, B, H, W, C, self._own_stream()), "pgan_up_fold_q8")
+
+    def up_fold(self, y, shift, out, act: int = 0) -> None:
+        """As up_fold_q8, into float32 out [B, 2H, 2W, C] through act: 0 none, 1 sigmoid, 2 tanh."""
+        if out.dim() != 4:
+            raise PganError(f"up_fold: out must be [B, 2H, 2W, C], got {tuple(out.shape)}")
+        C = out.shape[3]
+        yp, yt, hp = self._fold_args("up_fold", y, shift, C)
+        B, H, W = y.shape[:3]
+        if tuple(out.shape) != (B, 2 * H, 2 * W, C):
+            raise PganError(f"up_fold: out is {tuple(out.shape)} for y {tuple(y.shape)}")
+        if act not in (0, 1, 2):
+            raise PganError(f"up_fold: act is 0, 1 or 2, got {act}")
+        op = self._scales(out, "up_fold: out", out.numel())
+        self._apart(("out", out, True), ("y", y, False), ("shift", shift, False))
+        _check(_lib.pgan_up_fold(yp, yt, hp, op, B, H, W, C, int(act), self._own_stream()), "pgan_up_fold")
 
     def convt1d_up(self, y, w, x, act=0):
         N, Cs, Ls = y.shape

@@ -48,11 +48,18 @@ __device__ __forceinline__ typename Elem<TYPE>::type from_f32(float x) {
 
 // magnitude as a pattern: ordered like the magnitudes, infinities above every number and NaN above those
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
-// maximum over groups of G lanes (a power of two), in every lane of the group
-template <int G>
-__device__ __forceinline__ uint32_t group_max(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
+}
+// maximum over aligned groups of 2^log lanes, in every lane of the group
+__device__ __forceinline__ uint32_t group_max(uint32_t v, int log) {
+    if (log > 0) v = dpp_max<0xB1>(v);
+    if (log > 1) v = dpp_max<0x4E>(v);
+    if (log > 2) v = dpp_max<0x141>(v);
+    if (log > 3) v = dpp_max<0x140>(v);
+    if (log > 4) v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+    if (log > 5) v = max(v, (uint32_t)__shfl_xor((int)v, 32, 64));
     return v;
 }
 struct RowScale {
@@ -67,115 +74,337 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
 __device__ __forceinline__ int code_of(float x, float inv) { return inv == 0.f ? 0 : (int)rintf(x * inv); }
 __device__ __forceinline__ float slope(float x, bool lrelu) { return lrelu && !(x > 0.f) ? x * PGAN_SLOPE : x; }
 
-// ---- rows to codes ------------------------------------------------------------------------------------------------
-// one row a wave
+// eight elements from p on; `aligned` to 16 bytes
 template <int TYPE>
+__device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float (&v)[8]) {
+    if constexpr (TYPE == 0) {
+        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = a[e];
+            v[4 + e] = b[e];
+        }
+    } else {
+        const i32x4 a = *reinterpret_cast<const i32x4*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (TYPE == 1) {
+                v[2 * e] = __builtin_bit_cast(float, a[e] << 16);
+                v[2 * e + 1] = __builtin_bit_cast(float, a[e] & (int)0xffff0000);
+            } else {
+                v[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)a[e]);
+                v[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)((uint32_t)a[e] >> 16));
+            }
+        }
+    }
+}
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float inv) {
+    return (uint32_t)(code_of(a, inv) & 255) | (uint32_t)(code_of(b, inv) & 255) << 8 | (uint32_t)(code_of(c, inv) & 255) << 16
+           | (uint32_t)code_of(d, inv) << 24;
+}
+
+// ---- rows to codes ------------------------------------------------------------------------------------------------
+// 2^log lanes a row, whose values stay in their registers between the maximum and the codes: 8 NIT each, K <= 8 NIT 2^log.
+// VEC: eight neighbouring ones at a time, in rows that start on 16-byte borders (codes on 8); else every 2^log-th.
+// Bound by HBM (2 + 1 bytes an element of 16 bits).
+template <int TYPE, bool VEC, int NIT>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                          int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
-                                                         long long rows, int K, int lrelu) {
+                                                         long long rows, int K, int lrelu, int log) {
+    const long long row = (long long)blockIdx.x * (256 >> log) + (threadIdx.x >> log);
+    const int l = threadIdx.x & ((1 << log) - 1);
+    if (row >= rows) return;        // whole groups of 2^log lanes
+    const typename Elem<TYPE>::type* xr = x + row * ldx;
+    int8_t* qr = q + row * ldq;
+    float v[NIT][8];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+        if constexpr (VEC) {
+            const int k = ((it << log) + l) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[it][e] = 0.f;
+            if (k + 8 <= K) {
+                load8<TYPE>(xr + k, v[it]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k + e < K) v[it][e] = to_f32<TYPE>(xr[k + e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = ((it * 8 + e) << log) + l;
+                v[it][e] = k < K ? to_f32<TYPE>(xr[k]) : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int it = 0; it < NIT; ++it)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[it][e] = slope(v[it][e], lrelu);
+            mx = max(mx, magnitude(v[it][e]));
+        }
+    const RowScale rs = row_scale(group_max(mx, log));
+    if (l == 0) scale[row] = rs.scale;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+        if constexpr (VEC) {
+            const int k = ((it << log) + l) * 8;
+            uint2 u;
+            u.x = four_codes(v[it][0], v[it][1], v[it][2], v[it][3], rs.inv);
+            u.y = four_codes(v[it][4], v[it][5], v[it][6], v[it][7], rs.inv);
+            if (k + 8 <= K) {
+                *reinterpret_cast<uint2*>(qr + k) = u;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k + e < K) qr[k + e] = (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3)));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = ((it * 8 + e) << log) + l;
+                if (k < K) qr[k] = (int8_t)code_of(v[it][e], rs.inv);
+            }
+        }
+    }
+}
+
+// longer rows: one a wave, read twice
+template <int TYPE>
+__global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
+                                                              int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
+                                                              long long rows, int K, int lrelu) {
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
     const typename Elem<TYPE>::type* xr = x + row * ldx;
     uint32_t mx = 0;
     for (int k = lane; k < K; k += 64) mx = max(mx, magnitude(slope(to_f32<TYPE>(xr[k]), lrelu)));
-    const RowScale rs = row_scale(group_max<64>(mx));
+    const RowScale rs = row_scale(group_max(mx, 6));
     int8_t* qr = q + row * ldq;
     for (int k = lane; k < K; k += 64) qr[k] = (int8_t)code_of(slope(to_f32<TYPE>(xr[k]), lrelu), rs.inv);
     if (lane == 0) scale[row] = rs.scale;
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
-// A block of four waves makes 128 tokens x 128 channels, a wave 64 x 64 as 2 x 2 tiles of 32 x 32 (i32 <- i8, 32 deep).
-// Stages of 128 bytes along K go through registers into LDS, where chunk c (16 bytes) of row r lies at slot r ^ 2c of its
-// 32 rows: a stage's global reads are whole 128-byte lines and neither side of LDS has bank conflicts.
-constexpr int GT = 128, GN = 128, GK = 128;
+// A block of WT x WN waves makes a tile of tokens x channels, a wave FT x FN tiles of 32 x 32 (i32 <- i8, 32 deep; channels
+// are the matrix instruction's rows, so that a lane holds four neighbouring channels of one token).  Stages of 128 bytes
+// along K go through registers into LDS, where chunk c (16 bytes) of row r lies at slot r ^ 2c of its 32 rows: a stage's
+// global reads are whole 128-byte lines and neither side of LDS has bank conflicts.  The next stage's reads are under way
+// while a stage is multiplied.
+constexpr int GK = 128;
 
 __device__ __forceinline__ int lds_slot(int row, int c) { return (row >> 5) * (32 * GK / 16) + c * 32 + ((row & 31) ^ (2 * c)); }
 
-// 16 bytes of a row from byte k on, zero from byte K on (rows are readable up to the next multiple of 16)
-__device__ __forceinline__ i32x4 load16(const int8_t* row, int k, int K) {
-    i32x4 v = {0, 0, 0, 0};
-    if (k < K) {
-        v = *reinterpret_cast<const i32x4*>(row + k);
-        if (k + 16 > K) {
+__device__ __forceinline__ i32x4 below(i32x4 v, int left) {        // the first `left` of 16 bytes, zero behind them
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int left = K - k - 4 * e;
-                v[e] = left >= 4 ? v[e] : left <= 0 ? 0 : v[e] & ((1 << (8 * left)) - 1);
-            }
-        }
+    for (int e = 0; e < 4; ++e) {
+        const int n = left - 4 * e;
+        v[e] = n >= 4 ? v[e] : n <= 0 ? 0 : v[e] & ((1 << (8 * n)) - 1);
     }
     return v;
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(256) void gemm_q8_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restrict__ qs,
-                                                      const int8_t* __restrict__ w, long long ldw,
-                                                      const float* __restrict__ ws, const float* __restrict__ bias,
-                                                      typename Elem<TYPE>::type* __restrict__ y, long long ldy, long long T,
-                                                      int N, int K) {
-    __shared__ i32x4 sx[GT * GK / 16], sw[GN * GK / 16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long long t0 = (long long)blockIdx.y * GT;
-    const int n0 = blockIdx.x * GN;
-    i32x16 acc[2][2];
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    using H = std::conditional_t<TYPE == 1, __bf16, _Float16>;
+    typedef H h2 __attribute__((ext_vector_type(2)));
+    return uint2{__builtin_bit_cast(uint32_t, h2{(H)a, (H)b}), __builtin_bit_cast(uint32_t, h2{(H)c, (H)d})};
+}
+// 16 bytes of a row, of which `left` elements lie inside it; align: bytes that every row starts on a multiple of
+template <class Y>
+__device__ __forceinline__ void put16(Y* to, i32x4 v, int left, int align) {
+    constexpr int PER = 16 / (int)sizeof(Y);
+    if (left >= PER) {
+        if (align == 16) {
+            *reinterpret_cast<i32x4*>(to) = v;
+            return;
+        }
+        if (align == 8) {
+            reinterpret_cast<int2*>(to)[0] = int2{v[0], v[1]};
+            reinterpret_cast<int2*>(to)[1] = int2{v[2], v[3]};
+            return;
+        }
+        if (align == 4) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+            for (int e = 0; e < 4; ++e) reinterpret_cast<int*>(to)[e] = v[e];
+            return;
+        }
+    }
+    const Y* h = reinterpret_cast<const Y*>(&v);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int e = 0; e < PER; ++e)
+        if (e < left) to[e] = h[e];
+}
+
+// what a wave's lanes wrote to LDS is seen by its other lanes
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct GemmArgs {
+    const int8_t* q;
+    const float* qs;
+    const int8_t* w;
+    const float* ws;
+    const float* bias;
+    void* y;
+    long long ldq, ldw, ldy, T;
+    int N, K;
+    unsigned tt, tn, band;      // tiles along the tokens and along the channels, channel tiles of a band
+    int align;                  // bytes (16, 8, 4, 2) that every row of y starts on a multiple of
+};
+
+// Tile of a block: blocks go round the eight dies, each of which gets a run of neighbouring tiles -- bands of eight channel
+// tiles, token tile by token tile -- so that what it reads stays in its L2.
+__device__ __forceinline__ void tile_of(const GemmArgs& a, unsigned& tt, unsigned& tn) {
+    const unsigned tiles = a.tt * a.tn, per = tiles / 8, rest = tiles % 8, die = blockIdx.x % 8;
+    const unsigned id = die * per + min(die, rest) + blockIdx.x / 8;
+    const unsigned band = id / (a.band * a.tt), in = id - band * a.band * a.tt, wide = min(a.band, a.tn - band * a.band);
+    tt = in / wide;
+    tn = band * a.band + in - tt * wide;
+}
+
+template <int FT, int FN, int WT, int WN, int TYPE>
+__global__ __launch_bounds__(64 * WT * WN, FT * FN > 4 ? 2 : 3) void gemm_q8_kernel(const GemmArgs a) {
+    using Y = typename Elem<TYPE>::type;
+    constexpr int NT = 64 * WT * WN, BT = 32 * FT * WT, BN = 32 * FN * WN;
+    constexpr int RP = NT / 8;                           // rows that the block's threads read at a time
+    constexpr int LT = BT / RP, LN = BN / RP;
+    constexpr int STAGE = (BT + BN) * GK / 16;           // 16-byte chunks
+    constexpr int FO = FN < 2 ? FN : 2;                  // channel tiles whose results leave together
+    constexpr int YROW = 32 * FO * (int)sizeof(Y) + 16;  // a wave's row of results in LDS, 16 bytes apart
+    constexpr int OUT = 32 * YROW * WT * WN;
+    constexpr int BYTES = STAGE * 16 > OUT ? STAGE * 16 : OUT;
+    __shared__ __attribute__((aligned(16))) char mem[BYTES];
+    __shared__ __attribute__((aligned(16))) float sws[BN], sbias[BN], sqs[BT];
+    i32x4* lds = reinterpret_cast<i32x4*>(mem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave / WN, wn = wave % WN;
+    unsigned tt, tn;
+    tile_of(a, tt, tn);
+    const long long t0 = (long long)tt * BT;
+    const int n0 = (int)tn * BN, K = a.K, c = tid & 7;
+    const int trows = (int)(a.T - t0 < BT ? a.T - t0 : BT), nrows = min(a.N - n0, BN);
+    // rows past the end repeat the last one; what they give is not stored
+    const int8_t* xb = a.q + t0 * a.ldq;
+    const int8_t* wb = a.w + (long long)n0 * a.ldw;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xb), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wb), 0, 0x7fffffff, 0x00020000);
+    int xo[LT], wo[LN];
+#pragma unroll
+    for (int i = 0; i < LT; ++i) xo[i] = min((tid >> 3) + RP * i, trows - 1) * (int)a.ldq;
+#pragma unroll
+    for (int i = 0; i < LN; ++i) wo[i] = min((tid >> 3) + RP * i, nrows - 1) * (int)a.ldw;
+    i32x4 vx[LT], vw[LN];
+    const auto load = [&](int k0) {
+        const int k = k0 + 16 * c < K ? 16 * c : -k0;     // chunks past the end read the row's first one and count as zero
+#pragma unroll
+        for (int i = 0; i < LT; ++i) vx[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i] + k0 + k, 0, 0));
+#pragma unroll
+        for (int i = 0; i < LN; ++i) vw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wo[i] + k0 + k, 0, 0));
+    };
+    const auto store = [&](int k0) {
+        if (k0 + GK > K) {
+#pragma unroll
+            for (int i = 0; i < LN; ++i) vw[i] = below(vw[i], K - k0 - 16 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < LT; ++i) lds[lds_slot((tid >> 3) + RP * i, c)] = vx[i];
+#pragma unroll
+        for (int i = 0; i < LN; ++i) lds[BT * 8 + lds_slot((tid >> 3) + RP * i, c)] = vw[i];
+    };
+    i32x16 acc[FN][FT];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    const int c = tid & 7;
+    load(0);
+    // the scales follow on the first stage's reads
+    static_assert(BN <= NT && BT <= NT, "one scale a thread");
+    const int sn = n0 + min(tid, nrows - 1);
+    const float vws = a.ws[sn], vbias = a.bias ? a.bias[sn] : 0.f, vqs = a.qs[t0 + min(tid, trows - 1)];
+    store(0);
+    if (tid < BN) {
+        sws[tid] = vws;
+        sbias[tid] = vbias;
+    }
+    if (tid < BT) sqs[tid] = vqs;
+    __syncthreads();
     for (int k0 = 0; k0 < K; k0 += GK) {
-        i32x4 vx[4], vw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {       // rows past the end repeat the last one; what they give is not stored
-            const int r = (tid >> 3) + 32 * i;
-            const long long t = t0 + r < T ? t0 + r : T - 1;
-            const int n = n0 + r < N ? n0 + r : N - 1;
-            vx[i] = load16(q + t * ldq, k0 + 16 * c, K);
-            vw[i] = load16(w + (long long)n * ldw, k0 + 16 * c, K);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (tid >> 3) + 32 * i;
-            sx[lds_slot(r, c)] = vx[i];
-            sw[lds_slot(r, c)] = vw[i];
-        }
-        __syncthreads();
+        const bool more = k0 + GK < K;
+        if (more) load(k0 + GK);
 #pragma unroll
         for (int s = 0; s < GK / 32; ++s) {
             const int cc = 2 * s + (lane >> 5);
-            i32x4 a[2], b[2];
+            i32x4 fw[FN], fx[FT];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = sw[lds_slot((wave & 1) * 64 + 32 * i + (lane & 31), cc)];
-                b[i] = sx[lds_slot((wave >> 1) * 64 + 32 * i + (lane & 31), cc)];
-            }
+            for (int i = 0; i < FN; ++i) fw[i] = lds[BT * 8 + lds_slot((wn * FN + i) * 32 + (lane & 31), cc)];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < FT; ++j) fx[j] = lds[lds_slot((wt * FT + j) * 32 + (lane & 31), cc)];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
+        }
+        __syncthreads();
+        if (more) {
+            store(k0 + GK);
+            __syncthreads();
         }
     }
+    // The results of 32 tokens at a time pass through the wave's part of LDS, to leave as whole lines of y's rows.
     // channel (within 32): e % 4 + 8 (e / 4) + 4 (lane / 32); token: lane % 32
+    char* own = mem + wave * 32 * YROW;
+    constexpr int PER = 16 / (int)sizeof(Y), LANES = 32 * FO / PER;      // channels and lanes of a 16-byte row stretch
+    const bool whole = trows == BT && nrows == BN && a.align == 16;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const long long t = t0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
-        if (t >= T) continue;
-        const float st = qs[t];
+    for (int io = 0; io < FN; io += FO) {
+        const int wc0 = (wn * FN + io) * 32;
+        f32x4 ws[FO][4], bs[FO][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < FO; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int n = n0 + (wave & 1) * 64 + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-                if (n >= N) continue;
-                float v = (float)acc[i][j][e] * (st * ws[n]);
-                if (bias) v = v + bias[n];
-                y[t * ldy + n] = from_f32<TYPE>(v);
+            for (int g = 0; g < 4; ++g) {
+                const int ch = wc0 + 32 * i + 8 * g + 4 * (lane >> 5);
+                ws[i][g] = *reinterpret_cast<const f32x4*>(sws + ch);
+                bs[i][g] = *reinterpret_cast<const f32x4*>(sbias + ch);
             }
+#pragma unroll
+        for (int j = 0; j < FT; ++j) {
+            const int tr = (wt * FT + j) * 32;
+            const float st = sqs[tr + (lane & 31)];
+#pragma unroll
+            for (int i = 0; i < FO; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)acc[io + i][j][4 * g + e] * st, ws[i][g][e], bs[i][g][e]);
+                    char* to = own + (lane & 31) * YROW + (32 * i + 8 * g + 4 * (lane >> 5)) * (int)sizeof(Y);
+                    if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+                    else *reinterpret_cast<uint2*>(to) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
+                }
+            wave_sync();
+            Y* to = static_cast<Y*>(a.y) + (t0 + tr + lane / LANES) * a.ldy + n0 + wc0 + lane % LANES * PER;
+            const char* from = own + lane / LANES * YROW + lane % LANES * 16;
+            if (whole) {
+#pragma unroll
+                for (int r = 0; r < 32; r += 64 / LANES)
+                    *reinterpret_cast<i32x4*>(to + r * a.ldy) = *reinterpret_cast<const i32x4*>(from + r * YROW);
+            } else {
+                for (int r = 0; r < 32; r += 64 / LANES)
+                    if (tr + r + lane / LANES < trows)
+                        put16(to + r * a.ldy, *reinterpret_cast<const i32x4*>(from + r * YROW), nrows - wc0 - lane % LANES * PER, a.align);
+            }
+            wave_sync();
+        }
     }
 }
 
@@ -186,15 +415,15 @@ __global__ __launch_bounds__(256) void gemm_q8_kernel(const int8_t* __restrict__
 struct Taps {
     long long at[2][2];     // first element of the tap's channels, -1: outside
 };
-__device__ __forceinline__ Taps taps_of(long long pix, int H, int W, int C) {
-    const int W2 = 2 * W, H2 = 2 * H;
-    const int ow = (int)(pix % W2), oh = (int)(pix / W2 % H2);
-    const long long b = pix / W2 / H2;
+__device__ __forceinline__ Taps taps_of(unsigned pix, int H, int W, int C) {
+    const unsigned W2 = 2 * W, H2 = 2 * H;
+    const unsigned line = pix / W2, b = line / H2;
+    const int ow = (int)(pix - line * W2), oh = (int)(line - b * H2);
     const int ih = oh >> 1, iw = ow >> 1;
     const int h2 = oh & 1 ? ih + 1 : ih - 1, w2 = ow & 1 ? iw + 1 : iw - 1;
     const int ka = oh & 1 ? 2 : 1, kb = oh & 1 ? 0 : 3, la = ow & 1 ? 2 : 1, lb = ow & 1 ? 0 : 3;
     const bool hok = h2 >= 0 && h2 < H, wok = w2 >= 0 && w2 < W;
-    const long long ra = (b * H + ih) * W, rb = (b * H + h2) * W;
+    const long long ra = ((long long)b * H + ih) * W, rb = ((long long)b * H + h2) * W;
     Taps t;
     t.at[0][0] = ((ra + iw) * 16 + ka * 4 + la) * C;
     t.at[1][0] = hok ? ((rb + iw) * 16 + kb * 4 + la) * C : -1;
@@ -208,41 +437,166 @@ __device__ __forceinline__ float folded(const typename Elem<TYPE>::type* y, cons
     const float o = (get(0, 0) + get(1, 0)) + (get(0, 1) + get(1, 1));
     return shift ? o + shift[c] : o;
 }
-
-// one output pixel a wave: sum, LeakyReLU, codes
-template <int TYPE>
-__global__ __launch_bounds__(256) void up_fold_q8_kernel(const typename Elem<TYPE>::type* __restrict__ y,
-                                                         const float* __restrict__ shift, int8_t* __restrict__ q,
-                                                         long long ldq, float* __restrict__ scale, long long pixels, int H,
-                                                         int W, int C) {
-    const long long pix = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (pix >= pixels) return;
-    const Taps t = taps_of(pix, H, W, C);
-    uint32_t mx = 0;
-    for (int c = lane; c < C; c += 64) mx = max(mx, magnitude(slope(folded<TYPE>(y, t, c, shift), true)));
-    const RowScale rs = row_scale(group_max<64>(mx));
-    for (int c = lane; c < C; c += 64) q[pix * ldq + c] = (int8_t)code_of(slope(folded<TYPE>(y, t, c, shift), true), rs.inv);
-    if (lane == 0) scale[pix] = rs.scale;
+__device__ __forceinline__ float activate(float o, int act) {
+    if (act == 1) return 1.f / (1.f + expf(-o));
+    if (act == 2) return tanhf(o);
+    return o;
 }
 
+struct FoldArgs {
+    const float* shift;
+    int8_t* q;
+    float* scale;           // of codes
+    float* out;             // or fp32 results
+    long long ldq;
+    unsigned pixels;
+    int H, W, C, act, log;
+};
+
+// 2^log lanes an output pixel, eight channels each: neighbouring ones (VEC: every tap and row of results on a 16-byte
+// border), else every 2^log-th.  Every input value goes to exactly one output: nothing is read twice.  Bound by HBM.
+template <int TYPE, bool VEC, bool Q8>
+__global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
+    const unsigned pix = blockIdx.x * (256u >> a.log) + (threadIdx.x >> a.log);
+    const int l = threadIdx.x & ((1 << a.log) - 1), C = a.C;
+    if (pix >= a.pixels) return;        // whole groups of 2^log lanes
+    const Taps t = taps_of(pix, a.H, a.W, C);
+    float v[8];
+    if constexpr (VEC) {
+        const int c = l * 8;
+        float p[2][2][8], sh[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[i][j][e] = 0.f;
+                if (c < C && t.at[i][j] >= 0) load8<TYPE>(y + t.at[i][j] + c, p[i][j]);
+            }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sh[e] = a.shift && c < C ? a.shift[c + e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float o = (p[0][0][e] + p[1][0][e]) + (p[0][1][e] + p[1][1][e]);
+            v[e] = a.shift ? o + sh[e] : o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = (e << a.log) + l;
+            v[e] = c < C ? folded<TYPE>(y, t, c, a.shift) : 0.f;
+        }
+    }
+    if constexpr (Q8) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = slope(v[e], true);
+            mx = max(mx, magnitude(v[e]));
+        }
+        if constexpr (VEC) mx = l * 8 < C ? mx : 0u;
+        const RowScale rs = row_scale(group_max(mx, a.log));
+        if (l == 0) a.scale[pix] = rs.scale;
+        int8_t* qr = a.q + (long long)pix * a.ldq;
+        if constexpr (VEC) {
+            if (l * 8 < C)
+                *reinterpret_cast<uint2*>(qr + l * 8) = uint2{four_codes(v[0], v[1], v[2], v[3], rs.inv), four_codes(v[4], v[5], v[6], v[7], rs.inv)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = (e << a.log) + l;
+                if (c < C) qr[c] = (int8_t)code_of(v[e], rs.inv);
+            }
+        }
+    } else {
+        float* o = a.out + (long long)pix * C;
+        if constexpr (VEC) {
+            if (l * 8 < C) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 4)
+                    *reinterpret_cast<f32x4*>(o + l * 8 + e) = f32x4{activate(v[e], a.act), activate(v[e + 1], a.act), activate(v[e + 2], a.act), activate(v[e + 3], a.act)};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = (e << a.log) + l;
+                if (c < C) o[c] = activate(v[e], a.act);
+            }
+        }
+    }
+}
+
+// more than 512 channels: one output pixel a wave, codes in two passes
+template <int TYPE, bool Q8>
+__global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
+    const unsigned pix = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (pix >= a.pixels) return;
+    const Taps t = taps_of(pix, a.H, a.W, a.C);
+    if constexpr (Q8) {
+        uint32_t mx = 0;
+        for (int c = lane; c < a.C; c += 64) mx = max(mx, magnitude(slope(folded<TYPE>(y, t, c, a.shift), true)));
+        const RowScale rs = row_scale(group_max(mx, 6));
+        for (int c = lane; c < a.C; c += 64)
+            a.q[(long long)pix * a.ldq + c] = (int8_t)code_of(slope(folded<TYPE>(y, t, c, a.shift), true), rs.inv);
+        if (lane == 0) a.scale[pix] = rs.scale;
+    } else {
+        for (int c = lane; c < a.C; c += 64) a.out[(long long)pix * a.C + c] = activate(folded<TYPE>(y, t, c, a.shift), a.act);
+    }
+}
+
+// One channel: a lane an input pixel, for the 2 x 2 output pixels on it.  It reads what its column gives them -- taps of row 3
+// from the pixel above, 1 and 2 of its own, 0 of the one below -- sums them along the column, and takes from its left and
+// right neighbours their sums of column 3 and 0.  The first and last lane of a wave, whose neighbour is in another wave,
+// make that neighbour's sums themselves.
 template <int TYPE>
-__global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>::type* __restrict__ y,
-                                                      const float* __restrict__ shift, float* __restrict__ out,
-                                                      long long pixels, int H, int W, int C, int act) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= pixels * C) return;
-    const long long pix = i / C;
-    float o = folded<TYPE>(y, taps_of(pix, H, W, C), (int)(i % C), shift);
-    if (act == 1) o = 1.f / (1.f + expf(-o));
-    if (act == 2) o = tanhf(o);
-    out[i] = o;
+__global__ __launch_bounds__(256) void up_fold_one_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
+    const unsigned i = blockIdx.x * 256 + threadIdx.x, n = a.pixels / 4, at = min(i, n - 1);
+    const int H = a.H, W = a.W, lane = threadIdx.x & 63;
+    const unsigned line = at / W, b = line / H;
+    const int iw = (int)(at - line * W), ih = (int)(line - b * H);
+    const bool up = ih > 0, down = ih + 1 < H;
+    const auto column = [&](long long p, int k, float& even, float& odd) {      // sums of column k of pixel p's taps
+        const typename Elem<TYPE>::type* t = y + p * 16 + k;
+        even = to_f32<TYPE>(t[4]) + (up ? to_f32<TYPE>(t[12 - 16 * (long long)W]) : 0.f);
+        odd = to_f32<TYPE>(t[8]) + (down ? to_f32<TYPE>(t[16 * (long long)W]) : 0.f);
+    };
+    float e[4], o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) column(at, k, e[k], o[k]);
+    float le = __shfl_up(e[3], 1, 64), lo = __shfl_up(o[3], 1, 64), re = __shfl_down(e[0], 1, 64), ro = __shfl_down(o[0], 1, 64);
+    if (lane == 0 && iw > 0) column((long long)at - 1, 3, le, lo);
+    if (lane == 63 && iw + 1 < W) column((long long)at + 1, 0, re, ro);
+    if (i >= n) return;
+    if (iw == 0) le = lo = 0.f;
+    if (iw + 1 == W) re = ro = 0.f;
+    const float sh = a.shift ? a.shift[0] : 0.f;
+    const auto end = [&](float x) { return activate(a.shift ? x + sh : x, a.act); };
+    float* to = a.out + ((long long)line * 4 * W + 2 * iw);
+    typedef float f32x2 __attribute__((ext_vector_type(2), aligned(4)));
+    *reinterpret_cast<f32x2*>(to) = f32x2{end(e[1] + le), end(e[2] + re)};
+    *reinterpret_cast<f32x2*>(to + 2 * W) = f32x2{end(o[1] + lo), end(o[2] + ro)};
 }
 
 // threads of one launch stay below 2^32
 constexpr long long MAX_BLOCKS = 0xffffff;
 inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 inline int type_bytes(int type) { return type == 0 ? 4 : 2; }
+
+constexpr long long MAX_STRIDE = 1 << 22;      // offsets of a tile's rows fit 31 bits
+
+inline int row_align(const void* p, long long stride) {
+    const uintptr_t u = reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride;
+    return u % 16 == 0 ? 16 : u % 8 == 0 ? 8 : u % 4 == 0 ? 4 : 2;
+}
+
+template <int FT, int FN, int WT, int WN, int TYPE>
+void launch_gemm(GemmArgs a, hipStream_t st) {
+    a.tn = (a.N + 32 * FN * WN - 1) / (32 * FN * WN);
+    a.band = a.tn < 8 ? a.tn : 8;
+    a.tt = (unsigned)((a.T + 32 * FT * WT - 1) / (32 * FT * WT));
+    gemm_q8_kernel<FT, FN, WT, WN, TYPE><<<a.tt * a.tn, 64 * WT * WN, 0, st>>>(a);
+}
 
 template <class F>
 inline int by_type(int type, F f) {
@@ -254,6 +608,38 @@ inline int by_type(int type, F f) {
     return pgan_launch_status();
 }
 
+// lanes a row or an output pixel (as a power of two): eight elements each, all 64 for more than 256
+inline int lanes_log(int C) {
+    int log = 0;
+    while (log < 6 && (8 << log) < C) ++log;
+    return log;
+}
+inline bool fold_fits(int type, int B, int H, int W, int C) {
+    if (B < 0 || H < 1 || W < 1 || C < 1 || type < 0 || type > 2 || H > 32768 || W > 32768) return false;
+    return B <= ((MAX_BLOCKS * 256) >> lanes_log(C)) / (4LL * H * W);
+}
+template <bool Q8>
+int launch_fold(const void* y, int type, FoldArgs a, bool vec, hipStream_t st) {
+    a.log = lanes_log(a.C);
+    const unsigned per = 256u >> a.log, blocks = a.pixels / per + (a.pixels % per != 0);
+    return by_type(type, [&](auto t) {
+        const auto* p = static_cast<const typename Elem<t.value>::type*>(y);
+        if (a.C > 512) up_fold_wide_kernel<t.value, Q8><<<blocks, 256, 0, st>>>(p, a);
+        else if (vec) up_fold_kernel<t.value, true, Q8><<<blocks, 256, 0, st>>>(p, a);
+        else up_fold_kernel<t.value, false, Q8><<<blocks, 256, 0, st>>>(p, a);
+    });
+}
+
+inline int gemm_args(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
+                     const void* y, int y_type, long long ldy, long long T, int N, int K) {
+    if (T < 0 || N < 1 || K < 1 || K > 131072 || y_type < 0 || y_type > 2) return PGAN_EINVAL;
+    if (T == 0) return PGAN_OK;
+    if (!q || !q_scale || !w || !w_scale || !y || !aligned(q, 16) || !aligned(w, 16) || ldq % 16 || ldw % 16 || ldq < K
+        || ldw < K || ldy < N || ldq > MAX_STRIDE || ldw > MAX_STRIDE || !aligned(y, type_bytes(y_type)))
+        return PGAN_EINVAL;
+    return (T + 255) / 256 * ((N + 255) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -263,69 +649,74 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
     if (rows < 0 || K < 1 || x_type < 0 || x_type > 2) return PGAN_EINVAL;
     if (rows == 0) return PGAN_OK;
     if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4) || ldx < K || ldq < K) return PGAN_EINVAL;
-    const long long blocks = (rows + 3) / 4;
+    const bool vec = row_align(x, ldx * type_bytes(x_type)) == 16 && row_align(q, ldq) >= 8;
+    const int log = lanes_log(K);    // lanes a row
+    const long long blocks = (rows + (256 >> log) - 1) / (256 >> log);
     if (blocks > MAX_BLOCKS) return PGAN_EINVAL;
     return by_type(x_type, [&](auto t) {
-        quant_rows_kernel<t.value><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<t.value>::type*>(x), ldx,
-                                                                      static_cast<int8_t*>(q), ldq, scale, rows, K, lrelu);
+        constexpr int X = t.value;
+        const auto go = [&](auto kernel, auto... more) {
+            kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<X>::type*>(x), ldx, static_cast<int8_t*>(q), ldq,
+                                                      scale, rows, K, lrelu, more...);
+        };
+        if (K > 4096) go(quant_long_rows_kernel<X>);
+        else if (K > 2048) vec ? go(quant_rows_kernel<X, true, 8>, log) : go(quant_rows_kernel<X, false, 8>, log);
+        else if (K > 1024) vec ? go(quant_rows_kernel<X, true, 4>, log) : go(quant_rows_kernel<X, false, 4>, log);
+        else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2>, log) : go(quant_rows_kernel<X, false, 2>, log);
+        else vec ? go(quant_rows_kernel<X, true, 1>, log) : go(quant_rows_kernel<X, false, 1>, log);
     });
 }
 
 int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
                  const float* bias, void* y, int y_type, long long ldy, long long T, int N, int K, hipStream_t st) {
-    if (T < 0 || N < 1 || K < 1 || K > 131072 || y_type < 0 || y_type > 2) return PGAN_EINVAL;
-    if (T == 0) return PGAN_OK;
-    if (!q || !q_scale || !w || !w_scale || !y || !aligned(q, 16) || !aligned(w, 16) || ldq % 16 || ldw % 16 || ldq < K
-        || ldw < K || ldy < N || !aligned(y, type_bytes(y_type)))
-        return PGAN_EINVAL;
-    const long long bt = (T + GT - 1) / GT;
-    const int bn = (N + GN - 1) / GN;
-    if (bt > 65535) return PGAN_EINVAL;
+    const int rc = gemm_args(q, ldq, q_scale, w, ldw, w_scale, y, y_type, ldy, T, N, K);
+    if (rc || T == 0) return rc;
     return by_type(y_type, [&](auto t) {
-        gemm_q8_kernel<t.value><<<dim3((unsigned)bn, (unsigned)bt), 256, 0, st>>>(
-            static_cast<const int8_t*>(q), ldq, q_scale, static_cast<const int8_t*>(w), ldw, w_scale, bias,
-            static_cast<typename Elem<t.value>::type*>(y), ldy, T, N, K);
+        constexpr int Y = t.value;
+        GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0,
+                   row_align(y, ldy * type_bytes(y_type))};
+        const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
+        // The larger the tile the fewer LDS reads a product takes, as long as there is a tile for each of the 256 CUs:
+        // 4096 x 4096 x 4096 in 256 x 256: 70 us (1960 Tera operations/s), 128 x 128: 84, 128 x 64: 97, 64 x 64: 115;
+        // 64 x 4096 x 1024 (1 .. 16 tiles): 62, 32, 23, 16 us.  (One with two LDS buffers and one barrier a stage instead of
+        // one and two was not faster: 70 us.)
+        if (N <= 32) launch_gemm<2, 1, 4, 1, Y>(a, st);
+        else if (tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, Y>(a, st);
+        else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, Y>(a, st);
+        else if (tiles(128, 64) >= 256) launch_gemm<2, 1, 2, 2, Y>(a, st);
+        else launch_gemm<1, 1, 2, 2, Y>(a, st);
     });
 }
 
 int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long ldq, float* q_scale, const void* w,
                    long long ldw, const float* w_scale, const float* bias, void* y, int y_type, long long ldy, long long T,
                    int N, int K, int lrelu, hipStream_t st) {
-    if (T < 0 || N < 1 || K < 1 || K > 131072 || x_type < 0 || x_type > 2 || y_type < 0 || y_type > 2) return PGAN_EINVAL;
-    if (T == 0) return PGAN_OK;
-    if (!x || !w || !w_scale || !y || !q || !q_scale || !aligned(q, 16) || !aligned(w, 16) || ldq % 16 || ldw % 16
-        || ldq < K || ldw < K || ldx < K || ldy < N || !aligned(x, type_bytes(x_type)) || !aligned(y, type_bytes(y_type)))
-        return PGAN_EINVAL;
+    const int ok = gemm_args(q, ldq, q_scale, w, ldw, w_scale, y, y_type, ldy, T, N, K);
+    if (ok || T == 0) return ok;
     const int rc = pgan_quant_rows(x, x_type, ldx, q, ldq, q_scale, T, K, lrelu, st);
     return rc ? rc : pgan_gemm_q8(q, ldq, q_scale, w, ldw, w_scale, bias, y, y_type, ldy, T, N, K, st);
 }
 
 int pgan_up_fold_q8(const void* y, int y_type, const float* shift, void* q, long long ldq, float* scale, int B, int H, int W,
                     int C, hipStream_t st) {
-    if (B < 0 || H < 1 || W < 1 || C < 1 || y_type < 0 || y_type > 2 || H > 32768 || W > 32768) return PGAN_EINVAL;
+    if (!fold_fits(y_type, B, H, W, C)) return PGAN_EINVAL;
     if (B == 0) return PGAN_OK;
     if (!y || !q || !scale || ldq < C || !aligned(y, type_bytes(y_type)) || !aligned(scale, 4)) return PGAN_EINVAL;
-    const long long pixels = 4LL * B * H * W, blocks = (pixels + 3) / 4;
-    if (blocks > MAX_BLOCKS) return PGAN_EINVAL;
-    return by_type(y_type, [&](auto t) {
-        up_fold_q8_kernel<t.value><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<t.value>::type*>(y), shift,
-                                                                      static_cast<int8_t*>(q), ldq, scale, pixels, H, W, C);
-    });
+    FoldArgs a{shift, static_cast<int8_t*>(q), scale, nullptr, ldq, (unsigned)(4LL * B * H * W), H, W, C, 0, 0};
+    return launch_fold<true>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && row_align(q, ldq) >= 8, st);
 }
 
 int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int B, int H, int W, int C, int act,
                  hipStream_t st) {
-    if (B < 0 || H < 1 || W < 1 || C < 1 || y_type < 0 || y_type > 2 || act < 0 || act > 2 || H > 32768 || W > 32768)
-        return PGAN_EINVAL;
+    if (!fold_fits(y_type, B, H, W, C) || act < 0 || act > 2) return PGAN_EINVAL;
     if (B == 0) return PGAN_OK;
     if (!y || !out || !aligned(y, type_bytes(y_type)) || !aligned(out, 4)) return PGAN_EINVAL;
-    const long long pixels = 4LL * B * H * W;
-    if (pixels > MAX_BLOCKS * 256 / C) return PGAN_EINVAL;
-    const long long blocks = (pixels * C + 255) / 256;
-    return by_type(y_type, [&](auto t) {
-        up_fold_kernel<t.value><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<t.value>::type*>(y), shift,
-                                                                   out, pixels, H, W, C, act);
-    });
+    FoldArgs a{shift, nullptr, nullptr, out, 0, (unsigned)(4LL * B * H * W), H, W, C, act, 0};
+    if (C == 1)
+        return by_type(y_type, [&](auto t) {
+            up_fold_one_kernel<t.value><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(static_cast<const typename Elem<t.value>::type*>(y), a);
+        });
+    return launch_fold<false>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && aligned(out, 16), st);
 }
 
 }  // extern "C"

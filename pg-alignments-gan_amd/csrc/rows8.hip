@@ -8,6 +8,8 @@
 // The sum is exact: whole numbers in 32 bits (K <= 131072 keeps 127^2 K below 2^31).  A row's largest magnitude counts as at
 // least 2^-100, which keeps both quotients finite; a row that holds an infinity or a NaN gets codes 0 and the scale NaN, so
 // that its whole row of y is NaN and no other row is touched.
+#include <algorithm>
+
 #include "../../include/pgan_hip.h"
 #include "pgan_common.h"
 
@@ -408,6 +410,149 @@ __global__ __launch_bounds__(64 * WT * WN, FT * FN > 4 ? 2 : 3) void gemm_q8_ker
     }
 }
 
+// ---- the product for few tokens ------------------------------------------------------------------------------------
+// Up to 32 tokens: a block makes 32 channels, its WV waves share K and add up their sums (whole numbers: any order) in LDS.
+// Channels come straight from memory into the matrix instruction's registers, every line of them by one wave.  X >= 0: the
+// block makes the tokens' codes itself, a wave RW rows -- every block all of them, which for up to 32768 elements takes less time than a
+// launch of its own -- while its first channels are on their way; X < 0: it reads codes.  Bound by the launch, then by the
+// channels' bytes.
+struct FewArgs {
+    GemmArgs g;
+    const void* x;
+    long long ldx;
+    int lrelu, vec;         // vec: rows of x start on 16-byte borders
+};
+template <int X, int WV, int RW, int TYPE>
+__global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
+    using Y = typename Elem<TYPE>::type;
+    using XE = typename Elem<X < 0 ? 0 : X>::type;
+    extern __shared__ __attribute__((aligned(16))) char few[];
+    const GemmArgs& a = f.g;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int K = a.K, T = (int)a.T, N = a.N, end = (K + 15) / 16 * 16 - 16;      // a row's last 16 bytes
+    const int n0 = blockIdx.x * 32, half = lane >> 5, stride = (K + 31) / 32 * 32 + 16;
+    const int steps = (K + 31) / 32, s0 = wave * steps / WV, s1 = (wave + 1) * steps / WV;
+    const int8_t* wr = a.w + (long long)min(n0 + (lane & 31), N - 1) * a.ldw;
+    const auto channels = [&](int s, i32x4 (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < s1) v[i] = *reinterpret_cast<const i32x4*>(wr + min((s + i) * 32 + 16 * half, end));
+    };
+    i32x4 cur[4], nxt[4];
+    channels(s0, cur);
+    float ws[4], bs[4];         // of the four channels whose sums this lane ends
+    const int ch = n0 + 8 * wave + 4 * half;
+    if (wave < 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            ws[e] = a.ws[min(ch + e, N - 1)];
+            bs[e] = a.bias ? a.bias[min(ch + e, N - 1)] : 0.f;
+        }
+    }
+    __shared__ float scales[32];
+    if constexpr (X >= 0) {
+        const XE* x = static_cast<const XE*>(f.x);
+        float v[RW][8];
+        uint32_t mx[RW];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) mx[r] = 0;
+        const auto part = [&](int k0) {     // 512 elements of each of the wave's rows
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                const int row = wave + WV * r;
+                const XE* xr = x + (long long)row * f.ldx;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
+                if (row >= T) continue;
+                const int k = k0 + lane * 8;
+                if (f.vec && k + 8 <= K) {
+                    load8<X < 0 ? 0 : X>(xr + k, v[r]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k + e < K) v[r][e] = to_f32<X < 0 ? 0 : X>(xr[k + e]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[r][e] = slope(v[r][e], f.lrelu);
+        };
+        for (int k0 = 0; k0 < K; k0 += 512) {
+            part(k0);
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx[r] = max(mx[r], magnitude(v[r][e]));
+        }
+        float inv[RW];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            if (wave + WV * r >= T) continue;
+            const RowScale rs = row_scale(group_max(mx[r], 6));
+            inv[r] = rs.inv;
+            if (lane == 0) scales[wave + WV * r] = rs.scale;
+        }
+        for (int k0 = 0; k0 < K; k0 += 512) {
+            if (K > 512) part(k0);
+            const int k = k0 + lane * 8;
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+                if (wave + WV * r < T && k < K)
+                    *reinterpret_cast<uint2*>(few + (wave + WV * r) * stride + k) =
+                        uint2{four_codes(v[r][0], v[r][1], v[r][2], v[r][3], inv[r]), four_codes(v[r][4], v[r][5], v[r][6], v[r][7], inv[r])};
+        }
+    } else {
+        if (tid < 32) scales[tid] = a.qs[min(tid, T - 1)];
+    }
+    __syncthreads();
+    const int t = lane & 31, row = min(t, T - 1);      // rows past the end repeat the last one; what they give is not stored
+    i32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0;
+    for (int s = s0; s < s1; s += 4) {
+        if (s + 4 < s1) channels(s + 4, nxt);
+        i32x4 tok[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < s1) {
+                const int k = min((s + i) * 32 + 16 * half, end);
+                if constexpr (X >= 0) tok[i] = *reinterpret_cast<const i32x4*>(few + row * stride + k);
+                else tok[i] = *reinterpret_cast<const i32x4*>(a.q + row * a.ldq + k);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < s1) {
+                if ((s + i) * 32 + 32 > K) cur[i] = below(cur[i], K - (s + i) * 32 - 16 * half);
+                acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur[i], tok[i], acc, 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
+    }
+    __syncthreads();
+    i32x4* sums = reinterpret_cast<i32x4*>(few);       // [wave][four channels][lane]
+#pragma unroll
+    for (int g = 0; g < 4; ++g) sums[(wave * 4 + g) * 64 + lane] = i32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    __syncthreads();
+    if (wave >= 4 || t >= T) return;
+    i32x4 sum = sums[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < WV; ++w) sum += sums[(w * 4 + wave) * 64 + lane];
+    const float st = scales[t];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)sum[e] * st, ws[e], bs[e]);
+    Y* to = static_cast<Y*>(a.y) + t * a.ldy + ch;
+    if (a.align >= 4 * (int)sizeof(Y) && ch + 4 <= N) {
+        if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+        else *reinterpret_cast<uint2*>(to) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (ch + e < N) to[e] = from_f32<TYPE>(v[e]);
+    }
+}
+
 // ---- the fold -----------------------------------------------------------------------------------------------------
 // y: one row of 4 x 4 taps x C channels for each of B x H x W pixels; output pixel (oh, ow) of 2H x 2W is the sum of the
 // (up to) four taps (kh, kw) of pixels (ih, iw) with oh = 2 ih + kh - 1, ow = 2 iw + kw - 1.  An even row takes tap 1 of
@@ -546,27 +691,51 @@ __global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<T
 }
 
 // One channel: a lane an input pixel, for the 2 x 2 output pixels on it.  It reads what its column gives them -- taps of row 3
-// from the pixel above, 1 and 2 of its own, 0 of the one below -- sums them along the column, and takes from its left and
-// right neighbours their sums of column 3 and 0.  The first and last lane of a wave, whose neighbour is in another wave,
-// make that neighbour's sums themselves.
-template <int TYPE>
+// from the pixel above, 1 and 2 of its own, 0 of the one below, four at a time (VEC: y starts on a multiple of four
+// elements) -- sums them along the column, and takes from its left and right neighbours their sums of column 3 and 0.  The
+// first and last lane of a wave, whose neighbour is in another wave, make that neighbour's sums themselves.
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load_taps(const typename Elem<TYPE>::type* p, float (&v)[4]) {
+    if constexpr (VEC && TYPE == 0) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[e];
+    } else if constexpr (VEC) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        const uint16_t h[4] = {(uint16_t)x.x, (uint16_t)(x.x >> 16), (uint16_t)x.y, (uint16_t)(x.y >> 16)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_f32<TYPE>(__builtin_bit_cast(typename Elem<TYPE>::type, h[e]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_f32<TYPE>(p[e]);
+    }
+}
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void up_fold_one_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned i = blockIdx.x * 256 + threadIdx.x, n = a.pixels / 4, at = min(i, n - 1);
     const int H = a.H, W = a.W, lane = threadIdx.x & 63;
     const unsigned line = at / W, b = line / H;
     const int iw = (int)(at - line * W), ih = (int)(line - b * H);
     const bool up = ih > 0, down = ih + 1 < H;
-    const auto column = [&](long long p, int k, float& even, float& odd) {      // sums of column k of pixel p's taps
-        const typename Elem<TYPE>::type* t = y + p * 16 + k;
+    const auto* t = y + (long long)at * 16;
+    float r1[4], r2[4], r3[4] = {0.f, 0.f, 0.f, 0.f}, r0[4] = {0.f, 0.f, 0.f, 0.f};
+    load_taps<TYPE, VEC>(t + 4, r1);
+    load_taps<TYPE, VEC>(t + 8, r2);
+    if (up) load_taps<TYPE, VEC>(t + 12 - 16 * (long long)W, r3);
+    if (down) load_taps<TYPE, VEC>(t + 16 * (long long)W, r0);
+    float e[4], o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        e[k] = r1[k] + r3[k];
+        o[k] = r2[k] + r0[k];
+    }
+    const auto column = [&](const typename Elem<TYPE>::type* t, float& even, float& odd) {      // the sums of a neighbour's column
         even = to_f32<TYPE>(t[4]) + (up ? to_f32<TYPE>(t[12 - 16 * (long long)W]) : 0.f);
         odd = to_f32<TYPE>(t[8]) + (down ? to_f32<TYPE>(t[16 * (long long)W]) : 0.f);
     };
-    float e[4], o[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) column(at, k, e[k], o[k]);
     float le = __shfl_up(e[3], 1, 64), lo = __shfl_up(o[3], 1, 64), re = __shfl_down(e[0], 1, 64), ro = __shfl_down(o[0], 1, 64);
-    if (lane == 0 && iw > 0) column((long long)at - 1, 3, le, lo);
-    if (lane == 63 && iw + 1 < W) column((long long)at + 1, 0, re, ro);
+    if (lane == 0 && iw > 0) column(t - 16 + 3, le, lo);
+    if (lane == 63 && iw + 1 < W) column(t + 16, re, ro);
     if (i >= n) return;
     if (iw == 0) le = lo = 0.f;
     if (iw + 1 == W) re = ro = 0.f;
@@ -590,6 +759,8 @@ inline int row_align(const void* p, long long stride) {
     return u % 16 == 0 ? 16 : u % 8 == 0 ? 8 : u % 4 == 0 ? 4 : 2;
 }
 
+constexpr int FEW = 32, FEW_ELEMENTS = 32768;
+
 template <int FT, int FN, int WT, int WN, int TYPE>
 void launch_gemm(GemmArgs a, hipStream_t st) {
     a.tn = (a.N + 32 * FN * WN - 1) / (32 * FN * WN);
@@ -606,6 +777,26 @@ inline int by_type(int type, F f) {
         default: f(std::integral_constant<int, 2>{}); break;
     }
     return pgan_launch_status();
+}
+
+// What an operand covers; outputs may not share memory with anything else of the call.
+struct Span {
+    const void* p;
+    long long bytes;
+    bool written;
+};
+inline Span rows_of(const void* p, long long rows, long long cols, long long ld, int size, bool written = false) {
+    return Span{p, p ? ((rows - 1) * ld + cols) * size : 0, written};
+}
+template <int N>
+bool apart(const Span (&s)[N]) {
+    for (int i = 0; i < N; ++i)
+        for (int j = i + 1; j < N; ++j) {
+            if (!(s[i].written || s[j].written) || !s[i].bytes || !s[j].bytes) continue;
+            const uintptr_t a = reinterpret_cast<uintptr_t>(s[i].p), b = reinterpret_cast<uintptr_t>(s[j].p);
+            if (a < b + (uintptr_t)s[j].bytes && b < a + (uintptr_t)s[i].bytes) return false;
+        }
+    return true;
 }
 
 // lanes a row or an output pixel (as a power of two): eight elements each, all 64 for more than 256
@@ -630,12 +821,27 @@ int launch_fold(const void* y, int type, FoldArgs a, bool vec, hipStream_t st) {
     });
 }
 
+// up to 32 tokens, x (of type X) or their codes (X < 0)
+template <int X, int Y>
+void launch_few(const FewArgs& f, hipStream_t st) {
+    const int K = f.g.K, codes = X < 0 ? 0 : (int)f.g.T * ((K + 31) / 32 * 32 + 16);
+    const unsigned blocks = (unsigned)((f.g.N + 31) / 32);
+    // 16 waves where a wave of 4 would have 16 steps of 32 bytes or more to go through
+    if (K >= 2048) gemm_few_kernel<X, 16, 2, Y><<<blocks, 1024, std::max(codes, 16 * 4096), st>>>(f);
+    else if (X < 0 || f.g.T <= 4) gemm_few_kernel<X, 4, 1, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
+    else if (f.g.T <= 16) gemm_few_kernel<X, 4, X < 0 ? 1 : 4, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
+    else gemm_few_kernel<X, 4, X < 0 ? 1 : 8, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
+}
+
 inline int gemm_args(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
-                     const void* y, int y_type, long long ldy, long long T, int N, int K) {
+                     const float* bias, const void* y, int y_type, long long ldy, long long T, int N, int K) {
     if (T < 0 || N < 1 || K < 1 || K > 131072 || y_type < 0 || y_type > 2) return PGAN_EINVAL;
     if (T == 0) return PGAN_OK;
     if (!q || !q_scale || !w || !w_scale || !y || !aligned(q, 16) || !aligned(w, 16) || ldq % 16 || ldw % 16 || ldq < K
         || ldw < K || ldy < N || ldq > MAX_STRIDE || ldw > MAX_STRIDE || !aligned(y, type_bytes(y_type)))
+        return PGAN_EINVAL;
+    if (!apart({rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1), rows_of(q_scale, 1, T, 0, 4),
+                rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
     return (T + 255) / 256 * ((N + 255) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
 }
@@ -649,6 +855,8 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
     if (rows < 0 || K < 1 || x_type < 0 || x_type > 2) return PGAN_EINVAL;
     if (rows == 0) return PGAN_OK;
     if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4) || ldx < K || ldq < K) return PGAN_EINVAL;
+    if (!apart({rows_of(x, rows, K, ldx, type_bytes(x_type)), rows_of(q, rows, K, ldq, 1, true), rows_of(scale, 1, rows, 0, 4, true)}))
+        return PGAN_EINVAL;
     const bool vec = row_align(x, ldx * type_bytes(x_type)) == 16 && row_align(q, ldq) >= 8;
     const int log = lanes_log(K);    // lanes a row
     const long long blocks = (rows + (256 >> log) - 1) / (256 >> log);
@@ -669,7 +877,7 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
 
 int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
                  const float* bias, void* y, int y_type, long long ldy, long long T, int N, int K, hipStream_t st) {
-    const int rc = gemm_args(q, ldq, q_scale, w, ldw, w_scale, y, y_type, ldy, T, N, K);
+    const int rc = gemm_args(q, ldq, q_scale, w, ldw, w_scale, bias, y, y_type, ldy, T, N, K);
     if (rc || T == 0) return rc;
     return by_type(y_type, [&](auto t) {
         constexpr int Y = t.value;
@@ -680,7 +888,8 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         // 4096 x 4096 x 4096 in 256 x 256: 70 us (1960 Tera operations/s), 128 x 128: 84, 128 x 64: 97, 64 x 64: 115;
         // 64 x 4096 x 1024 (1 .. 16 tiles): 62, 32, 23, 16 us.  (One with two LDS buffers and one barrier a stage instead of
         // one and two was not faster: 70 us.)
-        if (N <= 32) launch_gemm<2, 1, 4, 1, Y>(a, st);
+        if (T <= FEW) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
+        else if (N <= 32) launch_gemm<2, 1, 4, 1, Y>(a, st);
         else if (tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, Y>(a, st);
         else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, Y>(a, st);
         else if (tiles(128, 64) >= 256) launch_gemm<2, 1, 2, 2, Y>(a, st);
@@ -691,8 +900,20 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
 int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long ldq, float* q_scale, const void* w,
                    long long ldw, const float* w_scale, const float* bias, void* y, int y_type, long long ldy, long long T,
                    int N, int K, int lrelu, hipStream_t st) {
-    const int ok = gemm_args(q, ldq, q_scale, w, ldw, w_scale, y, y_type, ldy, T, N, K);
+    const int ok = gemm_args(q, ldq, q_scale, w, ldw, w_scale, bias, y, y_type, ldy, T, N, K);
     if (ok || T == 0) return ok;
+    if (x_type < 0 || x_type > 2 || !x || ldx < K || !aligned(x, type_bytes(x_type))
+        || !apart({rows_of(x, T, K, ldx, type_bytes(x_type)), rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1, true),
+                   rows_of(q_scale, 1, T, 0, 4, true), rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
+        return PGAN_EINVAL;
+    if (T <= FEW && T * K <= FEW_ELEMENTS)
+        return by_type(x_type, [&](auto xt) {
+            (void)by_type(y_type, [&](auto t) {
+                const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0,
+                                 row_align(y, ldy * type_bytes(y_type))};
+                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, row_align(x, ldx * type_bytes(x_type)) == 16}, st);
+            });
+        });
     const int rc = pgan_quant_rows(x, x_type, ldx, q, ldq, q_scale, T, K, lrelu, st);
     return rc ? rc : pgan_gemm_q8(q, ldq, q_scale, w, ldw, w_scale, bias, y, y_type, ldy, T, N, K, st);
 }
@@ -702,7 +923,11 @@ int pgan_up_fold_q8(const void* y, int y_type, const float* shift, void* q, long
     if (!fold_fits(y_type, B, H, W, C)) return PGAN_EINVAL;
     if (B == 0) return PGAN_OK;
     if (!y || !q || !scale || ldq < C || !aligned(y, type_bytes(y_type)) || !aligned(scale, 4)) return PGAN_EINVAL;
-    FoldArgs a{shift, static_cast<int8_t*>(q), scale, nullptr, ldq, (unsigned)(4LL * B * H * W), H, W, C, 0, 0};
+    const long long pixels = 4LL * B * H * W;
+    if (!apart({rows_of(y, 1, pixels * 4 * C, 0, type_bytes(y_type)), rows_of(shift, 1, C, 0, 4), rows_of(q, pixels, C, ldq, 1, true),
+                rows_of(scale, 1, pixels, 0, 4, true)}))
+        return PGAN_EINVAL;
+    FoldArgs a{shift, static_cast<int8_t*>(q), scale, nullptr, ldq, (unsigned)pixels, H, W, C, 0, 0};
     return launch_fold<true>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && row_align(q, ldq) >= 8, st);
 }
 
@@ -711,10 +936,15 @@ int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int 
     if (!fold_fits(y_type, B, H, W, C) || act < 0 || act > 2) return PGAN_EINVAL;
     if (B == 0) return PGAN_OK;
     if (!y || !out || !aligned(y, type_bytes(y_type)) || !aligned(out, 4)) return PGAN_EINVAL;
-    FoldArgs a{shift, nullptr, nullptr, out, 0, (unsigned)(4LL * B * H * W), H, W, C, act, 0};
+    const long long pixels = 4LL * B * H * W;
+    if (!apart({rows_of(y, 1, pixels * 4 * C, 0, type_bytes(y_type)), rows_of(shift, 1, C, 0, 4), rows_of(out, 1, pixels * C, 0, 4, true)}))
+        return PGAN_EINVAL;
+    FoldArgs a{shift, nullptr, nullptr, out, 0, (unsigned)pixels, H, W, C, act, 0};
     if (C == 1)
         return by_type(y_type, [&](auto t) {
-            up_fold_one_kernel<t.value><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(static_cast<const typename Elem<t.value>::type*>(y), a);
+            const auto* p = static_cast<const typename Elem<t.value>::type*>(y);
+            if (aligned(y, 4 * type_bytes(y_type))) up_fold_one_kernel<t.value, true><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(p, a);
+            else up_fold_one_kernel<t.value, false><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(p, a);
         });
     return launch_fold<false>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && aligned(out, 16), st);
 }

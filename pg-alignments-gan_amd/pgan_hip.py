@@ -475,11 +475,11 @@ class AdamWPlan:
         ops = self.ops
         if len(grads) != self.n:
             raise PganError(f"adamw: {len(grads)} gradients for {self.n} parameters")
-        dev, kinds, gp = ops._device, [], []
+        dev, kinds, gp = ops._index, [], []
         for g, k in zip(grads, self.sizes):
-            if g.device != dev or g.numel() != k or not g.is_contiguous():
-                raise PganError(f"adamw: a gradient must be a contiguous tensor of its parameter's {k} elements on {dev}, got "
-                                f"{tuple(g.shape)} on {g.device}, contiguous: {g.is_contiguous()}")
+            if g.get_device() != dev or g.numel() != k or not g.is_contiguous():
+                raise PganError(f"adamw: a gradient must be a contiguous tensor of its parameter's {k} elements on cuda:{dev}, "
+                                f"got {tuple(g.shape)} on {g.device}, contiguous: {g.is_contiguous()}")
             kinds.append(g.dtype)
             gp.append(g.data_ptr())
         if kinds != self._types[0]:
@@ -491,7 +491,7 @@ class AdamWPlan:
             self._rates = (lr, weight_decay, self._per_tensor(lr, "lr"), self._per_tensor(weight_decay, "weight_decay"))
         sd = None
         if step_dev is not None:
-            if step_dev.device != dev or step_dev.dtype != torch.int32 or step_dev.numel() < 4 or not step_dev.is_contiguous():
+            if step_dev.get_device() != dev or step_dev.dtype != torch.int32 or step_dev.numel() < 4 or not step_dev.is_contiguous():
                 raise PganError("adamw: step_dev must be a contiguous int32 tensor of 4 elements on the device")
             sd = step_dev.data_ptr()
         elif step < 1:
@@ -996,7 +996,7 @@ class HipOps:
         return _raw_stream(self._index) if _raw_stream is not None else torch.cuda.current_stream(self._index).cuda_stream
 
     def _here(self, t, what):
-        if t.device != self._device:
+        if t.get_device() != self._index:
             raise PganError(f"{what} is on {t.device}, this backend works on {self._device}")
 
     def adamw_plan(self, params, m, v, scales=None) -> AdamWPlan:
@@ -1139,124 +1139,122 @@ class HipOps:
 
     # ---------------- products of 8-bit rows (evaluation only: no backward) ----------------
     def _float_rows(self, t, what):
-        """(pointer, type code, row stride) of a 2-D view with contiguous rows."""
-        self._here(t, what)
-        if t.dtype not in ELEMENT_TYPES or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise PganError(f"{what}: expected a 2-D float32, bfloat16 or float16 tensor with contiguous rows, got "
-                            f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-        ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-        if ld < t.shape[1]:
-            raise PganError(f"{what}: rows overlap (stride {ld} for {t.shape[1]} columns)")
-        return t.data_ptr(), ELEMENT_TYPES[t.dtype], ld
+        """(pointer, type code, rows, columns, row stride) of a 2-D view with contiguous rows."""
+        kind = ELEMENT_TYPES.get(t.dtype)
+        if t.get_device() != self._index:
+            self._here(t, what)
+        if kind is None or t.dim() != 2:
+            raise PganError(f"{what}: expected a 2-D float32, bfloat16 or float16 tensor, got {t.dtype} {tuple(t.shape)}")
+        rows, cols = t.shape
+        ld, one = t.stride()
+        if one != 1 and cols > 1:
+            raise PganError(f"{what}: the elements of a row must be neighbours, strides are {t.stride()}")
+        if rows < 2:
+            ld = cols
+        elif ld < cols:
+            raise PganError(f"{what}: rows overlap (stride {ld} for {cols} columns)")
+        return t.data_ptr(), kind, rows, cols, ld
 
     def _code_rows(self, t, what, rows, cols):
         """(pointer, row stride) of 8-bit rows: on 16-byte borders, readable up to a multiple of 16."""
-        self._here(t, what)
+        if t.get_device() != self._index:
+            self._here(t, what)
         if t.dtype != torch.int8 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
             raise PganError(f"{what}: expected int8 rows [{rows}, {cols}], got {t.dtype} {tuple(t.shape)} with strides "
                             f"{t.stride()}")
         wide = (cols + 15) // 16 * 16
         ld = t.stride(0) if t.shape[0] > 1 else wide
-        if t.data_ptr() % 16 or ld % 16 or ld < cols:
+        p = t.data_ptr()
+        if p % 16 or ld % 16 or ld < cols:
             raise PganError(f"{what}: rows must start on 16-byte borders (pgan_hip.rows8 makes such a buffer)")
-        if rows and t.storage_offset() + (rows - 1) * ld + wide > t.untyped_storage().nbytes():
+        if rows and wide != cols and t.storage_offset() + (rows - 1) * ld + wide > t.untyped_storage().nbytes():
             raise PganError(f"{what}: the last row is not readable up to a multiple of 16 bytes")
-        return t.data_ptr(), ld
+        return p, ld
 
     def _scales(self, t, what, n):
-        self._here(t, what)
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+        if t.get_device() != self._index:
+            self._here(t, what)
+        if t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous():
             raise PganError(f"{what}: expected a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
         return t.data_ptr()
 
     @staticmethod
-    def _apart(*named):
-        """Refuses outputs that share memory with another operand."""
-        spans = []
-        for what, t, written in named:
-            if t is not None and t.numel():
-                lo = t.data_ptr()
-                last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-                spans.append((lo, lo + (last + 1) * t.element_size(), written, what))
-        spans.sort()
-        top = (0, 0, False, "")
-        for s in spans:
-            if s[0] < top[1] and (s[2] or top[2]):
-                raise PganError(f"{top[3]} and {s[3]} share memory")
-            if s[1] > top[1]:
-                top = s
+    def _refused(rc, what, **tensors):
+        """The error of an entry point that refused arguments which passed the checks here: operands that share memory with
+        an output, or a size beyond what it takes."""
+        shapes = ", ".join(f"{k} {tuple(t.shape)} at {t.data_ptr():#x}" for k, t in tensors.items() if t is not None)
+        if rc == -1:
+            raise PganError(f"{what}: an output shares memory with another operand, or the sizes are beyond what the entry point "
+                            f"takes ({shapes})")
+        _check(rc, what)
 
     def quant_rows(self, x, q, scale, lrelu: bool = False) -> None:
         """Codes and scale of each row of x [T, K] (after LeakyReLU(0.1) if lrelu): q int8 [T, K], scale float32 [T] with
         x ~ q * scale.  A row that holds an infinity or a NaN gets codes 0 and the scale NaN."""
-        xp, xt, ldx = self._float_rows(x, "quant_rows: x")
-        T, K = x.shape
+        xp, xt, T, K, ldx = self._float_rows(x, "quant_rows: x")
         if K < 1:
             raise PganError("quant_rows: rows without elements have no scale")
         qp, ldq = self._code_rows(q, "quant_rows: q", T, K)
-        sp = self._scales(scale, "quant_rows: scale", T)
-        self._apart(("x", x, False), ("q", q, True), ("scale", scale, True))
-        _check(_lib.pgan_quant_rows(xp, xt, ldx, qp, ldq, sp, T, K, int(bool(lrelu)), self._own_stream()), "pgan_quant_rows")
+        rc = _lib.pgan_quant_rows(xp, xt, ldx, qp, ldq, self._scales(scale, "quant_rows: scale", T), T, K, int(lrelu),
+                                  self._own_stream())
+        if rc:
+            self._refused(rc, "pgan_quant_rows", x=x, q=q, scale=scale)
 
-    def _product_args(self, what, K, w, w_scale, y, bias):
-        yp, yt, ldy = self._float_rows(y, f"{what}: y")
-        T, N = y.shape
+    def _product_args(self, what, T, K, w, w_scale, y, bias):
+        yp, yt, ty, N, ldy = self._float_rows(y, f"{what}: y")
+        if ty != T or w.shape[0] != N or K < 1 or N < 1 or (bias is not None and bias.numel() != N):
+            raise PganError(f"{what}: {T} rows of {K} elements, w {tuple(w.shape)}, bias "
+                            f"{None if bias is None else tuple(bias.shape)} and y {tuple(y.shape)} do not fit together")
         wp, ldw = self._code_rows(w, f"{what}: w", N, K)
-        if w.shape[0] != N or (bias is not None and bias.numel() != N) or K < 1 or N < 1:
-            raise PganError(f"{what}: w {tuple(w.shape)} and bias do not fit y {tuple(y.shape)} and {K} inner elements")
-        return T, N, wp, ldw, self._scales(w_scale, f"{what}: w_scale", N), \
+        return N, wp, ldw, self._scales(w_scale, f"{what}: w_scale", N), \
             None if bias is None else self._scales(bias, f"{what}: bias", N), yp, yt, ldy
 
     def gemm_q8(self, q, q_scale, w, w_scale, y, bias=None) -> None:
         """y [T, N] = q_scale[t] w_scale[n] sum_k q[t, k] w[n, k] + bias[n]: q int8 [T, K], w int8 [N, K], y float32, bfloat16
         or float16; the sum is exact (K <= 131072)."""
-        K = q.shape[1]
-        T, N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("gemm_q8", K, w, w_scale, y, bias)
-        if q.shape[0] != T:
-            raise PganError(f"gemm_q8: {q.shape[0]} rows of q for {T} of y")
+        T, K = q.shape
+        N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("gemm_q8", T, K, w, w_scale, y, bias)
         qp, ldq = self._code_rows(q, "gemm_q8: q", T, K)
-        qs = self._scales(q_scale, "gemm_q8: q_scale", T)
-        self._apart(("y", y, True), ("q", q, False), ("q_scale", q_scale, False), ("w", w, False), ("w_scale", w_scale, False),
-                    ("bias", bias, False))
-        _check(_lib.pgan_gemm_q8(qp, ldq, qs, wp, ldw, ws, bp, yp, yt, ldy, T, N, K, self._own_stream()), "pgan_gemm_q8")
+        rc = _lib.pgan_gemm_q8(qp, ldq, self._scales(q_scale, "gemm_q8: q_scale", T), wp, ldw, ws, bp, yp, yt, ldy, T, N, K,
+                               self._own_stream())
+        if rc:
+            self._refused(rc, "pgan_gemm_q8", q=q, q_scale=q_scale, w=w, w_scale=w_scale, y=y, bias=bias)
 
     def linear_q8(self, x, w, w_scale, y, q, q_scale, bias=None, lrelu: bool = False) -> None:
         """quant_rows(x) and gemm_q8 in one call.  q int8 [at least T, K] and q_scale [at least T] are scratch of the caller:
         what they hold afterwards is not part of the result (few tokens skip them)."""
-        xp, xt, ldx = self._float_rows(x, "linear_q8: x")
-        K = x.shape[1]
-        T, N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("linear_q8", K, w, w_scale, y, bias)
-        if x.shape[0] != T:
-            raise PganError(f"linear_q8: {x.shape[0]} rows of x for {T} of y")
+        xp, xt, T, K, ldx = self._float_rows(x, "linear_q8: x")
+        N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("linear_q8", T, K, w, w_scale, y, bias)
         qp, ldq = self._code_rows(q, "linear_q8: q", T, K)
-        qs = self._scales(q_scale, "linear_q8: q_scale", T)
-        self._apart(("y", y, True), ("q", q, True), ("q_scale", q_scale, True), ("x", x, False), ("w", w, False),
-                    ("w_scale", w_scale, False), ("bias", bias, False))
-        _check(_lib.pgan_linear_q8(xp, xt, ldx, qp, ldq, qs, wp, ldw, ws, bp, yp, yt, ldy, T, N, K, int(bool(lrelu)),
-                                   self._own_stream()), "pgan_linear_q8")
+        rc = _lib.pgan_linear_q8(xp, xt, ldx, qp, ldq, self._scales(q_scale, "linear_q8: q_scale", T), wp, ldw, ws, bp, yp, yt, ldy,
+                                 T, N, K, int(lrelu), self._own_stream())
+        if rc:
+            self._refused(rc, "pgan_linear_q8", x=x, w=w, w_scale=w_scale, y=y, q=q, q_scale=q_scale, bias=bias)
 
     def _fold_args(self, what, y, shift, C):
+        kind = ELEMENT_TYPES.get(y.dtype)
         self._here(y, f"{what}: y")
-        if y.dtype not in ELEMENT_TYPES or y.dim() != 4 or not y.is_contiguous() or y.shape[3] != 16 * C or C < 1:
+        if kind is None or y.dim() != 4 or not y.is_contiguous() or y.shape[3] != 16 * C or C < 1:
             raise PganError(f"{what}: y must be a contiguous [B, H, W, 16 * {C}] tensor of float32, bfloat16 or float16, got "
                             f"{y.dtype} {tuple(y.shape)}")
         if shift is not None and shift.numel() != C:
             raise PganError(f"{what}: {shift.numel()} shifts for {C} channels")
-        return y.data_ptr(), ELEMENT_TYPES[y.dtype], None if shift is None else self._scales(shift, f"{what}: shift", C)
+        return y.data_ptr(), kind, None if shift is None else self._scales(shift, f"{what}: shift", C)
 
     def up_fold_q8(self, y, shift, q, scale) -> None:
         """y [B, H, W, (kh, kw, c)]: the taps of ConvTranspose2d(kernel 4, stride 2, padding 1) made as a product.  Sums the
         taps of each output pixel, adds shift[c] (or None), applies LeakyReLU(0.1) and writes the pixel's codes: q int8
         [B * 2H * 2W, C], scale [B * 2H * 2W]."""
-        C = q.shape[1]
+        pixels, C = q.shape
         yp, yt, hp = self._fold_args("up_fold_q8", y, shift, C)
-        B, H, W = y.shape[:3]
-        if q.shape[0] != 4 * B * H * W:
-            raise PganError(f"up_fold_q8: q has {q.shape[0]} rows for {4 * B * H * W} pixels")
-        qp, ldq = self._code_rows(q, "up_fold_q8: q", 4 * B * H * W, C)
-        sp = self._scales(scale, "up_fold_q8: scale", 4 * B * H * W)
-        self._apart(("q", q, True), ("scale", scale, True), ("y", y, False), ("shift", shift, False))
-        _check(_lib.pgan_up_fold_q8(yp, yt, hp, qp, ldq, sp, B, H, W, C, self._own_stream()), "pgan_up_fold_q8")
+        B, H, W, _ = y.shape
+        if pixels != 4 * B * H * W:
+            raise PganError(f"up_fold_q8: q has {pixels} rows for {4 * B * H * W} pixels")
+        qp, ldq = self._code_rows(q, "up_fold_q8: q", pixels, C)
+        rc = _lib.pgan_up_fold_q8(yp, yt, hp, qp, ldq, self._scales(scale, "up_fold_q8: scale", pixels), B, H, W, C,
+                                  self._own_stream())
+        if rc:
+            self._refused(rc, "pgan_up_fold_q8", y=y, shift=shift, q=q, scale=scale)
 
     def up_fold(self, y, shift, out, act: int = 0) -> None:
         """As up_fold_q8, into float32 out [B, 2H, 2W, C] through act: 0 none, 1 sigmoid, 2 tanh."""
@@ -1264,14 +1262,15 @@ class HipOps:
             raise PganError(f"up_fold: out must be [B, 2H, 2W, C], got {tuple(out.shape)}")
         C = out.shape[3]
         yp, yt, hp = self._fold_args("up_fold", y, shift, C)
-        B, H, W = y.shape[:3]
+        B, H, W, _ = y.shape
         if tuple(out.shape) != (B, 2 * H, 2 * W, C):
             raise PganError(f"up_fold: out is {tuple(out.shape)} for y {tuple(y.shape)}")
         if act not in (0, 1, 2):
             raise PganError(f"up_fold: act is 0, 1 or 2, got {act}")
-        op = self._scales(out, "up_fold: out", out.numel())
-        self._apart(("out", out, True), ("y", y, False), ("shift", shift, False))
-        _check(_lib.pgan_up_fold(yp, yt, hp, op, B, H, W, C, int(act), self._own_stream()), "pgan_up_fold")
+        rc = _lib.pgan_up_fold(yp, yt, hp, self._scales(out, "up_fold: out", 4 * B * H * W * C), B, H, W, C, int(act),
+                               self._own_stream())
+        if rc:
+            self._refused(rc, "pgan_up_fold", y=y, shift=shift, out=out)
 
     def convt1d_up(self, y, w, x, act=0):
         N, Cs, Ls = y.shape

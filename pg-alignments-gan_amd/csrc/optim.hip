@@ -70,203 +70,261 @@ __device__ __forceinline__ uint16_t to16(float x, int type) {
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// four elements of a tensor from i on; VEC: one access, else those below n one by one
+// Four elements of a tensor: o (a lane's) past b, which is the same for the whole wave and stays in scalar registers.  VEC: one
+// access, else those below n one by one.
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void load4(const void* src, long long i, long long n, float (&o)[4]) {
+__device__ __forceinline__ void load4(const void* src, long long b, int o, long long n, float (&v)[4]) {
     if constexpr (TYPE == 0) {
-        const float* s = static_cast<const float*>(src);
+        const float* s = static_cast<const float*>(src) + b;
         if constexpr (VEC) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(s + i);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(s + o);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = x[e];
+            for (int e = 0; e < 4; ++e) v[e] = x[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = i + e < n ? s[i + e] : 0.f;
+            for (int e = 0; e < 4; ++e) v[e] = b + o + e < n ? s[o + e] : 0.f;
         }
     } else {
-        const uint16_t* s = static_cast<const uint16_t*>(src);
+        const uint16_t* s = static_cast<const uint16_t*>(src) + b;
         if constexpr (VEC) {
-            const uint2 x = *reinterpret_cast<const uint2*>(s + i);
-            o[0] = from16((uint16_t)x.x, TYPE);
-            o[1] = from16((uint16_t)(x.x >> 16), TYPE);
-            o[2] = from16((uint16_t)x.y, TYPE);
-            o[3] = from16((uint16_t)(x.y >> 16), TYPE);
+            const uint2 x = *reinterpret_cast<const uint2*>(s + o);
+            if constexpr (TYPE == 1) {
+                v[0] = __builtin_bit_cast(float, x.x << 16);
+                v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
+                v[2] = __builtin_bit_cast(float, x.y << 16);
+                v[3] = __builtin_bit_cast(float, x.y & 0xffff0000u);
+            } else {
+                v[0] = from16((uint16_t)x.x, TYPE);
+                v[1] = from16((uint16_t)(x.x >> 16), TYPE);
+                v[2] = from16((uint16_t)x.y, TYPE);
+                v[3] = from16((uint16_t)(x.y >> 16), TYPE);
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = i + e < n ? from16(s[i + e], TYPE) : 0.f;
+            for (int e = 0; e < 4; ++e) v[e] = b + o + e < n ? from16(s[o + e], TYPE) : 0.f;
         }
     }
 }
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void store4(void* dst, long long i, long long n, const float (&o)[4]) {
+__device__ __forceinline__ void store4(void* dst, long long b, int o, long long n, const float (&v)[4]) {
     if constexpr (TYPE == 0) {
-        float* d = static_cast<float*>(dst);
+        float* d = static_cast<float*>(dst) + b;
         if constexpr (VEC) {
-            *reinterpret_cast<f32x4*>(d + i) = f32x4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f32x4*>(d + o) = f32x4{v[0], v[1], v[2], v[3]};
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (i + e < n) d[i + e] = o[e];
+                if (b + o + e < n) d[o + e] = v[e];
         }
     } else {
-        uint16_t* d = static_cast<uint16_t*>(dst);
+        uint16_t* d = static_cast<uint16_t*>(dst) + b;
         if constexpr (VEC) {
-            uint2 x;
-            x.x = (uint32_t)to16(o[0], TYPE) | (uint32_t)to16(o[1], TYPE) << 16;
-            x.y = (uint32_t)to16(o[2], TYPE) | (uint32_t)to16(o[3], TYPE) << 16;
-            *reinterpret_cast<uint2*>(d + i) = x;
+            using H = std::conditional_t<TYPE == 1, __bf16, _Float16>;
+            typedef H h2 __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<uint2*>(d + o) =
+                uint2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})};
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (i + e < n) d[i + e] = to16(o[e], TYPE);
+                if (b + o + e < n) d[o + e] = to16(v[e], TYPE);
         }
     }
 }
 template <bool VEC>
-__device__ __forceinline__ uint32_t load_codes(const void* src, long long i, long long n) {
-    const uint8_t* s = static_cast<const uint8_t*>(src);
-    if constexpr (VEC) return *reinterpret_cast<const uint32_t*>(s + i);
+__device__ __forceinline__ uint32_t load_codes(const void* src, long long b, int o, long long n) {
+    const uint8_t* s = static_cast<const uint8_t*>(src) + b;
+    if constexpr (VEC) return *reinterpret_cast<const uint32_t*>(s + o);
     uint32_t u = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (i + e < n) u |= (uint32_t)s[i + e] << (8 * e);
+        if (b + o + e < n) u |= (uint32_t)s[o + e] << (8 * e);
     return u;
 }
 template <bool VEC>
-__device__ __forceinline__ void store_codes(void* dst, long long i, long long n, uint32_t u) {
-    uint8_t* d = static_cast<uint8_t*>(dst);
+__device__ __forceinline__ void store_codes(void* dst, long long b, int o, long long n, uint32_t u) {
+    uint8_t* d = static_cast<uint8_t*>(dst) + b;
     if constexpr (VEC) {
-        *reinterpret_cast<uint32_t*>(d + i) = u;
+        *reinterpret_cast<uint32_t*>(d + o) = u;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (i + e < n) d[i + e] = (uint8_t)(u >> (8 * e));
+            if (b + o + e < n) d[o + e] = (uint8_t)(u >> (8 * e));
     }
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-    v = __builtin_fmaxf(v, dpp_move<0xB1>(v));
-    v = __builtin_fmaxf(v, dpp_move<0x4E>(v));
-    v = __builtin_fmaxf(v, dpp_move<0x141>(v));
-    v = __builtin_fmaxf(v, dpp_move<0x140>(v));
-    v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
-    return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
-__device__ __forceinline__ int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23) - 127; }
 __device__ __forceinline__ bool finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) != 0x7f800000u; }
 
 // e4m3 code of y in [0, 256), u in [0, 2^16): the low 20 bits of the fp32 pattern are the part of a step that is decided by
 // the random bits.  Below the smallest normal code the steps are even: adding 2^-6 there gives the pattern the same form.
 __device__ __forceinline__ uint32_t encode(float y, uint32_t u) {
     const bool small = y < 0x1p-6f;
-    const uint32_t bits = __builtin_bit_cast(uint32_t, small ? y + 0x1p-6f : y);
-    return ((bits + (u << 4) + 8u) >> 20) - (small ? 968u : 960u);
+    const uint32_t bits = __builtin_bit_cast(uint32_t, small ? y + 0x1p-6f : y), zero = (small ? 0u - (968u << 20) : 0u - (960u << 20)) + 8u;
+    return (bits + (u << 4) + zero) >> 20;
 }
 
 struct AwStep {
     float size, keep, b1, c1, b2, c2, eps, gs, inv2;
 };
+// Square root rounded to the nearest: the hardware's is within one unit of it, and the sign of x - s s' for the two values
+// s' next to s says which of the three is nearest.
+__device__ __forceinline__ float root_of(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float lo = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1), hi = __builtin_bit_cast(float, __builtin_bit_cast(int, s) + 1);
+    float r = __builtin_fmaf(-lo, s, x) <= 0.f ? lo : s;
+    r = __builtin_fmaf(-hi, s, x) > 0.f ? hi : r;
+    return r;           // s itself for zero, infinity and NaN: one of s' is no number there, and no comparison holds
+}
+// p is rounded to its own type once more than anything here errs: the quotient is a product with the hardware's reciprocal
+// (one unit off at most).
 __device__ __forceinline__ void update(const AwStep& s, float& p, float g, float& m, float& v, float& root) {
     g = g * s.gs;
     m = m * s.b1 + g * s.c1;
     v = v * s.b2 + (g * g) * s.c2;
-    root = sqrtf(v);
-    p = p * s.keep - (m * s.size) / (root * s.inv2 + s.eps);
+    root = root_of(v);
+    p = __builtin_fmaf(-(m * s.size), __builtin_amdgcn_rcpf(__builtin_fmaf(root, s.inv2, s.eps)), p * s.keep);
 }
 
 template <int PT, int GT, bool VEC>
-__device__ __forceinline__ void body32(const AwTensor& t, const AwStep& s, long long i) {
+__device__ __forceinline__ void body32(const AwTensor& t, const AwStep& s, long long b, int o) {
     float p[4], g[4], m[4], v[4], root;
-    load4<PT, VEC>(t.p, i, t.n, p);
-    load4<GT, VEC>(t.g, i, t.n, g);
-    load4<0, VEC>(t.m, i, t.n, m);
-    load4<0, VEC>(t.v, i, t.n, v);
+    load4<PT, VEC>(t.p, b, o, t.n, p);
+    load4<GT, VEC>(t.g, b, o, t.n, g);
+    load4<0, VEC>(t.m, b, o, t.n, m);
+    load4<0, VEC>(t.v, b, o, t.n, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) update(s, p[e], g[e], m[e], v[e], root);
-    store4<PT, VEC>(t.p, i, t.n, p);
-    store4<0, VEC>(t.m, i, t.n, m);
-    store4<0, VEC>(t.v, i, t.n, v);
+    store4<PT, VEC>(t.p, b, o, t.n, p);
+    store4<0, VEC>(t.m, b, o, t.n, m);
+    store4<0, VEC>(t.v, b, o, t.n, v);
 }
 
-// one block of 256 elements by one wave, four elements a lane; i: the lane's first element
-template <int PT, int GT, bool VEC>
-__device__ __forceinline__ void body8(const AwTensor& t, const AwStep& s, long long i, uint32_t key) {
-    const long long blk = i / AW_BLOCK;
-    float p[4], g[4], m[4], v[4], r[4];
-    load4<PT, VEC>(t.p, i, t.n, p);
-    load4<GT, VEC>(t.g, i, t.n, g);
-    const uint32_t cm = load_codes<VEC>(t.m, i, t.n), cv = load_codes<VEC>(t.v, i, t.n);
-    const float ms = t.ms[blk], rs = t.rs[blk];
-    m[0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0) * ms;
-    m[1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1) * ms;
-    m[2] = __builtin_amdgcn_cvt_f32_fp8(cm, 2) * ms;
-    m[3] = __builtin_amdgcn_cvt_f32_fp8(cm, 3) * ms;
-    v[0] = __builtin_amdgcn_cvt_f32_fp8(cv, 0) * rs;
-    v[1] = __builtin_amdgcn_cvt_f32_fp8(cv, 1) * rs;
-    v[2] = __builtin_amdgcn_cvt_f32_fp8(cv, 2) * rs;
-    v[3] = __builtin_amdgcn_cvt_f32_fp8(cv, 3) * rs;
-    float mmax = 0.f, vmax = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = v[e] * v[e];
-        update(s, p[e], g[e], m[e], v[e], r[e]);
-        if (finite(m[e])) mmax = __builtin_fmaxf(mmax, __builtin_fabsf(m[e]));
-        if (finite(v[e])) vmax = __builtin_fmaxf(vmax, v[e]);
-    }
-    store4<PT, VEC>(t.p, i, t.n, p);
-    mmax = wave_max(mmax);
-    vmax = wave_max(vmax);
-    const int em = max(exponent(mmax), -100) - 7, er = (max(exponent(vmax), -126) >> 1) - 7;
-    const float im = pow2(-em), ir = pow2(-er);
-    uint32_t nm = 0, nr = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t h = mix(key ^ (uint32_t)(i + e));
-        uint32_t a = encode(__builtin_fabsf(m[e]) * im, h & 0xffffu);
-        uint32_t b = encode(r[e] * ir, h >> 16);
-        b = (v[e] > 0.f && b == 0) ? 1u : b;
-        a = finite(m[e]) ? a : 0x7fu;
-        b = finite(v[e]) ? b : 0x7fu;
-        nm |= (a | (__builtin_bit_cast(uint32_t, m[e]) >> 31) << 7) << (8 * e);
-        nr |= b << (8 * e);
-    }
-    store_codes<VEC>(t.m, i, t.n, nm);
-    store_codes<VEC>(t.v, i, t.n, nr);
-    if ((threadIdx.x & 63) == 0) {
-        t.ms[blk] = pow2(em);
-        t.rs[blk] = pow2(er);
-    }
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    const auto step = [](uint32_t v, uint32_t o) { return max(v, o); };
+    v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+    v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+    v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+    v = step(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+    v = step(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+    return step(v, (uint32_t)__shfl_xor((int)v, 32, 64));
 }
+
+// one block of 256 elements by one wave, four elements a lane from i on
+template <int PT, int GT, bool VEC>
+struct Block8 {
+    float p[4], g[4], ms, rs;
+    uint32_t cm, cv;
+    __device__ __forceinline__ void load(const AwTensor& t, long long i, int o) {
+        load4<PT, VEC>(t.p, i, o, t.n, p);
+        load4<GT, VEC>(t.g, i, o, t.n, g);
+        cm = load_codes<VEC>(t.m, i, o, t.n);
+        cv = load_codes<VEC>(t.v, i, o, t.n);
+        ms = t.ms[i / AW_BLOCK];
+        rs = t.rs[i / AW_BLOCK];
+    }
+    __device__ __forceinline__ void step(const AwTensor& t, const AwStep& s, long long i, int o, uint32_t key) {
+        float m[4], v[4], r[4];
+        m[0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0) * ms;
+        m[1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1) * ms;
+        m[2] = __builtin_amdgcn_cvt_f32_fp8(cm, 2) * ms;
+        m[3] = __builtin_amdgcn_cvt_f32_fp8(cm, 3) * ms;
+        v[0] = __builtin_amdgcn_cvt_f32_fp8(cv, 0) * rs;
+        v[1] = __builtin_amdgcn_cvt_f32_fp8(cv, 1) * rs;
+        v[2] = __builtin_amdgcn_cvt_f32_fp8(cv, 2) * rs;
+        v[3] = __builtin_amdgcn_cvt_f32_fp8(cv, 3) * rs;
+        // magnitudes are compared as patterns: infinities and NaN come out on top, and only then are they looked for
+        uint32_t mmax = 0, vmax = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = v[e] * v[e];
+            update(s, p[e], g[e], m[e], v[e], r[e]);
+            mmax = max(mmax, __builtin_bit_cast(uint32_t, m[e]) & 0x7fffffffu);
+            vmax = max(vmax, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+        }
+        store4<PT, VEC>(t.p, i, o, t.n, p);
+        mmax = wave_max(mmax);
+        vmax = wave_max(vmax);
+        const bool odd = __builtin_amdgcn_readfirstlane(max(mmax, vmax)) >= 0x7f800000;
+        uint32_t no_m = 0, no_v = 0;        // codes of what is not finite, which counts as zero in what follows
+        if (odd) {
+            mmax = vmax = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!finite(m[e])) {
+                    no_m |= 0x7fu << (8 * e);
+                    m[e] = __builtin_copysignf(0.f, m[e]);
+                }
+                if (!finite(v[e])) {
+                    no_v |= 0x7fu << (8 * e);
+                    v[e] = r[e] = 0.f;
+                }
+                mmax = max(mmax, __builtin_bit_cast(uint32_t, m[e]) & 0x7fffffffu);
+                vmax = max(vmax, __builtin_bit_cast(uint32_t, v[e]));
+            }
+            mmax = wave_max(mmax);
+            vmax = wave_max(vmax);
+        }
+        const int em = max((int)(mmax >> 23) - 127, -100) - 7, er = (max((int)(vmax >> 23) - 127, -126) >> 1) - 7;
+        const float im = pow2(-em), ir = pow2(-er);
+        uint32_t nm = no_m, nr = no_v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t h = mix(key ^ ((uint32_t)i + (uint32_t)(o + e)));
+            const uint32_t a = encode(__builtin_fabsf(m[e]) * im, h & 0xffffu);
+            const uint32_t b = max(encode(r[e] * ir, h >> 16), min(__builtin_bit_cast(uint32_t, v[e]), 1u));
+            nm |= (a | ((__builtin_bit_cast(uint32_t, m[e]) >> 24) & 0x80u)) << (8 * e);
+            nr |= b << (8 * e);
+        }
+        store_codes<VEC>(t.m, i, o, t.n, nm);
+        store_codes<VEC>(t.v, i, o, t.n, nr);
+        if ((threadIdx.x & 63) == 0) {
+            t.ms[i / AW_BLOCK] = pow2(em);
+            t.rs[i / AW_BLOCK] = pow2(er);
+        }
+    }
+};
 
 template <int BITS, int PT, int GT>
 __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long long at, bool vec, uint32_t key) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (BITS == 32) {
 #pragma unroll
         for (int u = 0; u < AW_CHUNK / 1024; ++u) {
-            const long long i = at + u * 1024 + threadIdx.x * 4;
-            if (i >= t.n) continue;
-            if (vec && i + 4 <= t.n) body32<PT, GT, true>(t, s, i);
-            else body32<PT, GT, false>(t, s, i);
+            const long long b = at + u * 1024 + wave * 256;
+            if (vec && b + 256 <= t.n) {
+                body32<PT, GT, true>(t, s, b, lane * 4);
+            } else if (b + lane * 4 < t.n) {
+                body32<PT, GT, false>(t, s, b, lane * 4);
+            }
         }
     } else {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-        for (int u = 0; u < AW_CHUNK / 1024; ++u) {
-            const long long b = at + u * 1024 + wave * AW_BLOCK;        // the same for all lanes of the wave
-            if (b >= t.n) continue;
-            if (vec && b + AW_BLOCK <= t.n) body8<PT, GT, true>(t, s, b + lane * 4, key);
-            else body8<PT, GT, false>(t, s, b + lane * 4, key);
+        // two blocks of 256 a wave, the second one's reads under way while the first is computed
+        const long long b = at + wave * (2 * AW_BLOCK);
+        if (vec && b + 2 * AW_BLOCK <= t.n) {
+            Block8<PT, GT, true> x, y;
+            x.load(t, b, lane * 4);
+            y.load(t, b + AW_BLOCK, lane * 4);
+            x.step(t, s, b, lane * 4, key);
+            y.step(t, s, b + AW_BLOCK, lane * 4, key);
+        } else {
+            for (int u = 0; u < 2; ++u) {
+                const long long i = b + u * AW_BLOCK;
+                if (i >= t.n) break;
+                Block8<PT, GT, false> x;
+                x.load(t, i, lane * 4);
+                x.step(t, s, i, lane * 4, key);
+            }
         }
     }
 }
 
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(const AwArgs a) {
-    int k = 0;
-    for (int i = 1; i < a.n; ++i) k = blockIdx.x >= a.first[i] ? i : k;
+    // the block's tensor: the lanes compare it with every tensor's first chunk at once
+    const int lane = threadIdx.x & 63;
+    const unsigned first = lane < a.n ? a.first[lane] : 0xffffffffu;
+    const int k = __builtin_popcountll(__ballot(first <= blockIdx.x)) - 1;
     const AwTensor& t = a.t[k];
     const long long at = (long long)(blockIdx.x - a.first[k]) * AW_CHUNK;
     AwStep s{t.size, t.keep, a.b1, a.c1, a.b2, a.c2, a.eps, a.gs, a.inv2};

@@ -459,6 +459,7 @@ class AdamWPlan:
         self._ms, self._rs = (None, None) if scales is None else (ptrs(scales[0]), ptrs(scales[1]))
         self._numel = (c_longlong * n)(*self.sizes)
         self._rates = (None, None, None, None)
+        self._devices = [ops._index] * n
         self._types = (None, None)
 
     def _per_tensor(self, x, what):
@@ -475,13 +476,15 @@ class AdamWPlan:
         ops = self.ops
         if len(grads) != self.n:
             raise PganError(f"adamw: {len(grads)} gradients for {self.n} parameters")
-        dev, kinds, gp = ops._index, [], []
-        for g, k in zip(grads, self.sizes):
-            if g.get_device() != dev or g.numel() != k or not g.is_contiguous():
-                raise PganError(f"adamw: a gradient must be a contiguous tensor of its parameter's {k} elements on cuda:{dev}, "
-                                f"got {tuple(g.shape)} on {g.device}, contiguous: {g.is_contiguous()}")
-            kinds.append(g.dtype)
-            gp.append(g.data_ptr())
+        dev, T = ops._index, torch.Tensor
+        if (list(map(T.numel, grads)) != self.sizes or list(map(T.get_device, grads)) != self._devices
+                or not all(map(T.is_contiguous, grads))):
+            for i, (g, k) in enumerate(zip(grads, self.sizes)):
+                ops._here(g, f"adamw: gradient {i}")
+                if g.numel() != k or not g.is_contiguous():
+                    raise PganError(f"adamw: gradient {i} must be a contiguous tensor of its parameter's {k} elements, got "
+                                    f"{tuple(g.shape)} with strides {g.stride()}")
+        kinds = [g.dtype for g in grads]
         if kinds != self._types[0]:
             try:
                 self._types = (kinds, self._it(*[p + 3 * ELEMENT_TYPES[k] for p, k in zip(self._ptypes, kinds)]))
@@ -496,7 +499,7 @@ class AdamWPlan:
             sd = step_dev.data_ptr()
         elif step < 1:
             raise PganError(f"adamw: steps count from 1, got {step}")
-        _check(_lib.pgan_adamw_multi(self._p, self._pt(*gp), self._m, self._v, self._ms, self._rs, self._numel, self._types[1],
+        _check(_lib.pgan_adamw_multi(self._p, self._pt(*map(T.data_ptr, grads)), self._m, self._v, self._ms, self._rs, self._numel, self._types[1],
                                      self._rates[2], self._rates[3], self.n, self.bits, b1, b2, eps, grad_scale,
                                      (seed + (1 << 31)) % (1 << 32) - (1 << 31), sd, int(step), ops._own_stream()),
                "pgan_adamw_multi")

@@ -197,6 +197,13 @@ class _GeneratorBase(_FlatBacked):
     def forward(self, x):
         return _GenFn.apply(self, x, *self._param_list())
 
+    def sampler8(self, batch: int):
+        """A pgan_sampler.Sampler8 of this generator: alignments in evaluation (running BatchNorm statistics), the 2-D
+        tower's products in 8 bits.  Call its refresh() after further training."""
+        from pgan_sampler import Sampler8
+        _require_cuda(self._store.flat, "sampler8")
+        return Sampler8(_ops(self._store.flat.device), self._store.p, self._bstore.p, batch, self._act, self.latent_size)
+
 
 class DC_Generator_Leaky_Sig(_GeneratorBase):
     """layers.py:82-147: z (B, latent, 1, 1) -> sites (B,1,64,64) in (0,1), positions (B,1,64)."""

@@ -910,8 +910,39 @@ class Engine:
         self.D.step_dev = torch.full((1,), self.D.step, dtype=torch.int32, device=self.dev)
         self.G.step_dev = torch.full((1,), self.G.step, dtype=torch.int32, device=self.dev)
 
+    def use_adamw(self, weight_decay: float = 0.01, state_bits: int = 32, seed: int = 0) -> None:
+        """Step both networks with AdamW instead of Adam: decoupled weight decay on the weights of convolutions and the
+        linear head (norm parameters and biases decay not), states in 32 or in 8 bits (the 32-bit ones are then given
+        back).  seed: of the rounding of 8-bit states."""
+        if not hasattr(self.ops, "adamw_plan"):
+            raise RuntimeError("use_adamw needs the GPU op backend")
+        if state_bits not in (32, 8):
+            raise ValueError(f"states are held in 32 or in 8 bits, got {state_bits}")
+        for k, st in enumerate((self.D, self.G)):
+            names = list(st.p)
+            scales = None
+            if state_bits == 8:
+                st.mflat = st.vflat = None
+                code = lambda n: torch.zeros(n, dtype=torch.uint8, device=self.dev).view(torch.float8_e4m3fn)
+                scale = lambda n: torch.zeros(-(-n // 256), dtype=torch.float32, device=self.dev)
+                st.m = {n: code(st.p[n].numel()) for n in names}
+                st.v = {n: code(st.p[n].numel()) for n in names}
+                scales = [[scale(st.p[n].numel()) for n in names] for _ in range(2)]
+            plan = self.ops.adamw_plan([st.p[n] for n in names], [st.m[n] for n in names], [st.v[n] for n in names], scales)
+            decay = [float(weight_decay) if st.p[n].dim() > 1 else 0.0 for n in names]
+            st.adamw = (plan, [st.g[n] for n in names], decay, int(seed) + k,
+                        torch.tensor([st.step, 0, 0, 0], dtype=torch.int32, device=self.dev))
+
     def _adam(self, st: FlatStore, lr: float) -> None:
         st.step += 1
+        if getattr(st, "adamw", None) is not None:
+            plan, grads, decay, seed, counter = st.adamw
+            plan.step(grads, 0, lr, self.betas[0], self.betas[1], self.eps, decay, seed=seed, step_dev=counter,
+                      grad_scale=self.grad_scale)
+            stale = getattr(self.ops, "invalidate_weight_planes", None)
+            if stale is not None:
+                stale(st.flat)
+            return
         scale = {} if self.grad_scale == 1.0 else {"grad_scale": self.grad_scale}
         if getattr(st, "step_dev", None) is not None:
             self.ops.adam(st.flat, st.gflat, st.mflat, st.vflat, 0, lr, self.betas[0], self.betas[1], self.eps,

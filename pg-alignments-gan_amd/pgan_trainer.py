@@ -32,14 +32,20 @@ class FusedTrainer:
     def __init__(self, ops, batch: int, device, loss: str = "gp", act: str = "sigmoid", lam: float = 10.0,
                  critic_iter: int = 5, seed: int = 1234, lr_d: float = 5e-5, lr_g: float = 5e-5,
                  latent: int = 128, process_group=None, rank: int = 0, world: int = 1, sync_bn: Optional[bool] = None,
-                 batched_generator: bool = True, data: int = 64, global_stream: Optional[bool] = None):
-        """data: side of the square alignments, 64 (the reference's networks) or 128 (the scaled networks).
+                 batched_generator: bool = True, data: int = 64, global_stream: Optional[bool] = None,
+                 optimizer: str = "adam", weight_decay: float = 0.01, state_bits: int = 32):
+        """optimizer: "adam" (the reference's) or "adamw" with weight_decay and states in 32 or 8 bits (Engine.use_adamw).
+        data: side of the square alignments, 64 (the reference's networks) or 128 (the scaled networks).
         global_stream: the ranks take their rows of one global batch / draw (default on several ranks; see above)."""
         self.ops, self.dev, self.critic_iter = ops, torch.device(device), int(critic_iter)
         self.global_stream = (world > 1) if global_stream is None else bool(global_stream)
         self.eng = Engine(ops, batch, device, loss=loss, act=act, lam=lam, latent=latent, lr_d=lr_d, lr_g=lr_g,
                           data=data)
         self.eng.use_device_step_counters()
+        if optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer must be 'adam' or 'adamw', got {optimizer!r}")
+        if optimizer == "adamw":
+            self.eng.use_adamw(weight_decay, state_bits, seed)      # one seed on all ranks: the replicas stay identical
         # the generator forwards of an iteration after the first (critic steps 2.., the generator step's own) share
         # their weights and run as ONE pass over (critic_iter) x batch samples beside the first critic step
         self.batched_generator = bool(batched_generator)
@@ -194,6 +200,12 @@ class FusedTrainer:
             idx = order.view(n, 1, S, 1).expand(n, 1, S, S)
             self.pool_s.copy_(torch.gather(self.pool_s, 2, idx))
         self.cursor.zero_()
+
+    def sampler8(self, batch: int):
+        """A pgan_sampler.Sampler8 of the generator as it stands: alignments in evaluation, products in 8 bits."""
+        from pgan_sampler import Sampler8
+        e = self.eng
+        return Sampler8(self.ops, e.G.p, e.Gbuf.p, batch, e.act, e.latent, e.data)
 
     def enable_fake_buffer(self, size: int) -> None:
         """Replay buffer of generated alignments (FakeBuffer, src/train_wgan_v2.py:98-117): every critic step adds its

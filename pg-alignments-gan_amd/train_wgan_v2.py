@@ -308,6 +308,12 @@ def parse_args(argv=None):
     p.add_argument("--data_size", default="64",
                    help="individuals = sites per alignment: 64 (the reference's networks) or 128 (scaled networks with one "
                         "more stride-2 stage; no counterpart in the reference)")
+    p.add_argument("--optimizer", default="adam", help="adam (the reference's) or adamw")
+    p.add_argument("--weight_decay", default="0.01", help="adamw: decay of convolution and head weights")
+    p.add_argument("--state_bits", default="32", help="adamw: bits of each optimizer state, 32 or 8")
+    p.add_argument("--draw_n", default="0",
+                   help="alignments to draw from the trained generator at the end (evaluation, products in 8 bits)")
+    p.add_argument("--draw_slab", default="None", help="packed file (see --slab) that --draw_n alignments are written to")
     p.add_argument("--local_bn", action="store_true",
                    help="several GPUs: BatchNorm statistics of each GPU's own samples instead of the global batch")
     args = p.parse_args(argv)
@@ -386,6 +392,22 @@ def plotting_forward(trainer, normalize, n=1000):
     return sample_genotypes_bernoulli(fs.clamp(0, 1))
 
 
+def draw_alignments(trainer, n, normalize, batch=250):
+    """n genotyped alignments of the generator as it stands, in evaluation and with 8-bit products (pgan_sampler), as
+    packed bits [n, 512] and positions [n, 64] (alignment_slab's format)."""
+    import alignment_slab
+    sampler = trainer.sampler8(min(n, batch))
+    bits, pos = [], []
+    for lo in range(0, n, batch):
+        s, p = sampler.draw(torch.randn(min(batch, n - lo), trainer.eng.latent, device=trainer.dev))
+        if normalize:
+            s, p = s / 2 + 0.5, p / 2 + 0.5
+        g = sample_genotypes_bernoulli(s.clamp(0, 1))
+        bits.append(alignment_slab.pack_numpy(g[:, 0].cpu().numpy()))
+        pos.append(p[:, 0].cpu().numpy())
+    return np.concatenate(bits), np.concatenate(pos).astype(np.float32)
+
+
 def evaluate_2dswd(trainer, real_sites, normalize, n=500, seed=None, generated=None):
     """2DSWD of n generated against n input alignments (src/train_wgan_v2.py:723): SFS -> PCA(2) -> sliced
     Wasserstein of the first n genotyped alignments of the plotting forward (`generated`; made here when not given).
@@ -414,6 +436,11 @@ def main(argv=None):
     data_size = int(args.data_size)
     if data_size not in (64, 128):
         raise SystemExit("--data_size must be 64 or 128")
+    draw_n = int(args.draw_n)
+    if args.optimizer not in ("adam", "adamw") or int(args.state_bits) not in (8, 32):
+        raise SystemExit("--optimizer must be adam or adamw, --state_bits 8 or 32")
+    if draw_n < 0 or (draw_n > 0) != (args.draw_slab != "None") or (draw_n and data_size != 64):
+        raise SystemExit("--draw_n and --draw_slab go together, and need --data_size 64")
     act = "sigmoid" if args.gen == "sigGen" else "tanh"
     normalize = args.normalize or args.gen == "tanNorm"
     if args.plot:
@@ -457,7 +484,8 @@ def main(argv=None):
     trainer = FusedTrainer(HipOps(dev), batch, dev, loss=args.loss, act=act, lam=lam, critic_iter=critic_iter,
                            seed=seed, lr_d=float(args.disc_lr), lr_g=float(args.gen_lr),
                            latent=latent, rank=rank, world=world, sync_bn=(not args.local_bn) if world > 1 else None,
-                           data=data_size)
+                           data=data_size, optimizer=args.optimizer, weight_decay=float(args.weight_decay),
+                           state_bits=int(args.state_bits))
     # --label_smooth / --mono_switch: drawn afresh for every critic batch, on the device, inside the recorded step
     if args.label_smooth or args.mono_switch:
         trainer.enable_augment(label_noise=float(args.label_noise) if args.label_smooth else None,
@@ -512,6 +540,8 @@ def main(argv=None):
                 logging.info("Epoch:\t%d 2DSWD: %6.8f" % (epoch, w))
                 with open(os.path.join(args.odir, "w_dist_pca.txt"), "a") as f:   # src/train_wgan_v2.py:724-726
                     f.write(str(epoch) + "\t" + str(w) + "\n")
+    if draw_n and rank == 0:
+        alignment_slab.write_slab(args.draw_slab, *draw_alignments(trainer, draw_n, normalize))
     if world > 1:
         import torch.distributed as dist
         dump = os.environ.get("PGAN_DUMP_WEIGHT_SUMS")      # test aid: the replicas must stay identical

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
-// A block of WT x WN waves makes a tile of tokens x channels, a wave FT x FN tiles of 32 x 32 (i32 <- i8, 32 deep; channels
+// A block of WT x WN waves (MW of all blocks' on a SIMD at once) makes a tile of tokens x channels, a wave FT x FN tiles of 32 x 32 (i32 <- i8, 32 deep; channels
 // are the matrix instruction's rows, so that a lane holds four neighbouring channels of one token).  Stages of 128 bytes
 // along K go through registers into LDS, where chunk c (16 bytes) of row r lies at slot r ^ 2c of its 32 rows: a stage's
 // global reads are whole 128-byte lines and neither side of LDS has bank conflicts.  The next stage's reads are under way
@@ -272,8 +272,8 @@ __device__ __forceinline__ void tile_of(const GemmArgs& a, unsigned& tt, unsigne
     tn = band * a.band + in - tt * wide;
 }
 
-template <int FT, int FN, int WT, int WN, int TYPE>
-__global__ __launch_bounds__(64 * WT * WN, FT * FN > 4 ? 2 : 3) void gemm_q8_kernel(const GemmArgs a) {
+template <int FT, int FN, int WT, int WN, int MW, int TYPE>
+__global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArgs a) {
     using Y = typename Elem<TYPE>::type;
     constexpr int NT = 64 * WT * WN, BT = 32 * FT * WT, BN = 32 * FN * WN;
     constexpr int RP = NT / 8;                           // rows that the block's threads read at a time
@@ -281,7 +281,8 @@ __global__ __launch_bounds__(64 * WT * WN, FT * FN > 4 ? 2 : 3) void gemm_q8_ker
     constexpr int STAGE = (BT + BN) * GK / 16;           // 16-byte chunks
     constexpr int FO = FN < 2 ? FN : 2;                  // channel tiles whose results leave together
     constexpr int YROW = 32 * FO * (int)sizeof(Y) + 16;  // a wave's row of results in LDS, 16 bytes apart
-    constexpr int OUT = 32 * YROW * WT * WN;
+    constexpr int JO = TYPE == 0 || FT < 2 ? 1 : 2;      // token tiles
+    constexpr int OUT = 32 * JO * YROW * WT * WN;
     constexpr int BYTES = STAGE * 16 > OUT ? STAGE * 16 : OUT;
     __shared__ __attribute__((aligned(16))) char mem[BYTES];
     __shared__ __attribute__((aligned(16))) float sws[BN], sbias[BN], sqs[BT];
@@ -361,49 +362,52 @@ __global__ __launch_bounds__(64 * WT * WN, FT * FN > 4 ? 2 : 3) void gemm_q8_ker
             __syncthreads();
         }
     }
+    // (In 16 bits, tokens 16 to 31 keep the two eights of every 16 bytes the other way round: a store's 32 lanes then touch
+    // all 64 banks once.)
     // The results of 32 tokens at a time pass through the wave's part of LDS, to leave as whole lines of y's rows.
     // channel (within 32): e % 4 + 8 (e / 4) + 4 (lane / 32); token: lane % 32
-    char* own = mem + wave * 32 * YROW;
+    char* own = mem + wave * 32 * JO * YROW;
     constexpr int PER = 16 / (int)sizeof(Y), LANES = 32 * FO / PER;      // channels and lanes of a 16-byte row stretch
     const bool whole = trows == BT && nrows == BN && a.align == 16;
 #pragma unroll
     for (int io = 0; io < FN; io += FO) {
         const int wc0 = (wn * FN + io) * 32;
-        f32x4 ws[FO][4], bs[FO][4];
 #pragma unroll
-        for (int i = 0; i < FO; ++i)
+        for (int jo = 0; jo < FT; jo += JO) {
+            const int tr = (wt * FT + jo) * 32;
+            float st[JO];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int ch = wc0 + 32 * i + 8 * g + 4 * (lane >> 5);
-                ws[i][g] = *reinterpret_cast<const f32x4*>(sws + ch);
-                bs[i][g] = *reinterpret_cast<const f32x4*>(sbias + ch);
-            }
-#pragma unroll
-        for (int j = 0; j < FT; ++j) {
-            const int tr = (wt * FT + j) * 32;
-            const float st = sqs[tr + (lane & 31)];
+            for (int j = 0; j < JO; ++j) st[j] = sqs[tr + 32 * j + (lane & 31)];
 #pragma unroll
             for (int i = 0; i < FO; ++i)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    float v[4];
+                    const int ch = 32 * i + 8 * g + 4 * (lane >> 5);
+                    const f32x4 ws = *reinterpret_cast<const f32x4*>(sws + wc0 + ch), bs = *reinterpret_cast<const f32x4*>(sbias + wc0 + ch);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)acc[io + i][j][4 * g + e] * st, ws[i][g][e], bs[i][g][e]);
-                    char* to = own + (lane & 31) * YROW + (32 * i + 8 * g + 4 * (lane >> 5)) * (int)sizeof(Y);
-                    if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-                    else *reinterpret_cast<uint2*>(to) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
+                    for (int j = 0; j < JO; ++j) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)acc[io + i][jo + j][4 * g + e] * st[j], ws[e], bs[e]);
+                        char* to = own + (32 * j + (lane & 31)) * YROW;
+                        if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to + ch * 4) = f32x4{v[0], v[1], v[2], v[3]};
+                        else *reinterpret_cast<uint2*>(to + (ch * 2 ^ (lane & 16) / 2)) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
+                    }
                 }
             wave_sync();
             Y* to = static_cast<Y*>(a.y) + (t0 + tr + lane / LANES) * a.ldy + n0 + wc0 + lane % LANES * PER;
             const char* from = own + lane / LANES * YROW + lane % LANES * 16;
+            // 16 bytes of row r + lane / LANES; rows 16 to 31 of 32 hold their eights the other way round
+            const auto piece = [&](int r) {
+                const i32x4 v = *reinterpret_cast<const i32x4*>(from + r * YROW);
+                return TYPE != 0 && (r & 16) ? i32x4{v[2], v[3], v[0], v[1]} : v;
+            };
             if (whole) {
 #pragma unroll
-                for (int r = 0; r < 32; r += 64 / LANES)
-                    *reinterpret_cast<i32x4*>(to + r * a.ldy) = *reinterpret_cast<const i32x4*>(from + r * YROW);
+                for (int r = 0; r < 32 * JO; r += 64 / LANES) *reinterpret_cast<i32x4*>(to + r * a.ldy) = piece(r);
             } else {
-                for (int r = 0; r < 32; r += 64 / LANES)
-                    if (tr + r + lane / LANES < trows)
-                        put16(to + r * a.ldy, *reinterpret_cast<const i32x4*>(from + r * YROW), nrows - wc0 - lane % LANES * PER, a.align);
+                for (int r = 0; r < 32 * JO; r += 64 / LANES)
+                    if (tr + r + lane / LANES < trows) put16(to + r * a.ldy, piece(r), nrows - wc0 - lane % LANES * PER, a.align);
             }
             wave_sync();
         }
@@ -761,12 +765,12 @@ inline int row_align(const void* p, long long stride) {
 
 constexpr int FEW = 32, FEW_ELEMENTS = 32768;
 
-template <int FT, int FN, int WT, int WN, int TYPE>
+template <int FT, int FN, int WT, int WN, int MW, int TYPE>
 void launch_gemm(GemmArgs a, hipStream_t st) {
     a.tn = (a.N + 32 * FN * WN - 1) / (32 * FN * WN);
     a.band = a.tn < 8 ? a.tn : 8;
     a.tt = (unsigned)((a.T + 32 * FT * WT - 1) / (32 * FT * WT));
-    gemm_q8_kernel<FT, FN, WT, WN, TYPE><<<a.tt * a.tn, 64 * WT * WN, 0, st>>>(a);
+    gemm_q8_kernel<FT, FN, WT, WN, MW, TYPE><<<a.tt * a.tn, 64 * WT * WN, 0, st>>>(a);
 }
 
 template <class F>
@@ -884,16 +888,19 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0,
                    row_align(y, ldy * type_bytes(y_type))};
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
-        // The larger the tile the fewer LDS reads a product takes, as long as there is a tile for each of the 256 CUs:
-        // 4096 x 4096 x 4096 in 256 x 256: 70 us (1960 Tera operations/s), 128 x 128: 84, 128 x 64: 97, 64 x 64: 115;
-        // 64 x 4096 x 1024 (1 .. 16 tiles): 62, 32, 23, 16 us.  (One with two LDS buffers and one barrier a stage instead of
-        // one and two was not faster: 70 us.)
+        // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's loads
+        // and results behind the other's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight
+        // waves, one block a CU), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
+        //   4096 x 4096 x 4096       71   82   97  116        16000 x 512 x 4096       58   53   64   73
+        //   4096 x 2048 x 4096       40   45   52   61        64000 x 256 x 2048       86   67   75   86
+        //   4096 x 1024 x 4096       26   27   30   34       256000 x 128 x 1024      147  130  152  165
+        // and 777 x 1001 x 1234 (20 .. 260 tiles) 21, 12, 9, 9.
         if (T <= FEW) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
-        else if (N <= 32) launch_gemm<2, 1, 4, 1, Y>(a, st);
-        else if (tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, Y>(a, st);
-        else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, Y>(a, st);
-        else if (tiles(128, 64) >= 256) launch_gemm<2, 1, 2, 2, Y>(a, st);
-        else launch_gemm<1, 1, 2, 2, Y>(a, st);
+        else if (N <= 32) launch_gemm<2, 1, 4, 1, 4, Y>(a, st);
+        else if (K >= 1024 && tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, 2, Y>(a, st);
+        else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, 4, Y>(a, st);
+        else if (tiles(128, 64) >= 256) launch_gemm<2, 1, 2, 2, 4, Y>(a, st);
+        else launch_gemm<1, 1, 2, 2, 4, Y>(a, st);
     });
 }
 

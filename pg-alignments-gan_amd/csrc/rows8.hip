@@ -414,8 +414,8 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
     }
 }
 
-// ---- the product for few tokens ------------------------------------------------------------------------------------
-// Up to 32 tokens: a block makes 32 channels, its WV waves share K and add up their sums (whole numbers: any order) in LDS.
+// ---- the product for few tiles ------------------------------------------------------------------------------------
+// A block makes 32 tokens x 32 channels, its WV waves share K and add up their sums (whole numbers: any order) in LDS.
 // Channels come straight from memory into the matrix instruction's registers, every line of them by one wave.  X >= 0: the
 // block makes the tokens' codes itself, a wave RW rows -- every block all of them, which for up to 32768 elements takes less time than a
 // launch of its own -- while its first channels are on their way; X < 0: it reads codes.  Bound by the launch, then by the
@@ -433,17 +433,29 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
     extern __shared__ __attribute__((aligned(16))) char few[];
     const GemmArgs& a = f.g;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int K = a.K, T = (int)a.T, N = a.N, end = (K + 15) / 16 * 16 - 16;      // a row's last 16 bytes
+    const int K = a.K, T = (int)min(a.T - blockIdx.y * 32LL, 32LL), N = a.N, end = (K + 15) / 16 * 16 - 16;    // a row's last 16 bytes
+    const long long t0 = blockIdx.y * 32LL;
     const int n0 = blockIdx.x * 32, half = lane >> 5, stride = (K + 31) / 32 * 32 + 16;
     const int steps = (K + 31) / 32, s0 = wave * steps / WV, s1 = (wave + 1) * steps / WV;
     const int8_t* wr = a.w + (long long)min(n0 + (lane & 31), N - 1) * a.ldw;
-    const auto channels = [&](int s, i32x4 (&v)[4]) {
+    // Four steps (a line of each row) at a time.  A load of all lanes takes another step of every fourth row: were it the same
+    // one, all 32 rows' lines would be asked for the same 32 bytes, which the L1 serves one after the other.  in_order()
+    // turns a lane's four back.
+    const auto four = [&](const int8_t* from, int s, i32x4 (&v)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (s + i < s1) v[i] = *reinterpret_cast<const i32x4*>(wr + min((s + i) * 32 + 16 * half, end));
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const i32x4*>(from + min((s + ((i + lane) & 3)) * 32 + 16 * half, end));
+    };
+    const auto in_order = [&](i32x4 (&v)[4]) {
+        const i32x4 a = v[0], b = v[1], c = v[2], d = v[3];
+        const bool one = lane & 1, two = lane & 2;
+        const i32x4 e = one ? d : a, f = one ? a : b, g = one ? b : c, h = one ? c : d;
+        v[0] = two ? g : e;
+        v[1] = two ? h : f;
+        v[2] = two ? e : g;
+        v[3] = two ? f : h;
     };
     i32x4 cur[4], nxt[4];
-    channels(s0, cur);
+    four(wr, s0, cur);
     float ws[4], bs[4];         // of the four channels whose sums this lane ends
     const int ch = n0 + 8 * wave + 4 * half;
     if (wave < 4) {
@@ -507,23 +519,28 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
                         uint2{four_codes(v[r][0], v[r][1], v[r][2], v[r][3], inv[r]), four_codes(v[r][4], v[r][5], v[r][6], v[r][7], inv[r])};
         }
     } else {
-        if (tid < 32) scales[tid] = a.qs[min(tid, T - 1)];
+        if (tid < 32) scales[tid] = a.qs[t0 + min(tid, T - 1)];
     }
     __syncthreads();
     const int t = lane & 31, row = min(t, T - 1);      // rows past the end repeat the last one; what they give is not stored
     i32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0;
+    const int8_t* xr = X < 0 ? a.q + (t0 + row) * a.ldq : nullptr;
+    i32x4 tok[4], more[4];
+    if constexpr (X < 0) four(xr, s0, tok);
     for (int s = s0; s < s1; s += 4) {
-        if (s + 4 < s1) channels(s + 4, nxt);
-        i32x4 tok[4];
+        if (s + 4 < s1) {
+            four(wr, s + 4, nxt);
+            if constexpr (X < 0) four(xr, s + 4, more);
+        }
+        in_order(cur);
+        if constexpr (X < 0) {
+            in_order(tok);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (s + i < s1) {
-                const int k = min((s + i) * 32 + 16 * half, end);
-                if constexpr (X >= 0) tok[i] = *reinterpret_cast<const i32x4*>(few + row * stride + k);
-                else tok[i] = *reinterpret_cast<const i32x4*>(a.q + row * a.ldq + k);
-            }
+            for (int i = 0; i < 4; ++i) tok[i] = *reinterpret_cast<const i32x4*>(few + row * stride + min((s + i) * 32 + 16 * half, end));
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (s + i < s1) {
@@ -531,7 +548,10 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
                 acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(cur[i], tok[i], acc, 0, 0, 0);
             }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
+        for (int i = 0; i < 4; ++i) {
+            cur[i] = nxt[i];
+            if constexpr (X < 0) tok[i] = more[i];
+        }
     }
     __syncthreads();
     i32x4* sums = reinterpret_cast<i32x4*>(few);       // [wave][four channels][lane]
@@ -546,7 +566,7 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)sum[e] * st, ws[e], bs[e]);
-    Y* to = static_cast<Y*>(a.y) + t * a.ldy + ch;
+    Y* to = static_cast<Y*>(a.y) + (t0 + t) * a.ldy + ch;
     if (a.align >= 4 * (int)sizeof(Y) && ch + 4 <= N) {
         if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
         else *reinterpret_cast<uint2*>(to) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
@@ -825,16 +845,29 @@ int launch_fold(const void* y, int type, FoldArgs a, bool vec, hipStream_t st) {
     });
 }
 
-// up to 32 tokens, x (of type X) or their codes (X < 0)
+// up to 32 tokens x (of type X), or codes of any number (X < 0)
 template <int X, int Y>
 void launch_few(const FewArgs& f, hipStream_t st) {
     const int K = f.g.K, codes = X < 0 ? 0 : (int)f.g.T * ((K + 31) / 32 * 32 + 16);
-    const unsigned blocks = (unsigned)((f.g.N + 31) / 32);
-    // 16 waves where a wave of 4 would have 16 steps of 32 bytes or more to go through
-    if (K >= 2048) gemm_few_kernel<X, 16, 2, Y><<<blocks, 1024, std::max(codes, 16 * 4096), st>>>(f);
-    else if (X < 0 || f.g.T <= 4) gemm_few_kernel<X, 4, 1, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
-    else if (f.g.T <= 16) gemm_few_kernel<X, 4, X < 0 ? 1 : 4, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
-    else gemm_few_kernel<X, 4, X < 0 ? 1 : 8, Y><<<blocks, 256, std::max(codes, 4 * 4096), st>>>(f);
+    const dim3 blocks((unsigned)((f.g.N + 31) / 32), X < 0 ? (unsigned)((f.g.T + 31) / 32) : 1u);
+    // eight waves from K = 1024 on (us with 4, 8, 16: 1 x 8192 x 8192 16, 15, 15; 96 x 2048 x 2048 5.4, 4.8, 4.8; 64 x 4096 x
+    // 8192 12.5, 13.3, 15.2; 1 x 512 x 4096 3.7, 3.9, -)
+    const auto go = [&](auto waves, auto rows) {
+        constexpr int WV = waves.value;
+        gemm_few_kernel<X, WV, rows.value, Y><<<blocks, 64 * WV, std::max(codes, WV * 4096), st>>>(f);
+    };
+    using std::integral_constant;
+    if constexpr (X < 0) {
+        if (K >= 1024) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        else go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    } else if (K >= 1024) {
+        if (f.g.T <= 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        else go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    } else {
+        if (f.g.T <= 4) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        else if (f.g.T <= 16) go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+        else go(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    }
 }
 
 inline int gemm_args(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
@@ -894,8 +927,10 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         //   4096 x 4096 x 4096       71   82   97  116        16000 x 512 x 4096       58   53   64   73
         //   4096 x 2048 x 4096       40   45   52   61        64000 x 256 x 2048       86   67   75   86
         //   4096 x 1024 x 4096       26   27   30   34       256000 x 128 x 1024      147  130  152  165
-        // and 777 x 1001 x 1234 (20 .. 260 tiles) 21, 12, 9, 9.
-        if (T <= FEW) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
+        // and 777 x 1001 x 1234 (20 .. 260 tiles) 21, 12, 9, 8.  A product of few tiles shares K among the waves of a block of
+        // 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0, 64 x 4096 x 1024 7.6 against 14.9, but
+        // 777 x 1001 x 1234 10.
+        if (T <= FEW || tiles(64, 64) <= 128) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
         else if (N <= 32) launch_gemm<2, 1, 4, 1, 4, Y>(a, st);
         else if (K >= 1024 && tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, 2, Y>(a, st);
         else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, 4, Y>(a, st);

@@ -72,22 +72,36 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
     const float amax = __builtin_fmaxf(__builtin_bit_cast(float, amax_bits), 0x1p-100f);
     return RowScale{127.f / amax, amax * (float)(1.0 / 127)};
 }
-// the code of x; a row without a finite maximum (inv = 0) has none but 0
-__device__ __forceinline__ int code_of(float x, float inv) { return inv == 0.f ? 0 : (int)rintf(x * inv); }
-__device__ __forceinline__ float slope(float x, bool lrelu) { return lrelu && !(x > 0.f) ? x * PGAN_SLOPE : x; }
+// The code of x is the low byte of x inv + 1.5 2^23: that sum's last place is 1, so it is rounded to a whole number (ties to
+// the even one).  A row without a finite maximum has inv = 0: its elements have to be made 0 first (no_row).
+__device__ __forceinline__ uint32_t code_of(float x, float inv) { return __builtin_bit_cast(uint32_t, x * inv + 12582912.f); }
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float inv) {
+    return __builtin_amdgcn_perm(code_of(b, inv), code_of(a, inv), 0x0c0c0400) | __builtin_amdgcn_perm(code_of(d, inv), code_of(c, inv), 0x04000c0c);
+}
+template <int N>
+__device__ __forceinline__ void no_row(float (&v)[N], float inv) {
+    if (inv == 0.f) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = 0.f;
+    }
+}
+// LeakyReLU: of x and its tenth the larger
+__device__ __forceinline__ float slope(float x, bool lrelu) { return lrelu ? __builtin_fmaxf(x, x * PGAN_SLOPE) : x; }
 
-// eight elements from p on; `aligned` to 16 bytes
+// eight elements from p on, which lies on a multiple of 4 bytes
 template <int TYPE>
 __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float (&v)[8]) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
     if constexpr (TYPE == 0) {
-        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+        const f32x4 a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v[e] = a[e];
             v[4 + e] = b[e];
         }
     } else {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(p);
+        const i32x4 a = *reinterpret_cast<const i32x4u*>(p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (TYPE == 1) {
@@ -100,95 +114,115 @@ __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float 
         }
     }
 }
-__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float inv) {
-    return (uint32_t)(code_of(a, inv) & 255) | (uint32_t)(code_of(b, inv) & 255) << 8 | (uint32_t)(code_of(c, inv) & 255) << 16
-           | (uint32_t)code_of(d, inv) << 24;
-}
-
 // ---- rows to codes ------------------------------------------------------------------------------------------------
-// 2^log lanes a row, whose values stay in their registers between the maximum and the codes: 8 NIT each, K <= 8 NIT 2^log.
-// VEC: eight neighbouring ones at a time, in rows that start on 16-byte borders (codes on 8); else every 2^log-th.
-// Bound by HBM (2 + 1 bytes an element of 16 bits).
-template <int TYPE, bool VEC, int NIT>
+// 2^log lanes a row, whose values stay in their registers between the maximum and the codes: 8 NIT each, K <= 8 NIT 2^log; a
+// lane has R rows, to have more bytes on their way.  VEC: eight neighbouring elements at a time, in rows that start on
+// 4-byte borders (codes on 8); else every 2^log-th.  Bound by HBM (2 + 1 bytes an element of 16 bits).
+template <int TYPE, bool VEC, int NIT, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                          int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                                                          long long rows, int K, int lrelu, int log) {
-    const long long row = (long long)blockIdx.x * (256 >> log) + (threadIdx.x >> log);
+    const long long row0 = ((long long)blockIdx.x * (256 >> log) + (threadIdx.x >> log)) * R;
     const int l = threadIdx.x & ((1 << log) - 1);
-    if (row >= rows) return;        // whole groups of 2^log lanes
-    const typename Elem<TYPE>::type* xr = x + row * ldx;
-    int8_t* qr = q + row * ldq;
-    float v[NIT][8];
-    uint32_t mx = 0;
+    if (row0 >= rows) return;        // whole groups of 2^log lanes
+    float v[R][NIT][8];
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-        if constexpr (VEC) {
-            const int k = ((it << log) + l) * 8;
+    for (int r = 0; r < R; ++r) {
+        const typename Elem<TYPE>::type* xr = x + (row0 + r < rows ? row0 + r : row0) * ldx;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[it][e] = 0.f;
-            if (k + 8 <= K) {
-                load8<TYPE>(xr + k, v[it]);
+        for (int it = 0; it < NIT; ++it) {
+            if constexpr (VEC) {
+                const int k = ((it << log) + l) * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[r][it][e] = 0.f;
+                if (k + 8 <= K) {
+                    load8<TYPE>(xr + k, v[r][it]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k + e < K) v[r][it][e] = to_f32<TYPE>(xr[k + e]);
+                }
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < K) v[it][e] = to_f32<TYPE>(xr[k + e]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int k = ((it * 8 + e) << log) + l;
-                v[it][e] = k < K ? to_f32<TYPE>(xr[k]) : 0.f;
+                for (int e = 0; e < 8; ++e) {
+                    const int k = ((it * 8 + e) << log) + l;
+                    v[r][it][e] = k < K ? to_f32<TYPE>(xr[k]) : 0.f;
+                }
             }
         }
     }
 #pragma unroll
-    for (int it = 0; it < NIT; ++it)
+    for (int r = 0; r < R; ++r) {
+        uint32_t mx = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[it][e] = slope(v[it][e], lrelu);
-            mx = max(mx, magnitude(v[it][e]));
-        }
-    const RowScale rs = row_scale(group_max(mx, log));
-    if (l == 0) scale[row] = rs.scale;
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-        if constexpr (VEC) {
-            const int k = ((it << log) + l) * 8;
-            uint2 u;
-            u.x = four_codes(v[it][0], v[it][1], v[it][2], v[it][3], rs.inv);
-            u.y = four_codes(v[it][4], v[it][5], v[it][6], v[it][7], rs.inv);
-            if (k + 8 <= K) {
-                *reinterpret_cast<uint2*>(qr + k) = u;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < K) qr[k + e] = (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3)));
-            }
-        } else {
+        for (int it = 0; it < NIT; ++it)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int k = ((it * 8 + e) << log) + l;
-                if (k < K) qr[k] = (int8_t)code_of(v[it][e], rs.inv);
+                v[r][it][e] = slope(v[r][it][e], lrelu);
+                mx = max(mx, magnitude(v[r][it][e]));
+            }
+        const RowScale rs = row_scale(group_max(mx, log));
+        if (row0 + r >= rows) break;
+        if (l == 0) scale[row0 + r] = rs.scale;
+        int8_t* qr = q + (row0 + r) * ldq;
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+            no_row(v[r][it], rs.inv);
+            if constexpr (VEC) {
+                const int k = ((it << log) + l) * 8;
+                uint2 u;
+                u.x = four_codes(v[r][it][0], v[r][it][1], v[r][it][2], v[r][it][3], rs.inv);
+                u.y = four_codes(v[r][it][4], v[r][it][5], v[r][it][6], v[r][it][7], rs.inv);
+                if (k + 8 <= K) {
+                    *reinterpret_cast<uint2*>(qr + k) = u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k + e < K) qr[k + e] = (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3)));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = ((it * 8 + e) << log) + l;
+                    if (k < K) qr[k] = (int8_t)code_of(v[r][it][e], rs.inv);
+                }
             }
         }
     }
 }
 
-// longer rows: one a wave, read twice
-template <int TYPE>
+// longer rows: one a block, read twice (the second time from the L1 or L2)
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                               int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                                                               long long rows, int K, int lrelu) {
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
+    __shared__ uint32_t tops[4];
+    const long long row = blockIdx.x;
     const typename Elem<TYPE>::type* xr = x + row * ldx;
-    uint32_t mx = 0;
-    for (int k = lane; k < K; k += 64) mx = max(mx, magnitude(slope(to_f32<TYPE>(xr[k]), lrelu)));
-    const RowScale rs = row_scale(group_max(mx, 6));
     int8_t* qr = q + row * ldq;
-    for (int k = lane; k < K; k += 64) qr[k] = (int8_t)code_of(slope(to_f32<TYPE>(xr[k]), lrelu), rs.inv);
-    if (lane == 0) scale[row] = rs.scale;
+    const int whole = VEC ? K / 8 * 8 : 0;          // elements that are read eight at a time
+    uint32_t mx = 0;
+    for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+        float v[8];
+        load8<TYPE>(xr + k, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = max(mx, magnitude(slope(v[e], lrelu)));
+    }
+    for (int k = whole + threadIdx.x; k < K; k += 256) mx = max(mx, magnitude(slope(to_f32<TYPE>(xr[k]), lrelu)));
+    mx = group_max(mx, 6);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    const RowScale rs = row_scale(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+    if (threadIdx.x == 0) scale[row] = rs.scale;
+    for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+        float v[8];
+        load8<TYPE>(xr + k, v);
+        no_row(v, rs.inv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = slope(v[e], lrelu);
+        *reinterpret_cast<uint2*>(qr + k) = uint2{four_codes(v[0], v[1], v[2], v[3], rs.inv), four_codes(v[4], v[5], v[6], v[7], rs.inv)};
+    }
+    for (int k = whole + threadIdx.x; k < K; k += 256) qr[k] = rs.inv == 0.f ? 0 : (int8_t)code_of(slope(to_f32<TYPE>(xr[k]), lrelu), rs.inv);
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
@@ -424,7 +458,7 @@ struct FewArgs {
     GemmArgs g;
     const void* x;
     long long ldx;
-    int lrelu, vec;         // vec: rows of x start on 16-byte borders
+    int lrelu, vec;         // vec: rows of x start on 4-byte borders
 };
 template <int X, int WV, int RW, int TYPE>
 __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
@@ -514,9 +548,11 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
             const int k = k0 + lane * 8;
 #pragma unroll
             for (int r = 0; r < RW; ++r)
-                if (wave + WV * r < T && k < K)
+                if (wave + WV * r < T && k < K) {
+                    no_row(v[r], inv[r]);
                     *reinterpret_cast<uint2*>(few + (wave + WV * r) * stride + k) =
                         uint2{four_codes(v[r][0], v[r][1], v[r][2], v[r][3], inv[r]), four_codes(v[r][4], v[r][5], v[r][6], v[r][7], inv[r])};
+                }
         }
     } else {
         if (tid < 32) scales[tid] = a.qs[t0 + min(tid, T - 1)];
@@ -666,6 +702,7 @@ __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>:
         if constexpr (VEC) mx = l * 8 < C ? mx : 0u;
         const RowScale rs = row_scale(group_max(mx, a.log));
         if (l == 0) a.scale[pix] = rs.scale;
+        no_row(v, rs.inv);
         int8_t* qr = a.q + (long long)pix * a.ldq;
         if constexpr (VEC) {
             if (l * 8 < C)
@@ -707,7 +744,7 @@ __global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<T
         for (int c = lane; c < a.C; c += 64) mx = max(mx, magnitude(slope(folded<TYPE>(y, t, c, a.shift), true)));
         const RowScale rs = row_scale(group_max(mx, 6));
         for (int c = lane; c < a.C; c += 64)
-            a.q[(long long)pix * a.ldq + c] = (int8_t)code_of(slope(folded<TYPE>(y, t, c, a.shift), true), rs.inv);
+            a.q[(long long)pix * a.ldq + c] = rs.inv == 0.f ? 0 : (int8_t)code_of(slope(folded<TYPE>(y, t, c, a.shift), true), rs.inv);
         if (lane == 0) a.scale[pix] = rs.scale;
     } else {
         for (int c = lane; c < a.C; c += 64) a.out[(long long)pix * a.C + c] = activate(folded<TYPE>(y, t, c, a.shift), a.act);
@@ -894,9 +931,11 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
     if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4) || ldx < K || ldq < K) return PGAN_EINVAL;
     if (!apart({rows_of(x, rows, K, ldx, type_bytes(x_type)), rows_of(q, rows, K, ldq, 1, true), rows_of(scale, 1, rows, 0, 4, true)}))
         return PGAN_EINVAL;
-    const bool vec = row_align(x, ldx * type_bytes(x_type)) == 16 && row_align(q, ldq) >= 8;
+    const bool vec = row_align(x, ldx * type_bytes(x_type)) >= 4 && row_align(q, ldq) >= 8;
     const int log = lanes_log(K);    // lanes a row
-    const long long blocks = (rows + (256 >> log) - 1) / (256 >> log);
+    // rows a lane: two where there are enough of them (16000 x 512 in bf16: 9.3 us with one, 6.7 with two)
+    const int R = K <= 1024 && rows >= 8192 ? 2 : 1;
+    const long long groups = (rows + R - 1) / R, blocks = K > 4096 ? rows : (groups + (256 >> log) - 1) / (256 >> log);
     if (blocks > MAX_BLOCKS) return PGAN_EINVAL;
     return by_type(x_type, [&](auto t) {
         constexpr int X = t.value;
@@ -904,11 +943,13 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
             kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<X>::type*>(x), ldx, static_cast<int8_t*>(q), ldq,
                                                       scale, rows, K, lrelu, more...);
         };
-        if (K > 4096) go(quant_long_rows_kernel<X>);
-        else if (K > 2048) vec ? go(quant_rows_kernel<X, true, 8>, log) : go(quant_rows_kernel<X, false, 8>, log);
-        else if (K > 1024) vec ? go(quant_rows_kernel<X, true, 4>, log) : go(quant_rows_kernel<X, false, 4>, log);
-        else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2>, log) : go(quant_rows_kernel<X, false, 2>, log);
-        else vec ? go(quant_rows_kernel<X, true, 1>, log) : go(quant_rows_kernel<X, false, 1>, log);
+        if (K > 4096) vec ? go(quant_long_rows_kernel<X, true>) : go(quant_long_rows_kernel<X, false>);
+        else if (K > 2048) vec ? go(quant_rows_kernel<X, true, 8, 1>, log) : go(quant_rows_kernel<X, false, 8, 1>, log);
+        else if (K > 1024) vec ? go(quant_rows_kernel<X, true, 4, 1>, log) : go(quant_rows_kernel<X, false, 4, 1>, log);
+        else if (K > 512 && R == 2) vec ? go(quant_rows_kernel<X, true, 2, 2>, log) : go(quant_rows_kernel<X, false, 2, 2>, log);
+        else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2, 1>, log) : go(quant_rows_kernel<X, false, 2, 1>, log);
+        else if (R == 2) vec ? go(quant_rows_kernel<X, true, 1, 2>, log) : go(quant_rows_kernel<X, false, 1, 2>, log);
+        else vec ? go(quant_rows_kernel<X, true, 1, 1>, log) : go(quant_rows_kernel<X, false, 1, 1>, log);
     });
 }
 
@@ -953,7 +994,7 @@ int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long 
             (void)by_type(y_type, [&](auto t) {
                 const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0,
                                  row_align(y, ldy * type_bytes(y_type))};
-                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, row_align(x, ldx * type_bytes(x_type)) == 16}, st);
+                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, row_align(x, ldx * type_bytes(x_type)) >= 4}, st);
             });
         });
     const int rc = pgan_quant_rows(x, x_type, ldx, q, ldq, q_scale, T, K, lrelu, st);

@@ -226,15 +226,16 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
-// A block of WT x WN waves (MW of all blocks' on a SIMD at once) makes a tile of tokens x channels, a wave FT x FN tiles of 32 x 32 (i32 <- i8, 32 deep; channels
-// are the matrix instruction's rows, so that a lane holds four neighbouring channels of one token).  Stages of 128 bytes
-// along K go through registers into LDS, where chunk c (16 bytes) of row r lies at slot r ^ 2c of its 32 rows: a stage's
-// global reads are whole 128-byte lines and neither side of LDS has bank conflicts.  The next stage's reads are under way
-// while a stage is multiplied.
-constexpr int GK = 128;
-
-__device__ __forceinline__ int lds_slot(int row, int c) { return (row >> 5) * (32 * GK / 16) + c * 32 + ((row & 31) ^ (2 * c)); }
-
+// A block of WT x WN waves (MW waves of all blocks on a SIMD at once) makes a tile of tokens x channels, a wave FT x FN tiles
+// of 32 x 32 (i32 <- i8, 32 deep; channels are the matrix instruction's rows, so that a lane holds four neighbouring channels
+// of one token).  Stages of GK bytes along K go from memory straight into a ring of D in LDS, without a stop in registers: a
+// stage's place is refilled as soon as every wave has read its last step, which leaves the other D - 1 under way meanwhile.
+// A wave waits for its own reads of a stage by their count and meets the others at a barrier, once a stage; the operands of
+// a step of 32 are read from LDS while the step before is multiplied.
+// Bound by the matrix instructions and the power they draw where K is long (8192 x 8192 x 8192: 505 us, 2180 Top/s, 92% of
+// the rate of the library's product; 4096 x 4096 x 4096: 73 us, 64 with zeros for operands), by the results' way out where it
+// is short (256000 x 128 x 1024: 107 us, 5.2 TB/s).  With stages that went through registers into one place of LDS:
+// 4096 x 4096 x 4096 77 us, 16000 x 512 x 4096 53 for 48.5, 256000 x 128 x 1024 134, 2048 x 2048 x 2048 21 for 15.
 __device__ __forceinline__ i32x4 below(i32x4 v, int left) {        // the first `left` of 16 bytes, zero behind them
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -306,54 +307,81 @@ __device__ __forceinline__ void tile_of(const GemmArgs& a, unsigned& tt, unsigne
     tn = band * a.band + in - tt * wide;
 }
 
-template <int FT, int FN, int WT, int WN, int MW, int TYPE>
+// waits until at most VM of the wave's memory operations are under way and all its LDS reads have come back
+template <int VM>
+__device__ __forceinline__ void wait_for() {
+    __builtin_amdgcn_s_waitcnt((VM & 15) | 7 << 4 | (VM >> 4) << 14);
+}
+
+// 16 bytes a lane from `at` bytes into `from` to LDS: `to` + 16 * lane, without a stop in registers
+__device__ __forceinline__ void read_to_lds(__amdgpu_buffer_rsrc_t from, char* to, int at) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((address_space(3))) void lds_void;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)to, 16, at, 0, 0, 0);
+#endif
+}
+
+template <int FT, int FN, int WT, int WN, int GK, int D, int MW, int TYPE>
 __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArgs a) {
     using Y = typename Elem<TYPE>::type;
-    constexpr int NT = 64 * WT * WN, BT = 32 * FT * WT, BN = 32 * FN * WN;
-    constexpr int RP = NT / 8;                           // rows that the block's threads read at a time
-    constexpr int LT = BT / RP, LN = BN / RP;
-    constexpr int STAGE = (BT + BN) * GK / 16;           // 16-byte chunks
+    constexpr int NW = WT * WN, NT = 64 * NW, BT = 32 * FT * WT, BN = 32 * FN * WN;
+    constexpr int RR = 1024 / GK, CH = GK / 16;          // rows of a wave's read, 16-byte chunks of a stage's row
+    constexpr int SH = GK == 64 ? 2 : 1;                 // rows that 64 banks hold: 1 << SH
+    constexpr int PX = BT / RR / NW, PW = BN / RR / NW, P = PX + PW;      // reads of a wave a stage, RR rows each
+    static_assert(PX * RR * NW == BT && PW * RR * NW == BN && (D - 1) * P < 64 && NW % 2 == 0, "whole reads");
+    constexpr int STAGE = (BT + BN) * GK;
     constexpr int FO = FN < 2 ? FN : 2;                  // channel tiles whose results leave together
     constexpr int YROW = 32 * FO * (int)sizeof(Y) + 16;  // a wave's row of results in LDS, 16 bytes apart
     constexpr int JO = TYPE == 0 || FT < 2 ? 1 : 2;      // token tiles
     constexpr int OUT = 32 * JO * YROW * WT * WN;
-    constexpr int BYTES = STAGE * 16 > OUT ? STAGE * 16 : OUT;
+    constexpr int BYTES = D * STAGE > OUT ? D * STAGE : OUT;
     __shared__ __attribute__((aligned(16))) char mem[BYTES];
     __shared__ __attribute__((aligned(16))) float sws[BN], sbias[BN], sqs[BT];
-    i32x4* lds = reinterpret_cast<i32x4*>(mem);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave / WN, wn = wave % WN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave / WN, wn = wave % WN;
     unsigned tt, tn;
     tile_of(a, tt, tn);
     const long long t0 = (long long)tt * BT;
-    const int n0 = (int)tn * BN, K = a.K, c = tid & 7;
+    const int n0 = (int)tn * BN, K = a.K, stages = (K + GK - 1) / GK;
     const int trows = (int)(a.T - t0 < BT ? a.T - t0 : BT), nrows = min(a.N - n0, BN);
-    // rows past the end repeat the last one; what they give is not stored
-    const int8_t* xb = a.q + t0 * a.ldq;
-    const int8_t* wb = a.w + (long long)n0 * a.ldw;
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xb), 0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wb), 0, 0x7fffffff, 0x00020000);
-    int xo[LT], wo[LN];
+    // the scales come first
+    static_assert(BN <= NT && BT <= NT, "one scale a thread");
+    const int sn = n0 + min(tid, nrows - 1);
+    const float vws = a.ws[sn], vbias = a.bias ? a.bias[sn] : 0.f, vqs = a.qs[t0 + min(tid, trows - 1)];
+    // A wave's read takes GK bytes of RR rows.  Chunk c of row r lies in LDS at r * CH + (c ^ ((r >> SH) % CH)): the 16 rows
+    // that a quarter wave reads one chunk of then lie in different banks.  Rows past the end repeat the last one;
+    // what they give is not stored.
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.q + t0 * a.ldq), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.w + (long long)n0 * a.ldw), 0, 0x7fffffff, 0x00020000);
+    const int chunk = ((lane & (CH - 1)) ^ ((RR * wave + lane / CH) >> SH & (CH - 1))) * 16;       // the same for all of a lane's rows
+    int xo[PX], wo[PW];
 #pragma unroll
-    for (int i = 0; i < LT; ++i) xo[i] = min((tid >> 3) + RP * i, trows - 1) * (int)a.ldq;
+    for (int i = 0; i < PX; ++i) xo[i] = min((wave + NW * i) * RR + lane / CH, trows - 1) * (int)a.ldq;
 #pragma unroll
-    for (int i = 0; i < LN; ++i) wo[i] = min((tid >> 3) + RP * i, nrows - 1) * (int)a.ldw;
-    i32x4 vx[LT], vw[LN];
-    const auto load = [&](int k0) {
-        const int k = k0 + 16 * c < K ? 16 * c : -k0;     // chunks past the end read the row's first one and count as zero
+    for (int i = 0; i < PW; ++i) wo[i] = min((wave + NW * i) * RR + lane / CH, nrows - 1) * (int)a.ldw;
+    const int last = (K + 15) / 16 * 16 - 16;                // a row's last 16 bytes
+    const auto fetch = [&](int st) {
+        char* to = mem + st % D * STAGE;
+        const int k = min(st * GK + chunk, last);
 #pragma unroll
-        for (int i = 0; i < LT; ++i) vx[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i] + k0 + k, 0, 0));
+        for (int i = 0; i < PX; ++i)
+            read_to_lds(xr, to + (wave + NW * i) * 1024, xo[i] + k);
 #pragma unroll
-        for (int i = 0; i < LN; ++i) vw[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wo[i] + k0 + k, 0, 0));
+        for (int i = 0; i < PW; ++i)
+            read_to_lds(wr, to + BT * GK + (wave + NW * i) * 1024, wo[i] + k);
     };
-    const auto store = [&](int k0) {
-        if (k0 + GK > K) {
+    const int at = (lane & 31) * GK + ((lane >> 5) ^ ((lane >> SH) & (CH - 1))) * 16;      // of step 0 in 32 rows; step 1: ^ 32
+    i32x4 fw[2][FN], fx[2][FT];
+    const auto read = [&](int st, int s) {
+        const char* from = mem + st % D * STAGE + (at ^ 32 * s);
 #pragma unroll
-            for (int i = 0; i < LN; ++i) vw[i] = below(vw[i], K - k0 - 16 * c);
+        for (int i = 0; i < FN; ++i) fw[s & 1][i] = *reinterpret_cast<const i32x4*>(from + (BT + (wn * FN + i) * 32) * GK);
+#pragma unroll
+        for (int j = 0; j < FT; ++j) fx[s & 1][j] = *reinterpret_cast<const i32x4*>(from + (wt * FT + j) * 32 * GK);
+        const int k = st * GK + 32 * s;
+        if (k + 32 > K) {           // what stands past K does not count
+#pragma unroll
+            for (int i = 0; i < FN; ++i) fw[s & 1][i] = below(fw[s & 1][i], K - k - 16 * (lane >> 5));
         }
-#pragma unroll
-        for (int i = 0; i < LT; ++i) lds[lds_slot((tid >> 3) + RP * i, c)] = vx[i];
-#pragma unroll
-        for (int i = 0; i < LN; ++i) lds[BT * 8 + lds_slot((tid >> 3) + RP * i, c)] = vw[i];
     };
     i32x16 acc[FN][FT];
 #pragma unroll
@@ -362,40 +390,49 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
         for (int j = 0; j < FT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    load(0);
-    // the scales follow on the first stage's reads
-    static_assert(BN <= NT && BT <= NT, "one scale a thread");
-    const int sn = n0 + min(tid, nrows - 1);
-    const float vws = a.ws[sn], vbias = a.bias ? a.bias[sn] : 0.f, vqs = a.qs[t0 + min(tid, trows - 1)];
-    store(0);
+    const auto multiply = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s & 1][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
+    };
+    const auto in_order = [] { __builtin_amdgcn_sched_barrier(0); };
+    // Every wave's part of a stage is there, and every wave has read the stage before it.
+    const auto arrived = [&](int st) {
+        if (st + D - 1 <= stages) wait_for<(D - 2) * P>();
+        else wait_for<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+#pragma unroll
+    for (int st = 0; st < D; ++st)
+        if (st < stages) fetch(st);
     if (tid < BN) {
         sws[tid] = vws;
         sbias[tid] = vbias;
     }
     if (tid < BT) sqs[tid] = vqs;
-    __syncthreads();
-    for (int k0 = 0; k0 < K; k0 += GK) {
-        const bool more = k0 + GK < K;
-        if (more) load(k0 + GK);
+    if (D <= stages) wait_for<(D - 1) * P>();
+    else wait_for<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0);
+    for (int st = 0; st < stages; ++st) {
 #pragma unroll
         for (int s = 0; s < GK / 32; ++s) {
-            const int cc = 2 * s + (lane >> 5);
-            i32x4 fw[FN], fx[FT];
-#pragma unroll
-            for (int i = 0; i < FN; ++i) fw[i] = lds[BT * 8 + lds_slot((wn * FN + i) * 32 + (lane & 31), cc)];
-#pragma unroll
-            for (int j = 0; j < FT; ++j) fx[j] = lds[lds_slot((wt * FT + j) * 32 + (lane & 31), cc)];
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
-        }
-        __syncthreads();
-        if (more) {
-            store(k0 + GK);
-            __syncthreads();
+            if (s + 1 < GK / 32) read(st, s + 1);
+            else if (st + 1 < stages) {
+                arrived(st + 1);
+                if (st + D < stages) fetch(st + D);
+                in_order();
+                read(st + 1, 0);
+            }
+            in_order();
+            multiply(s & 1);
+            in_order();
         }
     }
+    __syncthreads();
     // (In 16 bits, tokens 16 to 31 keep the two eights of every 16 bytes the other way round: a store's 32 lanes then touch
     // all 64 banks once.)
     // The results of 32 tokens at a time pass through the wave's part of LDS, to leave as whole lines of y's rows.
@@ -822,12 +859,12 @@ inline int row_align(const void* p, long long stride) {
 
 constexpr int FEW = 32, FEW_ELEMENTS = 32768;
 
-template <int FT, int FN, int WT, int WN, int MW, int TYPE>
+template <int FT, int FN, int WT, int WN, int GK, int D, int MW, int TYPE>
 void launch_gemm(GemmArgs a, hipStream_t st) {
     a.tn = (a.N + 32 * FN * WN - 1) / (32 * FN * WN);
     a.band = a.tn < 8 ? a.tn : 8;
     a.tt = (unsigned)((a.T + 32 * FT * WT - 1) / (32 * FT * WT));
-    gemm_q8_kernel<FT, FN, WT, WN, MW, TYPE><<<a.tt * a.tn, 64 * WT * WN, 0, st>>>(a);
+    gemm_q8_kernel<FT, FN, WT, WN, GK, D, MW, TYPE><<<a.tt * a.tn, 64 * WT * WN, 0, st>>>(a);
 }
 
 template <class F>
@@ -962,21 +999,24 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0,
                    row_align(y, ldy * type_bytes(y_type))};
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
-        // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's loads
-        // and results behind the other's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight
-        // waves, one block a CU), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
-        //   4096 x 4096 x 4096       71   82   97  116        16000 x 512 x 4096       58   53   64   73
-        //   4096 x 2048 x 4096       40   45   52   61        64000 x 256 x 2048       86   67   75   86
-        //   4096 x 1024 x 4096       26   27   30   34       256000 x 128 x 1024      147  130  152  165
-        // and 777 x 1001 x 1234 (20 .. 260 tiles) 21, 12, 9, 8.  A product of few tiles shares K among the waves of a block of
-        // 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0, 64 x 4096 x 1024 7.6 against 14.9, but
-        // 777 x 1001 x 1234 10.
+        // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
+        // behind another's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight waves, one block
+        // a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
+        //   4096 x 4096 x 4096     73   83   85   93  105        8192 x 8192 x 8192    505  560  650  690  830
+        //   16000 x 512 x 4096     55   49   52   61   73        4000 x 1000 x 2000     25   18   19   21   22
+        //   64000 x 256 x 2048     97   83   66   81   92      256000 x 128 x 1024     150  133  107  182  219
+        //   6000 x 1024 x 1024     19   13   14   12   14        2048 x 2048 x 2048     31   21   20   15   17
+        //   2000 x 2000 x 1000     31   20   21   15   13          600 x 2000 x 1000     31   19   20   13    9
+        // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
+        // shares K among the waves of a block of 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0,
+        // 64 x 4096 x 1024 7.6 against 14.9, but 777 x 1001 x 1234 10 against 9.5.
         if (T <= FEW || tiles(64, 64) <= 128) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
-        else if (N <= 32) launch_gemm<2, 1, 4, 1, 4, Y>(a, st);
-        else if (K >= 1024 && tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, 2, Y>(a, st);
-        else if (tiles(128, 128) >= 256) launch_gemm<2, 2, 2, 2, 4, Y>(a, st);
-        else if (tiles(128, 64) >= 256) launch_gemm<2, 1, 2, 2, 4, Y>(a, st);
-        else launch_gemm<1, 1, 2, 2, 4, Y>(a, st);
+        else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
+        else if (K >= 1024 && tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
+        else if (K >= 512 && tiles(128, 256) >= 224) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
+        else if (tiles(128, 128) >= 512) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
+        else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
+        else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);
     });
 }
 

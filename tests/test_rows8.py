@@ -142,6 +142,22 @@ def test_gemm_q8(hip, T, K, N, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,N,Ks", [(4097, 4100, (1024, 1030)), (7300, 1025, (512, 1001)), (6500, 1300, (1, 64, 65, 128, 190, 200, 256, 500)),
+                                    (5000, 1100, (1, 128, 129, 256, 300, 513, 700)), (1000, 700, (1, 127, 129, 300, 385, 2000)),
+                                    (100000, 30, (1, 64, 70, 129, 200)), (9000, 32, (33, 4096))])
+def test_gemm_q8_of_every_tile(hip, T, N, Ks):
+    """Each tile size with K of one stage of its ring, of a few, of more than it holds, and with a rest.  (The sums of the oracle
+    are whole numbers below 2^53: exact on the device too.)"""
+    for K in Ks:
+        q, w, qs, ws, bias = product_case(T + K + N, T, K, N)
+        y = torch.full((T + 1, N), 7.0, dtype=torch.bfloat16, device=DEV)
+        hip.gemm_q8(rows8(q, 5), qs.to(DEV), rows8(w, -3), ws.to(DEV), y[:T], bias.to(DEV))
+        want, tol = (v.cpu() for v in product64(*(v.to(DEV) for v in (q, qs, w, ws, bias))))
+        check_product(y[:T], want, tol, torch.bfloat16)
+        assert bool((y[T] == 7).all())
+
+
+@pytest.mark.gpu
 def test_the_sum_is_exact_at_its_largest(hip):
     K = 131072
     q = torch.full((3, K), 127, dtype=torch.int8)

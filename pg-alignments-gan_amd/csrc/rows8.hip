@@ -970,9 +970,12 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
         return PGAN_EINVAL;
     const bool vec = row_align(x, ldx * type_bytes(x_type)) >= 4 && row_align(q, ldq) >= 8;
     const int log = lanes_log(K);    // lanes a row
-    // rows a lane: two where there are enough of them (16000 x 512 in bf16: 9.3 us with one, 6.7 with two)
+    // Rows of more than 2048 elements by a block: in a wave's registers 4096 x 4096 in bf16 took 14.9 us for 14.3, 3000 x 3001
+    // (borders of 2 bytes) 50 for 21, 300 x 4096 6.4 for 3.8, though 2000 x 4096 in fp32 10.9 for 11.6.
+    constexpr int LONG_ROW = 2048;
+    // Rows a lane: two where there are enough of them (16000 x 512 in bf16: 9.3 us with one, 6.7 with two)
     const int R = K <= 1024 && rows >= 8192 ? 2 : 1;
-    const long long groups = (rows + R - 1) / R, blocks = K > 4096 ? rows : (groups + (256 >> log) - 1) / (256 >> log);
+    const long long groups = (rows + R - 1) / R, blocks = K > LONG_ROW ? rows : (groups + (256 >> log) - 1) / (256 >> log);
     if (blocks > MAX_BLOCKS) return PGAN_EINVAL;
     return by_type(x_type, [&](auto t) {
         constexpr int X = t.value;
@@ -980,8 +983,7 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
             kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<X>::type*>(x), ldx, static_cast<int8_t*>(q), ldq,
                                                       scale, rows, K, lrelu, more...);
         };
-        if (K > 4096) vec ? go(quant_long_rows_kernel<X, true>) : go(quant_long_rows_kernel<X, false>);
-        else if (K > 2048) vec ? go(quant_rows_kernel<X, true, 8, 1>, log) : go(quant_rows_kernel<X, false, 8, 1>, log);
+        if (K > LONG_ROW) vec ? go(quant_long_rows_kernel<X, true>) : go(quant_long_rows_kernel<X, false>);
         else if (K > 1024) vec ? go(quant_rows_kernel<X, true, 4, 1>, log) : go(quant_rows_kernel<X, false, 4, 1>, log);
         else if (K > 512 && R == 2) vec ? go(quant_rows_kernel<X, true, 2, 2>, log) : go(quant_rows_kernel<X, false, 2, 2>, log);
         else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2, 1>, log) : go(quant_rows_kernel<X, false, 2, 1>, log);

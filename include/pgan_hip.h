@@ -264,7 +264,8 @@ int pgan_adam(float* p, const float* g, float* m, float* v, long long n, float l
  * weight decay.  bits 32: m and v are fp32.  bits 8: m and v hold e4m3 codes of m and of sqrt(v), one byte an element, and
  * m_scale / r_scale one power of two for every 256 elements (codes and scales of zeros are a fresh state); codes are rounded
  * stochastically from a hash of (seed, step, tensor's number, element).  Elements past a tensor's last one are left alone.
- * Refused (-1): two written buffers that share memory, pointers that are not aligned to their element.
+ * Refused (-1): a written buffer that shares memory with another one or with a gradient, pointers that are not aligned to
+ * their element.
  * step_dev: NULL (step >= 1 is the number of this step), or 4 device ints: [0] is incremented and used, [1] and [2] get the
  * corrections 1 / (1 - b1^t) and 1 / sqrt(1 - b2^t) as fp32 -- a captured graph then counts on every replay.
  * grad_scale as in pgan_adam.  (src/train_wgan_v2.py:489-490,612,634 step torch.optim.Adam.) */
@@ -340,7 +341,8 @@ int pgan_gemm(const float* A, const float* B, float* C, int M, int N, int K, int
 
 /* ---- products of 8-bit rows with a scale for each token and channel, for drawing alignments from a trained generator
  * (its ConvTranspose2d stacks, src/layers.py:91-147, in evaluation; no backward).  Types: 0 fp32, 1 bf16, 2 fp16; strides
- * in elements; no rows (T, rows, B = 0): nothing is launched.
+ * in elements; no rows (T, rows, B = 0): nothing is launched.  Refused (-1): an output whose first to last byte overlaps
+ * those of another operand, K or C past 2^30.
  * pgan_quant_rows: q[r][k] = rint(x[r][k] * 127 / max_k |x[r][k]|), scale[r] = max / 127, after LeakyReLU(0.1) of x when
  *   lrelu is set; bytes past K of a row of q are left alone.  A row with an infinity or a NaN: codes 0, scale NaN.
  * pgan_gemm_q8: y[t][n] = q_scale[t] w_scale[n] sum_k q[t][k] w[n][k] + bias[n] (bias may be NULL), K <= 131072.  Rows of q

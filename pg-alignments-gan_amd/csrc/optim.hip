@@ -168,7 +168,8 @@ struct AwStep {
     float size, keep, b1, c1, b2, c2, eps, gs, inv2;
 };
 // Square root rounded to the nearest: the hardware's is within one unit of it, and the sign of x - s s' for the two values
-// s' next to s says which of the three is nearest.
+// s' next to s says which of the three is nearest.  (Below 2^-100 that difference is lost in the denormals, and the
+// hardware's stays.)
 __device__ __forceinline__ float root_of(float x) {
     const float s = __builtin_amdgcn_sqrtf(x);
     const float lo = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1), hi = __builtin_bit_cast(float, __builtin_bit_cast(int, s) + 1);
@@ -378,8 +379,13 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
     const int size_of[3] = {4, 2, 2};
     try {
         // what is written: no two of these may share memory (the same tensor twice in the lists, a state for two of them)
-        std::vector<Span> out;
-        out.reserve((size_t)n * 5);
+        std::vector<Span> out, in;
+        out.reserve((size_t)n * 5 + 1);
+        in.reserve((size_t)n);
+        const auto add = [](std::vector<Span>& to, const void* q, long long bytes) {
+            const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
+            to.push_back(Span{lo, lo + (uintptr_t)bytes});
+        };
         for (int i = 0; i < n; ++i) {
             if (numel[i] < 0 || numel[i] > AW_MOST * AW_CHUNK || types[i] < 0 || types[i] > 8) return PGAN_EINVAL;
             if (numel[i] == 0) continue;
@@ -387,22 +393,25 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
             const int ps = size_of[types[i] % 3], gsz = size_of[types[i] / 3];
             if (!aligned(p[i], ps) || !aligned(g[i], gsz)) return PGAN_EINVAL;
             if (bits == 32 && (!aligned(m[i], 4) || !aligned(v[i], 4))) return PGAN_EINVAL;
-            const auto add = [&out](const void* q, long long bytes) {
-                const uintptr_t lo = reinterpret_cast<uintptr_t>(q);
-                out.push_back(Span{lo, lo + (uintptr_t)bytes});
-            };
-            add(p[i], numel[i] * ps);
-            add(m[i], numel[i] * (bits / 8));
-            add(v[i], numel[i] * (bits / 8));
+            add(in, g[i], numel[i] * gsz);
+            add(out, p[i], numel[i] * ps);
+            add(out, m[i], numel[i] * (bits / 8));
+            add(out, v[i], numel[i] * (bits / 8));
             if (bits == 8) {
                 const long long nb = (numel[i] + AW_BLOCK - 1) / AW_BLOCK * 4;
-                add(m_scale[i], nb);
-                add(r_scale[i], nb);
+                add(out, m_scale[i], nb);
+                add(out, r_scale[i], nb);
             }
         }
+        if (step_dev) add(out, step_dev, 16);
         std::sort(out.begin(), out.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
         for (size_t i = 1; i < out.size(); ++i)
             if (out[i].lo < out[i - 1].hi) return PGAN_EINVAL;
+        // nor may a gradient with any of them
+        for (const Span& s : in) {
+            const auto next = std::partition_point(out.begin(), out.end(), [&s](const Span& o) { return o.hi <= s.lo; });
+            if (next != out.end() && next->lo < s.hi) return PGAN_EINVAL;
+        }
     } catch (...) {
         return PGAN_EINVAL;
     }

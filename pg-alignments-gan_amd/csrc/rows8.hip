@@ -851,6 +851,7 @@ inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintp
 inline int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 constexpr long long MAX_STRIDE = 1 << 22;      // offsets of a tile's rows fit 31 bits
+constexpr int MAX_ROW = 1 << 30;               // elements, so that a place in a row plus a block's stride does too
 
 inline int row_align(const void* p, long long stride) {
     const uintptr_t u = reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride;
@@ -904,7 +905,7 @@ inline int lanes_log(int C) {
     return log;
 }
 inline bool fold_fits(int type, int B, int H, int W, int C) {
-    if (B < 0 || H < 1 || W < 1 || C < 1 || type < 0 || type > 2 || H > 32768 || W > 32768) return false;
+    if (B < 0 || H < 1 || W < 1 || C < 1 || C > MAX_ROW || type < 0 || type > 2 || H > 32768 || W > 32768) return false;
     return B <= ((MAX_BLOCKS * 256) >> lanes_log(C)) / (4LL * H * W);
 }
 template <bool Q8>
@@ -954,7 +955,9 @@ inline int gemm_args(const void* q, long long ldq, const float* q_scale, const v
     if (!apart({rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1), rows_of(q_scale, 1, T, 0, 4),
                 rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
-    return (T + 255) / 256 * ((N + 255) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
+    // fewer than 2^32 threads in every tiling: 512 for 256 x 256, and for the 32 channels of a product of few tiles
+    if ((N + 31LL) / 32 > MAX_BLOCKS / 2) return PGAN_EINVAL;
+    return (T + 255) / 256 * ((N + 255LL) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
 }
 
 }  // namespace
@@ -963,7 +966,7 @@ extern "C" {
 
 int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long ldq, float* scale, long long rows, int K,
                     int lrelu, hipStream_t st) {
-    if (rows < 0 || K < 1 || x_type < 0 || x_type > 2) return PGAN_EINVAL;
+    if (rows < 0 || K < 1 || K > MAX_ROW || x_type < 0 || x_type > 2) return PGAN_EINVAL;
     if (rows == 0) return PGAN_OK;
     if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4) || ldx < K || ldq < K) return PGAN_EINVAL;
     if (!apart({rows_of(x, rows, K, ldx, type_bytes(x_type)), rows_of(q, rows, K, ldq, 1, true), rows_of(scale, 1, rows, 0, 4, true)}))

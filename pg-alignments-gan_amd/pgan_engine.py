@@ -912,12 +912,17 @@ class Engine:
 
     def use_adamw(self, weight_decay: float = 0.01, state_bits: int = 32, seed: int = 0) -> None:
         """Step both networks with AdamW instead of Adam: decoupled weight decay on the weights of convolutions and the
-        linear head (norm parameters and biases decay not), states in 32 or in 8 bits (the 32-bit ones are then given
-        back).  seed: of the rounding of 8-bit states."""
+        linear head (norm parameters and biases decay not), states in 32 bits -- Adam's, as they stand -- or in 8 bits,
+        which start from zero and count their steps from one (the 32-bit ones are given back).  seed: of the rounding of
+        8-bit states.  Called before the launches of an iteration are recorded."""
         if not hasattr(self.ops, "adamw_plan"):
             raise RuntimeError("use_adamw needs the GPU op backend")
         if state_bits not in (32, 8):
             raise ValueError(f"states are held in 32 or in 8 bits, got {state_bits}")
+        if not weight_decay >= 0:
+            raise ValueError(f"weight_decay must not be negative, got {weight_decay}")
+        if state_bits == 32 and any(st.mflat is None for st in (self.D, self.G)):
+            raise RuntimeError("use_adamw: the states are held in 8 bits already")
         for k, st in enumerate((self.D, self.G)):
             names = list(st.p)
             scales = None
@@ -931,7 +936,7 @@ class Engine:
             plan = self.ops.adamw_plan([st.p[n] for n in names], [st.m[n] for n in names], [st.v[n] for n in names], scales)
             decay = [float(weight_decay) if st.p[n].dim() > 1 else 0.0 for n in names]
             st.adamw = (plan, [st.g[n] for n in names], decay, int(seed) + k,
-                        torch.tensor([st.step, 0, 0, 0], dtype=torch.int32, device=self.dev))
+                        torch.tensor([st.step if state_bits == 32 else 0, 0, 0, 0], dtype=torch.int32, device=self.dev))
 
     def _adam(self, st: FlatStore, lr: float) -> None:
         st.step += 1

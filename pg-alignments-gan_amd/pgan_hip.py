@@ -8,6 +8,7 @@ enqueues kernels on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import numbers
 import os
 from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 from typing import List, Optional, Sequence
@@ -463,7 +464,7 @@ class AdamWPlan:
         self._types = (None, None)
 
     def _per_tensor(self, x, what):
-        if isinstance(x, (int, float)):
+        if isinstance(x, float):
             return self._dt(*[x] * self.n)
         if len(x) != self.n:
             raise PganError(f"adamw: {len(x)} values of {what} for {self.n} tensors")
@@ -490,6 +491,8 @@ class AdamWPlan:
                 self._types = (kinds, self._it(*[p + 3 * ELEMENT_TYPES[k] for p, k in zip(self._ptypes, kinds)]))
             except KeyError as e:
                 raise PganError(f"adamw: gradients are float32, bfloat16 or float16, got {e}") from None
+        # numbers and lists of their own: a caller's list may change
+        lr, weight_decay = (x if type(x) is float else float(x) if isinstance(x, numbers.Real) else list(x) for x in (lr, weight_decay))
         if self._rates[0] is None or self._rates[0] != lr or self._rates[1] != weight_decay:
             self._rates = (lr, weight_decay, self._per_tensor(lr, "lr"), self._per_tensor(weight_decay, "weight_decay"))
         sd = None
@@ -1141,44 +1144,47 @@ class HipOps:
         _check(_lib.pgan_gemm(_ptr(a), _ptr(b), _ptr(c), M, N, K, 1, _stream()), "pgan_gemm")
 
     # ---------------- products of 8-bit rows (evaluation only: no backward) ----------------
-    def _float_rows(self, t, what):
+    def _float_rows(self, t, op, name):
         """(pointer, type code, rows, columns, row stride) of a 2-D view with contiguous rows."""
         kind = ELEMENT_TYPES.get(t.dtype)
         if t.get_device() != self._index:
-            self._here(t, what)
+            self._here(t, f"{op}: {name}")
         if kind is None or t.dim() != 2:
-            raise PganError(f"{what}: expected a 2-D float32, bfloat16 or float16 tensor, got {t.dtype} {tuple(t.shape)}")
+            raise PganError(f"{op}: {name}: expected a 2-D float32, bfloat16 or float16 tensor, got {t.dtype} {tuple(t.shape)}")
         rows, cols = t.shape
         ld, one = t.stride()
         if one != 1 and cols > 1:
-            raise PganError(f"{what}: the elements of a row must be neighbours, strides are {t.stride()}")
+            raise PganError(f"{op}: {name}: the elements of a row must be neighbours, strides are {t.stride()}")
         if rows < 2:
             ld = cols
         elif ld < cols:
-            raise PganError(f"{what}: rows overlap (stride {ld} for {cols} columns)")
+            raise PganError(f"{op}: {name}: rows overlap (stride {ld} for {cols} columns)")
         return t.data_ptr(), kind, rows, cols, ld
 
-    def _code_rows(self, t, what, rows, cols):
+    def _code_rows(self, t, op, name, rows, cols):
         """(pointer, row stride) of 8-bit rows: on 16-byte borders, readable up to a multiple of 16."""
         if t.get_device() != self._index:
-            self._here(t, what)
-        if t.dtype != torch.int8 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
-            raise PganError(f"{what}: expected int8 rows [{rows}, {cols}], got {t.dtype} {tuple(t.shape)} with strides "
+            self._here(t, f"{op}: {name}")
+        have, wide_as = t.shape if t.dim() == 2 else (-1, -1)
+        ld, one = t.stride() if have >= 0 else (0, 0)
+        if t.dtype != torch.int8 or have < rows or wide_as != cols or (one != 1 and cols > 1):
+            raise PganError(f"{op}: {name}: expected int8 rows [{rows}, {cols}], got {t.dtype} {tuple(t.shape)} with strides "
                             f"{t.stride()}")
         wide = (cols + 15) // 16 * 16
-        ld = t.stride(0) if t.shape[0] > 1 else wide
+        if have < 2:
+            ld = wide
         p = t.data_ptr()
         if p % 16 or ld % 16 or ld < cols:
-            raise PganError(f"{what}: rows must start on 16-byte borders (pgan_hip.rows8 makes such a buffer)")
+            raise PganError(f"{op}: {name}: rows must start on 16-byte borders (pgan_hip.rows8 makes such a buffer)")
         if rows and wide != cols and t.storage_offset() + (rows - 1) * ld + wide > t.untyped_storage().nbytes():
-            raise PganError(f"{what}: the last row is not readable up to a multiple of 16 bytes")
+            raise PganError(f"{op}: {name}: the last row is not readable up to a multiple of 16 bytes")
         return p, ld
 
-    def _scales(self, t, what, n):
+    def _scales(self, t, op, name, n):
         if t.get_device() != self._index:
-            self._here(t, what)
+            self._here(t, f"{op}: {name}")
         if t.dtype != torch.float32 or t.numel() < n or not t.is_contiguous():
-            raise PganError(f"{what}: expected a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
+            raise PganError(f"{op}: {name}: expected a contiguous float32 tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
         return t.data_ptr()
 
     @staticmethod
@@ -1194,31 +1200,31 @@ class HipOps:
     def quant_rows(self, x, q, scale, lrelu: bool = False) -> None:
         """Codes and scale of each row of x [T, K] (after LeakyReLU(0.1) if lrelu): q int8 [T, K], scale float32 [T] with
         x ~ q * scale.  A row that holds an infinity or a NaN gets codes 0 and the scale NaN."""
-        xp, xt, T, K, ldx = self._float_rows(x, "quant_rows: x")
+        xp, xt, T, K, ldx = self._float_rows(x, "quant_rows", "x")
         if K < 1:
             raise PganError("quant_rows: rows without elements have no scale")
-        qp, ldq = self._code_rows(q, "quant_rows: q", T, K)
-        rc = _lib.pgan_quant_rows(xp, xt, ldx, qp, ldq, self._scales(scale, "quant_rows: scale", T), T, K, int(lrelu),
+        qp, ldq = self._code_rows(q, "quant_rows", "q", T, K)
+        rc = _lib.pgan_quant_rows(xp, xt, ldx, qp, ldq, self._scales(scale, "quant_rows", "scale", T), T, K, int(lrelu),
                                   self._own_stream())
         if rc:
             self._refused(rc, "pgan_quant_rows", x=x, q=q, scale=scale)
 
     def _product_args(self, what, T, K, w, w_scale, y, bias):
-        yp, yt, ty, N, ldy = self._float_rows(y, f"{what}: y")
+        yp, yt, ty, N, ldy = self._float_rows(y, what, "y")
         if ty != T or w.shape[0] != N or K < 1 or N < 1 or (bias is not None and bias.numel() != N):
             raise PganError(f"{what}: {T} rows of {K} elements, w {tuple(w.shape)}, bias "
                             f"{None if bias is None else tuple(bias.shape)} and y {tuple(y.shape)} do not fit together")
-        wp, ldw = self._code_rows(w, f"{what}: w", N, K)
-        return N, wp, ldw, self._scales(w_scale, f"{what}: w_scale", N), \
-            None if bias is None else self._scales(bias, f"{what}: bias", N), yp, yt, ldy
+        wp, ldw = self._code_rows(w, what, "w", N, K)
+        return N, wp, ldw, self._scales(w_scale, what, "w_scale", N), \
+            None if bias is None else self._scales(bias, what, "bias", N), yp, yt, ldy
 
     def gemm_q8(self, q, q_scale, w, w_scale, y, bias=None) -> None:
         """y [T, N] = q_scale[t] w_scale[n] sum_k q[t, k] w[n, k] + bias[n]: q int8 [T, K], w int8 [N, K], y float32, bfloat16
         or float16; the sum is exact (K <= 131072)."""
         T, K = q.shape
         N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("gemm_q8", T, K, w, w_scale, y, bias)
-        qp, ldq = self._code_rows(q, "gemm_q8: q", T, K)
-        rc = _lib.pgan_gemm_q8(qp, ldq, self._scales(q_scale, "gemm_q8: q_scale", T), wp, ldw, ws, bp, yp, yt, ldy, T, N, K,
+        qp, ldq = self._code_rows(q, "gemm_q8", "q", T, K)
+        rc = _lib.pgan_gemm_q8(qp, ldq, self._scales(q_scale, "gemm_q8", "q_scale", T), wp, ldw, ws, bp, yp, yt, ldy, T, N, K,
                                self._own_stream())
         if rc:
             self._refused(rc, "pgan_gemm_q8", q=q, q_scale=q_scale, w=w, w_scale=w_scale, y=y, bias=bias)
@@ -1226,10 +1232,10 @@ class HipOps:
     def linear_q8(self, x, w, w_scale, y, q, q_scale, bias=None, lrelu: bool = False) -> None:
         """quant_rows(x) and gemm_q8 in one call.  q int8 [at least T, K] and q_scale [at least T] are scratch of the caller:
         what they hold afterwards is not part of the result (few tokens skip them)."""
-        xp, xt, T, K, ldx = self._float_rows(x, "linear_q8: x")
+        xp, xt, T, K, ldx = self._float_rows(x, "linear_q8", "x")
         N, wp, ldw, ws, bp, yp, yt, ldy = self._product_args("linear_q8", T, K, w, w_scale, y, bias)
-        qp, ldq = self._code_rows(q, "linear_q8: q", T, K)
-        rc = _lib.pgan_linear_q8(xp, xt, ldx, qp, ldq, self._scales(q_scale, "linear_q8: q_scale", T), wp, ldw, ws, bp, yp, yt, ldy,
+        qp, ldq = self._code_rows(q, "linear_q8", "q", T, K)
+        rc = _lib.pgan_linear_q8(xp, xt, ldx, qp, ldq, self._scales(q_scale, "linear_q8", "q_scale", T), wp, ldw, ws, bp, yp, yt, ldy,
                                  T, N, K, int(lrelu), self._own_stream())
         if rc:
             self._refused(rc, "pgan_linear_q8", x=x, w=w, w_scale=w_scale, y=y, q=q, q_scale=q_scale, bias=bias)
@@ -1242,7 +1248,7 @@ class HipOps:
                             f"{y.dtype} {tuple(y.shape)}")
         if shift is not None and shift.numel() != C:
             raise PganError(f"{what}: {shift.numel()} shifts for {C} channels")
-        return y.data_ptr(), kind, None if shift is None else self._scales(shift, f"{what}: shift", C)
+        return y.data_ptr(), kind, None if shift is None else self._scales(shift, what, "shift", C)
 
     def up_fold_q8(self, y, shift, q, scale) -> None:
         """y [B, H, W, (kh, kw, c)]: the taps of ConvTranspose2d(kernel 4, stride 2, padding 1) made as a product.  Sums the
@@ -1253,8 +1259,8 @@ class HipOps:
         B, H, W, _ = y.shape
         if pixels != 4 * B * H * W:
             raise PganError(f"up_fold_q8: q has {pixels} rows for {4 * B * H * W} pixels")
-        qp, ldq = self._code_rows(q, "up_fold_q8: q", pixels, C)
-        rc = _lib.pgan_up_fold_q8(yp, yt, hp, qp, ldq, self._scales(scale, "up_fold_q8: scale", pixels), B, H, W, C,
+        qp, ldq = self._code_rows(q, "up_fold_q8", "q", pixels, C)
+        rc = _lib.pgan_up_fold_q8(yp, yt, hp, qp, ldq, self._scales(scale, "up_fold_q8", "scale", pixels), B, H, W, C,
                                   self._own_stream())
         if rc:
             self._refused(rc, "pgan_up_fold_q8", y=y, shift=shift, q=q, scale=scale)
@@ -1270,7 +1276,7 @@ class HipOps:
             raise PganError(f"up_fold: out is {tuple(out.shape)} for y {tuple(y.shape)}")
         if act not in (0, 1, 2):
             raise PganError(f"up_fold: act is 0, 1 or 2, got {act}")
-        rc = _lib.pgan_up_fold(yp, yt, hp, self._scales(out, "up_fold: out", 4 * B * H * W * C), B, H, W, C, int(act),
+        rc = _lib.pgan_up_fold(yp, yt, hp, self._scales(out, "up_fold", "out", 4 * B * H * W * C), B, H, W, C, int(act),
                                self._own_stream())
         if rc:
             self._refused(rc, "pgan_up_fold", y=y, shift=shift, out=out)

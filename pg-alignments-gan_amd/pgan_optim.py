@@ -57,7 +57,7 @@ class AdamW(torch.optim.Optimizer):
         """The plan of these parameters, made anew where a parameter or a state is no longer the memory it was made for."""
         names = _STATE[bits]
         held = [[self.state[p][name] for p in ps] for name in names]
-        made_of = [p.data_ptr() for p in ps] + [t.data_ptr() for ts in held for t in ts]
+        made_of = [(p.data_ptr(), p.dtype, p.is_contiguous()) for p in ps] + [t.data_ptr() for ts in held for t in ts]
         old = self._plans.get(key)
         if old is not None and old[1] == made_of:
             return old[0]
@@ -100,6 +100,8 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW: with capturable=True all parameters of a group are stepped together")
                 counter = group.get("counter")
                 if counter is None:
+                    if capturing:
+                        raise RuntimeError("AdamW: make a step before the capture (it makes the counter on the device)")
                     counter = group["counter"] = torch.tensor([next(iter(by_step)), 0, 0, 0], dtype=torch.int32, device=ps[0].device)
             for k, (made, members) in enumerate(sorted(by_step.items(), key=lambda kv: kv[0])):
                 plan = self._plan((gi, k), members, group["state_bits"])

@@ -441,6 +441,8 @@ def main(argv=None):
         raise SystemExit("--optimizer must be adam or adamw, --state_bits 8 or 32")
     if draw_n < 0 or (draw_n > 0) != (args.draw_slab != "None") or (draw_n and data_size != 64):
         raise SystemExit("--draw_n and --draw_slab go together, and need --data_size 64")
+    if draw_n and not os.path.isdir(os.path.dirname(os.path.abspath(args.draw_slab))):
+        raise SystemExit(f"--draw_slab: there is no folder for {args.draw_slab}")
     act = "sigmoid" if args.gen == "sigGen" else "tanh"
     normalize = args.normalize or args.gen == "tanNorm"
     if args.plot:

@@ -389,3 +389,39 @@ def test_entry_point_refusals():
     if not torch.cuda.is_available():
         return
     assert call(k=0) == 0
+
+
+def test_a_gradient_may_not_share_memory_with_what_is_written():
+    """(No GPU needed: refused before anything is launched.)  Nor may the device's step counter."""
+    import pgan_hip
+    fn = pgan_hip._lib._real.pgan_adamw_multi
+    P, LL, I, D = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_double
+    two = lambda t, x, y: (t * 2)(x, y)
+    p, m, v, s, r = two(P, 4096, 1 << 16), two(P, 1 << 20, 1 << 21), two(P, 1 << 22, 1 << 23), two(P, 1 << 24, 1 << 25), two(P, 1 << 26, 1 << 27)
+
+    def call(g0, g1, bits=32, counter=None):
+        return fn(p, two(P, g0, g1), m, v, s, r, two(LL, 100, 300), two(I, 0, 0), two(D, 1e-3, 1e-3), two(D, 0.0, 0.0), 2, bits, 0.5, 0.999,
+                  1e-8, 1.0, 0, counter, 1, None)
+    free = 1 << 28
+    for bits in (32, 8):
+        for g0, g1 in ((4096, free), (free, 4096), ((1 << 16) + 1196, free), ((1 << 16) - 396, free), (free, (1 << 20) - 1196), (free, (1 << 21) + 296),
+                       (free, (1 << 23) - 4)):
+            assert call(g0, g1, bits) == -1, (bits, g0, g1)
+    for g1 in ((1 << 24) - 4, 1 << 27):
+        assert call(free, g1, 8) == -1
+    assert call(free, free, 32, (1 << 16) + 1196) == -1
+    assert call(free, free, 32, free) == -1
+
+
+@pytest.mark.gpu
+def test_a_callers_list_of_rates_may_change_between_steps(hip):
+    p = [torch.ones(10, device=DEV), torch.ones(10, device=DEV)]
+    z = lambda: [torch.zeros(10, device=DEV) for _ in p]
+    plan = hip.adamw_plan(p, z(), z())
+    lr, decay = [0.0, 0.5], [0.1, 0.1]
+    plan.step(z(), 1, lr, B1, B2, EPS, decay)        # no gradient: p (1 - lr wd)
+    lr[0], decay[1] = 0.5, 0.2
+    plan.step(z(), 2, lr, B1, B2, EPS, decay)
+    plan.step(z(), 3, np.float32(0.5), B1, B2, EPS, np.float64(0.5))
+    for t, want in zip(p, (0.95 * 0.75, 0.95 * 0.9 * 0.75)):
+        assert torch.allclose(t.cpu().double(), torch.full((10,), want, dtype=torch.float64), rtol=8 * U, atol=0)

@@ -476,3 +476,48 @@ def test_adamw_needs_the_gpu_backend():
     p.grad = torch.zeros(3)
     with pytest.raises(RuntimeError):
         AdamW([p]).step()
+
+
+@pytest.mark.gpu
+def test_optimizer_follows_its_parameters_and_counter():
+    from pgan_hip import PganError
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.randn(6, 4, device=DEV))
+    opt = AdamW([p], capturable=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    opt.load_state_dict(opt.state_dict())            # its counter on the device is made by the next eager step
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    opt.step()
+    assert int(opt.param_groups[0]["counter"][0]) == 2
+    p.data = p.data.t()                              # the same memory in another order
+    p.grad = torch.ones_like(p)
+    with pytest.raises(PganError):
+        opt.step()
+
+
+@pytest.mark.gpu
+def test_engine_adamw_refusals_and_late_start():
+    from pgan_hip import HipOps
+    from pgan_trainer import FusedTrainer
+    tr = FusedTrainer(HipOps(torch.device(DEV)), 8, DEV, critic_iter=1)
+    for bad in (dict(weight_decay=-1.0), dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            tr.eng.use_adamw(**bad)
+    tr.eng.D.step = tr.eng.G.step = 7                # as after seven steps of Adam
+    tr.eng.use_adamw(0.0)
+    assert int(tr.eng.D.adamw[4][0]) == 7            # goes on with Adam's moments
+    tr.eng.use_adamw(0.0, state_bits=8)
+    assert int(tr.eng.D.adamw[4][0]) == 0            # moments of zero are those of no step
+    with pytest.raises(RuntimeError):
+        tr.eng.use_adamw(0.0, state_bits=32)
+
+
+@pytest.mark.gpu
+def test_draw_slab_needs_its_folder(tmp_path):
+    import train_wgan_v2
+    with pytest.raises(SystemExit, match="no folder"):
+        train_wgan_v2.main(["--use_cuda", "--idir", str(tmp_path), "--odir", str(tmp_path), "--draw_n", "4", "--draw_slab", str(tmp_path / "none" / "x.slab")])

@@ -396,3 +396,17 @@ def test_entry_point_refusals():
         for bad in bads:
             assert fn(**bad) == -1, (fn.__name__, bad)
     assert quant(rows=0) == gemm(T=0) == linear(T=0) == fold8(B=0) == fold(B=0) == 0
+
+
+def test_entry_point_refuses_what_a_launch_cannot_hold():
+    """Rows whose places a 32-bit loop would run past, and more channels than a launch has threads for (no GPU needed)."""
+    import pgan_hip
+    lib = pgan_hip._lib._real
+    a, b, c, d, far = 1 << 12, 1 << 40, 1 << 44, 1 << 45, 1 << 46
+    big = (1 << 30) + 1
+    assert lib.pgan_quant_rows(a, 1, big, b, big, c, 1, big, 0, None) == -1
+    assert lib.pgan_up_fold_q8(a, 1, None, b, big, c, 1, 1, 1, big, None) == -1
+    assert lib.pgan_up_fold(a, 1, None, b, 1, 1, 1, big, 0, None) == -1
+    n = 1 << 29
+    assert lib.pgan_gemm_q8(a, 16, b, c, 16, d, None, far, 1, n, 1, n, 16, None) == -1
+    assert lib.pgan_linear_q8(a, 1, 16, b, 16, c, d, 16, 1 << 47, None, far, 1, n, 1, n, 16, 0, None) == -1

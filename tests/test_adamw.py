@@ -425,3 +425,41 @@ def test_a_callers_list_of_rates_may_change_between_steps(hip):
     plan.step(z(), 3, np.float32(0.5), B1, B2, EPS, np.float64(0.5))
     for t, want in zip(p, (0.95 * 0.75, 0.95 * 0.9 * 0.75)):
         assert torch.allclose(t.cpu().double(), torch.full((10,), want, dtype=torch.float64), rtol=8 * U, atol=0)
+
+
+@pytest.mark.gpu
+def test_elements_past_31_bits(hip, monkeypatch):
+    """A tensor of 2^31 + 700 elements, both its ends against the definition."""
+    n, t, lr, wd = (1 << 31) + 700, 4, 1e-3, 0.01
+    p = torch.full((n,), 0.25, dtype=torch.bfloat16, device=DEV)
+    g = torch.full((n,), 1e-3, dtype=torch.bfloat16, device=DEV)
+    code = lambda: torch.full((n,), 0x58, dtype=torch.uint8, device=DEV)
+    scale = lambda: torch.full((-(-n // BLOCK),), 2.0 ** -10, device=DEV)
+    m, v, ms, rs = code(), code(), scale(), scale()
+    ends = [(0, 1000), ((1 << 31) - 512, n)]
+    d = make(11, [hi - lo for lo, hi in ends], torch.bfloat16, torch.bfloat16, bits=8)
+    for i, (lo, hi) in enumerate(ends):
+        for whole, part in ((p, d["p"][i]), (g, d["g"][i]), (m, d["m"][i]), (v, d["v"][i])):
+            whole[lo:hi] = part.to(DEV)
+        for whole, part in ((ms, d["ms"][i]), (rs, d["rs"][i])):
+            whole[lo // BLOCK:-(-hi // BLOCK)] = part.to(DEV)
+    # the first range ends inside a block: the rest of that block is part of its scale
+    ends[0], lo = (0, 768), 0
+    f8 = lambda x: x.view(torch.float8_e4m3fn)
+    hip.adamw([p], [g], [f8(m)], [f8(v)], t, lr, B1, B2, EPS, wd, scales=([ms], [rs]), seed=5)
+    torch.cuda.synchronize()
+    for i, (lo, hi) in enumerate(ends):
+        k = hi - lo
+        m0, r0 = values8(d["m"][i][:k], d["ms"][i][:-(-k // BLOCK)]), values8(d["v"][i][:k], d["rs"][i][:-(-k // BLOCK)])
+        want, _, _, _, tol = step64(d["p"][i][:k], d["g"][i][:k], m0, r0 * r0, t, lr, wd)
+        within(f"p from {lo}", p[lo:hi], want, tol + half_step(want.abs() + tol, torch.bfloat16))
+
+        def bits_from(n, seed, step, index, lo=lo):
+            h = _mix(torch.full((n,), _mix((seed + step * 0xA54FF53B + index * 0x3C6EF373) & M32), dtype=torch.int64) ^ (torch.arange(lo, lo + n) & M32))
+            return h & 0xFFFF, h >> 16
+        monkeypatch.setitem(globals(), "random_bits", bits_from)
+        cm, cr, sm, sr = hold8(*states32(m0, r0 * r0, d["g"][i][:k].float()), 5, t, 0)
+        assert torch.equal(m[lo:hi].cpu(), cm) and torch.equal(v[lo:hi].cpu(), cr)
+        assert torch.equal(ms[lo // BLOCK:-(-hi // BLOCK)].cpu(), sm) and torch.equal(rs[lo // BLOCK:-(-hi // BLOCK)].cpu(), sr)
+    monkeypatch.undo()
+    torch.cuda.empty_cache()

@@ -410,3 +410,49 @@ def test_entry_point_refuses_what_a_launch_cannot_hold():
     n = 1 << 29
     assert lib.pgan_gemm_q8(a, 16, b, c, 16, d, None, far, 1, n, 1, n, 16, None) == -1
     assert lib.pgan_linear_q8(a, 1, 16, b, 16, c, d, 16, 1 << 47, None, far, 1, n, 1, n, 16, 0, None) == -1
+
+
+@pytest.mark.gpu
+def test_offsets_past_31_bits(hip):
+    """Rows, codes, results and taps whose last places lie past 2^31 elements; the first and last rows against the definition."""
+    rng = np.random.default_rng(2)
+    T, K, N = 270000, 8192, 40
+    x = torch.full((T, K), 0.5, dtype=torch.bfloat16, device=DEV)
+    q, s = torch.zeros(T, K, dtype=torch.int8, device=DEV), torch.zeros(T, device=DEV)
+    ends = torch.cat([torch.arange(3), torch.arange(T - 3, T)])
+    x[ends.to(DEV)] = rnd(rng, 6, K).to(torch.bfloat16).to(DEV)
+    hip.quant_rows(x, q, s)
+    want, ws = codes_of(x[ends.to(DEV)].float().cpu())
+    assert torch.equal(q[ends.to(DEV)].cpu(), want)
+    same(s[ends.to(DEV)].cpu(), ws)
+    _, w, _, wscale, bias = product_case(4, 1, K, N)
+    y = torch.zeros(T, N, device=DEV)
+    hip.gemm_q8(q, s, w.to(DEV), wscale.to(DEV), y, bias.to(DEV))
+    out, tol = product64(want, ws, w, wscale, bias)
+    check_product(y[ends.to(DEV)], out, tol, torch.float32)
+    del x, q, y
+    T, K, N = 70000, 64, 32768
+    q, w, qs, wscale, bias = product_case(5, T, K, N)
+    y = torch.zeros(T, N, dtype=torch.bfloat16, device=DEV)
+    hip.gemm_q8(q.to(DEV), qs.to(DEV), w.to(DEV), wscale.to(DEV), y, bias.to(DEV))
+    ends = torch.cat([torch.arange(3), torch.arange(T - 3, T)])
+    out, tol = product64(q[ends], qs[ends], w, wscale, bias)
+    check_product(y[ends.to(DEV)], out, tol, torch.bfloat16)
+    del y
+    B, H, W, C = 33000, 16, 16, 16
+    y = torch.full((B, H, W, 16 * C), 0.25, dtype=torch.bfloat16, device=DEV)
+    part = rnd(rng, 1, H, W, 16 * C).to(torch.bfloat16)
+    y[-1] = part[0].to(DEV)
+    q, s = torch.zeros(4 * B * H * W, C, dtype=torch.int8, device=DEV), torch.zeros(4 * B * H * W, device=DEV)
+    hip.up_fold_q8(y, None, q, s)
+    want, ws = codes_of(lrelu(fold32(part, None)).view(-1, C))
+    assert torch.equal(q[-4 * H * W:].cpu(), want)
+    same(s[-4 * H * W:].cpu(), ws)
+    one = torch.full((2100000, 8, 8, 16), 0.25, dtype=torch.bfloat16, device=DEV)
+    part = rnd(rng, 1, 8, 8, 16).to(torch.bfloat16)
+    one[-1] = part[0].to(DEV)
+    out = torch.zeros(2100000, 16, 16, 1, device=DEV)
+    hip.up_fold(one, None, out)
+    assert torch.equal(out[-1:].cpu(), fold32(part, None))
+    del one, out, y, q, s
+    torch.cuda.empty_cache()

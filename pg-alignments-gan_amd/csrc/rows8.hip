@@ -231,11 +231,12 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
 // of one token).  Stages of GK bytes along K go from memory straight into a ring of D in LDS, without a stop in registers: a
 // stage's place is refilled as soon as every wave has read its last step, which leaves the other D - 1 under way meanwhile.
 // A wave waits for its own reads of a stage by their count and meets the others at a barrier, once a stage; the operands of
-// a step of 32 are read from LDS while the step before is multiplied.
-// Bound by the matrix instructions and the power they draw where K is long (8192 x 8192 x 8192: 505 us, 2180 Top/s, 92% of
-// the rate of the library's product; 4096 x 4096 x 4096: 73 us, 64 with zeros for operands), by the results' way out where it
-// is short (256000 x 128 x 1024: 107 us, 5.2 TB/s).  With stages that went through registers into one place of LDS:
-// 4096 x 4096 x 4096 77 us, 16000 x 512 x 4096 53 for 48.5, 256000 x 128 x 1024 134, 2048 x 2048 x 2048 21 for 15.
+// a step of 32 are read from LDS between the products of the step before.
+// Bound by the matrix instructions and the power they draw where K is long (8192 x 8192 x 8192: 458 us, 2400 Top/s, the
+// rate of the library's product; 4096 x 4096 x 4096: 67 us, 2040 Top/s), by the results' way out where it is short (256000 x
+// 128 x 1024: 115 us, 4.8 TB/s).  With stages that went through registers into one place of LDS 4096 x 4096 x 4096 took 77
+// us and 2048 x 2048 x 2048 21 for 14; with all of a step's LDS reads before its products, and so the next stage's reads
+// from memory waited for at once, 74 and 15.
 __device__ __forceinline__ i32x4 below(i32x4 v, int left) {        // the first `left` of 16 bytes, zero behind them
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -313,11 +314,11 @@ __device__ __forceinline__ void wait_for() {
     __builtin_amdgcn_s_waitcnt((VM & 15) | 7 << 4 | (VM >> 4) << 14);
 }
 
-// 16 bytes a lane from `at` bytes into `from` to LDS: `to` + 16 * lane, without a stop in registers
-__device__ __forceinline__ void read_to_lds(__amdgpu_buffer_rsrc_t from, char* to, int at) {
+// 16 bytes a lane from `at` + `same` (the wave's) bytes into `from` to LDS: `to` + 16 * lane, without a stop in registers
+__device__ __forceinline__ void read_to_lds(__amdgpu_buffer_rsrc_t from, char* to, int at, int same) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef __attribute__((address_space(3))) void lds_void;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)to, 16, at, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)to, 16, at, same, 0, 0);
 #endif
 }
 
@@ -355,33 +356,24 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
     const int chunk = ((lane & (CH - 1)) ^ ((RR * wave + lane / CH) >> SH & (CH - 1))) * 16;       // the same for all of a lane's rows
     int xo[PX], wo[PW];
 #pragma unroll
-    for (int i = 0; i < PX; ++i) xo[i] = min((wave + NW * i) * RR + lane / CH, trows - 1) * (int)a.ldq;
+    for (int i = 0; i < PX; ++i) xo[i] = min((wave + NW * i) * RR + lane / CH, trows - 1) * (int)a.ldq + chunk;
 #pragma unroll
-    for (int i = 0; i < PW; ++i) wo[i] = min((wave + NW * i) * RR + lane / CH, nrows - 1) * (int)a.ldw;
-    const int last = (K + 15) / 16 * 16 - 16;                // a row's last 16 bytes
-    const auto fetch = [&](int st) {
-        char* to = mem + st % D * STAGE;
-        const int k = min(st * GK + chunk, last);
-#pragma unroll
-        for (int i = 0; i < PX; ++i)
-            read_to_lds(xr, to + (wave + NW * i) * 1024, xo[i] + k);
-#pragma unroll
-        for (int i = 0; i < PW; ++i)
-            read_to_lds(wr, to + BT * GK + (wave + NW * i) * 1024, wo[i] + k);
+    for (int i = 0; i < PW; ++i) wo[i] = min((wave + NW * i) * RR + lane / CH, nrows - 1) * (int)a.ldw + chunk;
+    const int last = (K + 15) / 16 * 16 - 16 - chunk;        // of a stage's first byte, so that a row's last 16 bytes are read at most
+    // one of the P reads of a stage; WHOLE: no place of the stage lies past K
+    const auto fetch = [&](auto whole, int st, int i) {
+        char* to = mem + st % D * STAGE + ((i < PX ? 0 : BT * GK) + (wave + NW * (i < PX ? i : i - PX)) * 1024);
+        const int at = whole.value ? st * GK : 0, more = whole.value ? 0 : min(st * GK, last);
+        if (i < PX) read_to_lds(xr, to, xo[i] + more, at);
+        else read_to_lds(wr, to, wo[i - PX] + more, at);
     };
-    const int at = (lane & 31) * GK + ((lane >> 5) ^ ((lane >> SH) & (CH - 1))) * 16;      // of step 0 in 32 rows; step 1: ^ 32
+    const int at = (lane & 31) * GK + ((lane >> 5) ^ ((lane >> SH) & (CH - 1))) * 16;      // of step 0 in 32 rows; step s: ^ 32 s
     i32x4 fw[2][FN], fx[2][FT];
-    const auto read = [&](int st, int s) {
+    // one of the FN + FT operands of a step, in the order in which they are needed
+    const auto read = [&](int st, int s, int r) {
         const char* from = mem + st % D * STAGE + (at ^ 32 * s);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) fw[s & 1][i] = *reinterpret_cast<const i32x4*>(from + (BT + (wn * FN + i) * 32) * GK);
-#pragma unroll
-        for (int j = 0; j < FT; ++j) fx[s & 1][j] = *reinterpret_cast<const i32x4*>(from + (wt * FT + j) * 32 * GK);
-        const int k = st * GK + 32 * s;
-        if (k + 32 > K) {           // what stands past K does not count
-#pragma unroll
-            for (int i = 0; i < FN; ++i) fw[s & 1][i] = below(fw[s & 1][i], K - k - 16 * (lane >> 5));
-        }
+        if (r == 0 || r > FT) fw[s & 1][r == 0 ? 0 : r - FT] = *reinterpret_cast<const i32x4*>(from + (BT + (wn * FN + (r == 0 ? 0 : r - FT)) * 32) * GK);
+        else fx[s & 1][r - 1] = *reinterpret_cast<const i32x4*>(from + (wt * FT + r - 1) * 32 * GK);
     };
     i32x16 acc[FN][FT];
 #pragma unroll
@@ -390,23 +382,17 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
         for (int j = 0; j < FT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    const auto multiply = [&](int s) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s & 1][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
-    };
     const auto in_order = [] { __builtin_amdgcn_sched_barrier(0); };
-    // Every wave's part of a stage is there, and every wave has read the stage before it.
-    const auto arrived = [&](int st) {
-        if (st + D - 1 <= stages) wait_for<(D - 2) * P>();
-        else wait_for<0>();
+    const auto meet = [] {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    using std::bool_constant;
 #pragma unroll
     for (int st = 0; st < D; ++st)
-        if (st < stages) fetch(st);
+        if (st < stages)
+#pragma unroll
+            for (int i = 0; i < P; ++i) fetch(bool_constant<false>{}, st, i);
     if (tid < BN) {
         sws[tid] = vws;
         sbias[tid] = vbias;
@@ -414,24 +400,49 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
     if (tid < BT) sqs[tid] = vqs;
     if (D <= stages) wait_for<(D - 1) * P>();
     else wait_for<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(0, 0);
-    for (int st = 0; st < stages; ++st) {
+    meet();
 #pragma unroll
-        for (int s = 0; s < GK / 32; ++s) {
-            if (s + 1 < GK / 32) read(st, s + 1);
-            else if (st + 1 < stages) {
-                arrived(st + 1);
-                if (st + D < stages) fetch(st + D);
-                in_order();
-                read(st + 1, 0);
+    for (int r = 0; r < FN + FT; ++r) read(0, 0, r);
+    // A stage's products, and between them the reads of the next step's operands and of stage st + D.  WHAT: 0 that is a whole
+    // stage, 1 it is the last, 2 there is none, 3 nor a next one.
+    const auto stage = [&](auto what, int st) {
+        constexpr int WHAT = what.value, STEPS = GK / 32, NM = FN * FT, H = NM < 2 ? 1 : NM / 2;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const bool end = s + 1 == STEPS, more = !end || WHAT < 3;
+            if (end && more) {      // every wave's part of the next stage is there, and every wave has read this one
+                if (WHAT < 2 || st + D <= stages) wait_for<(D - 2) * P>();
+                else wait_for<0>();
+                meet();
+            }
+            if (WHAT == 3 && st * GK + 32 * s + 32 > K) {      // what stands past K does not count
+#pragma unroll
+                for (int i = 0; i < FN; ++i) fw[s & 1][i] = below(fw[s & 1][i], K - st * GK - 32 * s - 16 * (lane >> 5));
             }
             in_order();
-            multiply(s & 1);
-            in_order();
+#pragma unroll
+            for (int n = 0; n < NM; ++n) {
+                const int i = n / FT, j = n % FT;
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s & 1][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
+                in_order();
+                // LDS is read before it is written to: the compiler lets no read of it pass a write from memory
+                if (more && n < H)
+#pragma unroll
+                    for (int r = n * (FN + FT) / H; r < (n + 1) * (FN + FT) / H; ++r) read(end ? st + 1 : st, end ? 0 : s + 1, r);
+                in_order();
+                if (WHAT < 2 && end && n >= NM - H)
+#pragma unroll
+                    for (int f = (n - NM + H) * P / H; f < (n - NM + H + 1) * P / H; ++f) fetch(bool_constant<WHAT == 0>{}, st + D, f);
+                in_order();
+            }
         }
-    }
+    };
+    using std::integral_constant;
+    int st = 0;
+    for (; st < stages - D - 1; ++st) stage(integral_constant<int, 0>{}, st);
+    if (st < stages - D) stage(integral_constant<int, 1>{}, st++);
+    for (; st < stages - 1; ++st) stage(integral_constant<int, 2>{}, st);
+    stage(integral_constant<int, 3>{}, st);
     __syncthreads();
     // (In 16 bits, tokens 16 to 31 keep the two eights of every 16 bytes the other way round: a store's 32 lanes then touch
     // all 64 banks once.)
@@ -1006,20 +1017,20 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
         // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
         // behind another's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight waves, one block
-        // a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
-        //   4096 x 4096 x 4096     73   83   85   93  105        8192 x 8192 x 8192    505  560  650  690  830
-        //   16000 x 512 x 4096     55   49   52   61   73        4000 x 1000 x 2000     25   18   19   21   22
-        //   64000 x 256 x 2048     97   83   66   81   92      256000 x 128 x 1024     150  133  107  182  219
-        //   6000 x 1024 x 1024     19   13   14   12   14        2048 x 2048 x 2048     31   21   20   15   17
-        //   2000 x 2000 x 1000     31   20   21   15   13          600 x 2000 x 1000     31   19   20   13    9
+        // a CU), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
+        //   4096 x 4096 x 4096     64   86   84    -       16000 x 512 x 4096     66   61   75   85
+        //   3000 x 4000 x 3000     52   66   65   77       64000 x 256 x 2048     98   84  107  113
+        //   2000 x 8000 x 2000     81   64   51   65      256000 x 128 x 1024    147  118  187  257
+        //   5000 x 2048 x 2000     31   31   31   39        8000 x 1024 x 1024    17   15   17   20
+        //   2048 x 2048 x 2048     23   16   15   16         777 x 1001 x 1234    17    9    8    8
+        //   4000 x 1000 x 2000     22   18   19   21         600 x 2000 x 1000    24   14    9    8
         // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
         // shares K among the waves of a block of 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0,
-        // 64 x 4096 x 1024 7.6 against 14.9, but 777 x 1001 x 1234 10 against 9.5.
+        // 64 x 4096 x 1024 7.6 against 14.9, but 777 x 1001 x 1234 10 against 8.
         if (T <= FEW || tiles(64, 64) <= 128) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
         else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
-        else if (K >= 1024 && tiles(256, 256) >= 256) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
-        else if (K >= 512 && tiles(128, 256) >= 224) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
-        else if (tiles(128, 128) >= 512) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
+        else if (K >= 1024 && tiles(256, 256) >= (K < 2048 ? 256 : 144)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
+        else if (tiles(128, 128) >= 448) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
         else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
         else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);
     });

@@ -191,8 +191,9 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYP
     }
 }
 
-// longer rows: one a block, read twice (the second time from the L1 or L2)
-template <int TYPE, bool VEC>
+// Longer rows: one a block.  NIT > 0: the values stay in registers, 8 NIT of a thread (K <= 2048 NIT, VEC); 0: rows are read
+// twice, the second time from the L1 or L2.  8192 x 8192 in bf16, from memory: 42.5 us, 4.7 TB/s (read twice: 49).
+template <int TYPE, bool VEC, int NIT>
 __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                               int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                                                               long long rows, int K, int lrelu) {
@@ -202,11 +203,27 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
     int8_t* qr = q + row * ldq;
     const int whole = VEC ? K / 8 * 8 : 0;          // elements that are read eight at a time
     uint32_t mx = 0;
-    for (int k = threadIdx.x * 8; k < whole; k += 2048) {
-        float v[8];
-        load8<TYPE>(xr + k, v);
+    const auto top = [&](float (&v)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = max(mx, magnitude(slope(v[e], lrelu)));
+        for (int e = 0; e < 8; ++e) {
+            v[e] = slope(v[e], lrelu);
+            mx = max(mx, magnitude(v[e]));
+        }
+    };
+    float kept[NIT > 0 ? NIT : 1][8];
+    if constexpr (NIT > 0) {
+#pragma unroll
+        for (int i = 0; i < NIT; ++i)
+            if (threadIdx.x * 8 + 2048 * i < whole) load8<TYPE>(xr + threadIdx.x * 8 + 2048 * i, kept[i]);
+#pragma unroll
+        for (int i = 0; i < NIT; ++i)
+            if (threadIdx.x * 8 + 2048 * i < whole) top(kept[i]);
+    } else {
+        for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+            float v[8];
+            load8<TYPE>(xr + k, v);
+            top(v);
+        }
     }
     for (int k = whole + threadIdx.x; k < K; k += 256) mx = max(mx, magnitude(slope(to_f32<TYPE>(xr[k]), lrelu)));
     mx = group_max(mx, 6);
@@ -214,13 +231,22 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
     __syncthreads();
     const RowScale rs = row_scale(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
     if (threadIdx.x == 0) scale[row] = rs.scale;
-    for (int k = threadIdx.x * 8; k < whole; k += 2048) {
-        float v[8];
-        load8<TYPE>(xr + k, v);
+    const auto put = [&](int k, float (&v)[8]) {
         no_row(v, rs.inv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = slope(v[e], lrelu);
         *reinterpret_cast<uint2*>(qr + k) = uint2{four_codes(v[0], v[1], v[2], v[3], rs.inv), four_codes(v[4], v[5], v[6], v[7], rs.inv)};
+    };
+    if constexpr (NIT > 0) {
+#pragma unroll
+        for (int i = 0; i < NIT; ++i)
+            if (threadIdx.x * 8 + 2048 * i < whole) put(threadIdx.x * 8 + 2048 * i, kept[i]);
+    } else {
+        for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+            float v[8];
+            load8<TYPE>(xr + k, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = slope(v[e], lrelu);
+            put(k, v);
+        }
     }
     for (int k = whole + threadIdx.x; k < K; k += 256) qr[k] = rs.inv == 0.f ? 0 : (int8_t)code_of(slope(to_f32<TYPE>(xr[k]), lrelu), rs.inv);
 }
@@ -984,9 +1010,9 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
         return PGAN_EINVAL;
     const bool vec = row_align(x, ldx * type_bytes(x_type)) >= 4 && row_align(q, ldq) >= 8;
     const int log = lanes_log(K);    // lanes a row
-    // Rows of more than 2048 elements by a block: in a wave's registers 4096 x 4096 in bf16 took 14.9 us for 14.3, 3000 x 3001
-    // (borders of 2 bytes) 50 for 21, 300 x 4096 6.4 for 3.8, though 2000 x 4096 in fp32 10.9 for 11.6.
-    constexpr int LONG_ROW = 2048;
+    // Rows of more than 1024 elements by a block: in a wave's registers 4096 x 4096 in bf16 took 14.9 us for 12.9, 8192 x 2048
+    // 15.0 for 12.8, 300 x 2048 4.2 for 2.8, 3000 x 3001 (borders of 2 bytes) 50 for 21, though 4000 x 1024 6.0 for 6.4.
+    constexpr int LONG_ROW = 1024;
     // Rows a lane: two where there are enough of them (16000 x 512 in bf16: 9.3 us with one, 6.7 with two)
     const int R = K <= 1024 && rows >= 8192 ? 2 : 1;
     const long long groups = (rows + R - 1) / R, blocks = K > LONG_ROW ? rows : (groups + (256 >> log) - 1) / (256 >> log);
@@ -997,8 +1023,11 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
             kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<X>::type*>(x), ldx, static_cast<int8_t*>(q), ldq,
                                                       scale, rows, K, lrelu, more...);
         };
-        if (K > LONG_ROW) vec ? go(quant_long_rows_kernel<X, true>) : go(quant_long_rows_kernel<X, false>);
-        else if (K > 1024) vec ? go(quant_rows_kernel<X, true, 4, 1>, log) : go(quant_rows_kernel<X, false, 4, 1>, log);
+        if (K > LONG_ROW && !vec) go(quant_long_rows_kernel<X, false, 0>);
+        else if (K > 8192) go(quant_long_rows_kernel<X, true, 0>);
+        else if (K > 4096) go(quant_long_rows_kernel<X, true, 4>);
+        else if (K > 2048) go(quant_long_rows_kernel<X, true, 2>);
+        else if (K > LONG_ROW) go(quant_long_rows_kernel<X, true, 1>);
         else if (K > 512 && R == 2) vec ? go(quant_rows_kernel<X, true, 2, 2>, log) : go(quant_rows_kernel<X, false, 2, 2>, log);
         else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2, 1>, log) : go(quant_rows_kernel<X, false, 2, 1>, log);
         else if (R == 2) vec ? go(quant_rows_kernel<X, true, 1, 2>, log) : go(quant_rows_kernel<X, false, 1, 2>, log);

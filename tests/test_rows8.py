@@ -456,3 +456,25 @@ def test_offsets_past_31_bits(hip):
     assert torch.equal(out[-1:].cpu(), fold32(part, None))
     del one, out, y, q, s
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [1025, 1032, 2047, 2056, 4097, 4104, 8190, 8192, 8200])
+def test_quant_rows_of_more_than_a_wave(hip, K, dtype):
+    """Rows of a block, on borders of 16 bytes and of one element, an infinity and a NaN in their last elements."""
+    rng = np.random.default_rng(K)
+    x = rnd(rng, 9, K) * torch.exp(2 * rnd(rng, 9, 1))
+    x[3, K - 1], x[5, K - 2] = float("inf"), float("nan")
+    x[7, K - 1] = 100.0
+    x = x.to(dtype)
+    for gap in (0, 1, 16 - K % 8):
+        for neg in (False, True):
+            view = torch.full((9, K + gap), float("nan"), dtype=dtype, device=DEV)[:, :K]
+            view.copy_(x.to(DEV))
+            want, ws = codes_of(lrelu(x.float()) if neg else x.float())
+            q, s = rows8(torch.zeros(9, K, dtype=torch.int8)), torch.zeros(9, device=DEV)
+            hip.quant_rows(view, q, s, lrelu=neg)
+            assert torch.equal(q.cpu(), want)
+            same(s.cpu(), ws)
+            rest_kept(q)

@@ -13,7 +13,10 @@
 // 1): a zero denominator beside an m that survived its own rounding would throw the parameter off by m / eps.  A state that
 // is not finite is held as NaN, as it would poison the element in 32 bits too; it does not touch its block's scale.
 //
-// Bound by HBM: 28 bytes an element with fp32 states, 16 with 8-bit ones.
+// One launch for all tensors, as most of a network's are tiny: a block takes 2048 elements of one of them (a wave two blocks
+// of 256 with 8-bit states, the second's reads under way while the first is computed).  Bound by HBM: 28 bytes an element
+// with fp32 states (36 M elements: 191 us, 5.25 TB/s; a copy makes 4.86), 10 in bf16 with 8-bit ones (46 M elements: 98 us,
+// 4.7 TB/s, hash and codes take almost as long), 26 tensors of 2.8 M elements 13 us.
 #include <algorithm>
 #include <vector>
 

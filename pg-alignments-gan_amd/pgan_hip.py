@@ -491,8 +491,10 @@ class AdamWPlan:
                 self._types = (kinds, self._it(*[p + 3 * ELEMENT_TYPES[k] for p, k in zip(self._ptypes, kinds)]))
             except KeyError as e:
                 raise PganError(f"adamw: gradients are float32, bfloat16 or float16, got {e}") from None
-        # numbers and lists of their own: a caller's list may change
-        lr, weight_decay = (x if type(x) is float else float(x) if isinstance(x, numbers.Real) else list(x) for x in (lr, weight_decay))
+        if type(lr) is not float:           # a caller's list may change
+            lr = float(lr) if isinstance(lr, numbers.Real) else list(lr)
+        if type(weight_decay) is not float:
+            weight_decay = float(weight_decay) if isinstance(weight_decay, numbers.Real) else list(weight_decay)
         if self._rates[0] is None or self._rates[0] != lr or self._rates[1] != weight_decay:
             self._rates = (lr, weight_decay, self._per_tensor(lr, "lr"), self._per_tensor(weight_decay, "weight_decay"))
         sd = None

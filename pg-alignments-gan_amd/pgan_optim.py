@@ -43,15 +43,16 @@ class AdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         self._plans = {}
 
+    @staticmethod
+    def _layout(p, bits):
+        """Names of a parameter's states with their types and elements."""
+        n, blocks = p.numel(), -(-p.numel() // ADAMW_BLOCK)
+        kinds = [(torch.float32, n)] * 2 if bits == 32 else [(torch.float8_e4m3fn, n)] * 2 + [(torch.float32, blocks)] * 2
+        return dict(zip(_STATE[bits], kinds))
+
     def _fresh(self, p, bits):
-        n = p.numel()
-        if bits == 32:
-            made = (torch.zeros(n, device=p.device), torch.zeros(n, device=p.device))
-        else:
-            code = lambda: torch.zeros(n, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
-            scale = lambda: torch.zeros(-(-n // ADAMW_BLOCK), device=p.device)
-            made = (code(), code(), scale(), scale())
-        return dict(zip(_STATE[bits], made))
+        zeros = lambda dtype, n: torch.zeros(n * dtype.itemsize, dtype=torch.uint8, device=p.device).view(dtype)
+        return {name: zeros(*kind) for name, kind in self._layout(p, bits).items()}
 
     def _plan(self, key, ps, bits):
         """The plan of these parameters, made anew where a parameter or a state is no longer the memory it was made for."""
@@ -131,9 +132,18 @@ class AdamW(torch.optim.Optimizer):
                         self.state[p]["step"] = made
 
     def load_state_dict(self, state_dict):
-        """States keep the types they are held in (torch's own loading would cast codes and scales to the parameter's)."""
+        """States keep the types they are held in (torch's own loading would cast codes and scales to the parameter's) and, where
+        they are there already, their memory: a captured step goes on from what was loaded."""
         state_dict = copy.copy(state_dict)
-        saved = state_dict["state"]
+        saved, held = state_dict["state"], dict(self.state)
+        counters = [g.get("counter") for g in self.param_groups]
+        for own, g in zip(self.param_groups, state_dict["param_groups"]):      # before anything is changed
+            for i, p in zip(g["params"], own["params"]):
+                b = g.get("state_bits", self.defaults["state_bits"])
+                for name, (dtype, n) in self._layout(p, b).items() if i in saved else ():
+                    t = saved[i].get(name)
+                    if t is None or t.dtype != dtype or t.numel() != n:
+                        raise ValueError(f"AdamW: the saved state holds no {name} of {n} elements in {dtype}")
         super().load_state_dict({**state_dict, "state": {}})
         for g in self.param_groups:     # options that another AdamW's groups do not have
             for k, v in self.defaults.items():
@@ -141,20 +151,26 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ps = [p for g in self.param_groups for p in g["params"]]
         bits = [g["state_bits"] for g in self.param_groups for _ in g["params"]]
-        self.state.clear()
+        loaded = {}
         for i, p, b in zip(ids, ps, bits):
             if i not in saved:
                 continue
-            st, want = saved[i], self._fresh(p, b)
+            st, had = saved[i], held.get(p, {})
             new = {"step": int(st["step"])}
-            for name, like in want.items():
-                t = st.get(name)
-                if t is None or t.dtype != like.dtype or t.numel() != like.numel():
-                    raise ValueError(f"AdamW: the saved state holds no {name} of {like.numel()} elements in {like.dtype}")
-                new[name] = t.detach().to(p.device).reshape(-1).clone()
+            for name, like in self._fresh(p, b).items():
+                there = had.get(name)
+                new[name] = there if there is not None and there.dtype == like.dtype and there.numel() == like.numel() else like
+                loaded[p, name] = st[name].detach().reshape(-1)
             self.state[p] = new
-        for group in self.param_groups:
-            group.pop("counter", None)
+        for (p, name), t in loaded.items():
+            self.state[p][name].view(torch.uint8).copy_(t.contiguous().view(torch.uint8))
+        for group, counter in zip(self.param_groups, counters):
+            steps = {self.state[p]["step"] for p in group["params"] if p in self.state}
+            if counter is not None and len(steps) == 1 and group["capturable"]:
+                counter.copy_(torch.tensor([steps.pop(), 0, 0, 0], dtype=torch.int32))
+                group["counter"] = counter
+            else:
+                group.pop("counter", None)
         self._plans = {}
 
 

@@ -21,7 +21,8 @@ BN_EPS = 1e-5
 
 
 class Sampler8:
-    """sites, positions = Sampler8(...).draw(z), z [n <= batch, latent]; refresh() after the weights have changed."""
+    """sites, positions = Sampler8(...).draw(z), z [n <= batch, latent], of the weights and running statistics that the last
+    refresh() took over, also where a captured draw is replayed."""
 
     def __init__(self, ops, params: Dict[str, torch.Tensor], buffers: Dict[str, torch.Tensor], batch: int, act: str = "sigmoid",
                  latent: int = 128, data: int = 64):
@@ -50,6 +51,9 @@ class Sampler8:
         self.hA = [None] + [torch.zeros(B, self.g1c[i], self.g1l[i], **f) for i in range(1, self.n + 1)]
         self.hH = [None] + [torch.zeros(B, self.g1c[i], self.g1l[i], **f) for i in range(1, self.n + 1)]
         self.stats = [None] + [torch.zeros(2, self.g1c[i], **f) for i in range(1, self.n + 1)]
+        self.w1 = [torch.empty_like(params[f"oned_conv_layers.{3 * i}.weight"]) for i in range(self.n + 1)]
+        self.norm1 = [None] + [tuple(torch.zeros(self.g1c[i], **f) for _ in range(4)) for i in range(1, self.n + 1)]
+        self._parts = {}            # batch size -> running statistics in the form the BatchNorm kernels take sums
         self.refresh()
 
     def _norm(self, tower: str, i: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -70,7 +74,15 @@ class Sampler8:
                 self.ws[i].mul_(gain.repeat(16))
                 self.shift[i].copy_(shift)
         self.bias0.copy_(self.shift[0].repeat(16))
-        self._parts = {}            # batch size -> running statistics in the form the BatchNorm kernels take sums
+        for i in range(self.n + 1):
+            self.w1[i].copy_(self.P[f"oned_conv_layers.{3 * i}.weight"])
+            if i > 0:
+                k = f"oned_conv_layers.{3 * (i - 1) + 1}"
+                for to, of in zip(self.norm1[i], (self.P[k + ".weight"], self.P[k + ".bias"], self.Bf[k + ".running_mean"],
+                                                  self.Bf[k + ".running_var"])):
+                    to.copy_(of)
+        for n in self._parts:
+            self._fill_sums(n)
 
     def _running_sums(self, n: int):
         """The running statistics as the batch sums that give them: per channel sum and sum of squares of n x length
@@ -78,17 +90,16 @@ class Sampler8:
         if n not in self._parts:
             if torch.cuda.is_current_stream_capturing():
                 raise PganError(f"draw: make one draw of {n} alignments before capturing one")
-            parts = [None]
-            for i in range(1, self.n + 1):
-                k = f"oned_conv_layers.{3 * (i - 1) + 1}"
-                mean, var = self.Bf[k + ".running_mean"].double(), self.Bf[k + ".running_var"].double()
-                count = n * self.g1l[i]
-                part = torch.zeros(self.ops.bn_fwd_partials(n, self.g1c[i], self.g1l[i]), dtype=torch.float64, device=mean.device)
-                slices = part.view(self.g1c[i], -1, 2)
-                slices[:, 0, 0], slices[:, 0, 1] = mean * count, (var + mean * mean) * count
-                parts.append((part, self.Bf[k + ".running_mean"].clone(), self.Bf[k + ".running_var"].clone()))
-            self._parts[n] = parts
+            self._parts[n] = [None] + [torch.zeros(self.ops.bn_fwd_partials(n, self.g1c[i], self.g1l[i]), dtype=torch.float64,
+                                                   device=self.bias0.device) for i in range(1, self.n + 1)]
+            self._fill_sums(n)
         return self._parts[n]
+
+    def _fill_sums(self, n: int) -> None:
+        for i in range(1, self.n + 1):
+            mean, var = (t.double() for t in self.norm1[i][2:])
+            count, slices = n * self.g1l[i], self._parts[n][i].view(self.g1c[i], -1, 2)
+            slices[:, 0, 0], slices[:, 0, 1] = mean * count, (var + mean * mean) * count
 
     @torch.no_grad()
     def draw(self, z: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -97,7 +108,7 @@ class Sampler8:
         n = z.shape[0]
         if n > self.batch or z.numel() != n * self.latent:
             raise PganError(f"draw: z {tuple(z.shape)} is not at most {self.batch} rows of {self.latent}")
-        o, P, c, h = self.ops, self.P, self.g2c, self.g2h
+        o, c, h = self.ops, self.g2c, self.g2h
         if n == 0:
             return self.sites[:0].view(0, 1, self.data, self.data), self.pos[:0]
         z = z.detach().reshape(n, self.latent).to(torch.float32).contiguous()
@@ -115,15 +126,12 @@ class Sampler8:
                 o.up_fold(y, None, self.sites[:n], self.act_id)
         # positions
         parts = self._running_sums(n)
-        o.gemm_nn(z, P["oned_conv_layers.0.weight"].detach().view(self.latent, -1), self.hA[1][:n].view(n, -1))
+        o.gemm_nn(z, self.w1[0].view(self.latent, -1), self.hA[1][:n].view(n, -1))
         for i in range(1, self.n + 1):
-            k = f"oned_conv_layers.{3 * (i - 1) + 1}"
-            part, rm, rv = parts[i]
-            o.bn_fwd_apply(self.hA[i][:n], P[k + ".weight"].detach(), P[k + ".bias"].detach(), rm, rv, self.hH[i][:n], self.stats[i],
-                           part, 1, momentum=0.0)
-            w = P[f"oned_conv_layers.{3 * i}.weight"].detach()
+            gain, bias, mean, var = self.norm1[i]        # (momentum 0: the statistics stay)
+            o.bn_fwd_apply(self.hA[i][:n], gain, bias, mean, var, self.hH[i][:n], self.stats[i], parts[i], 1, momentum=0.0)
             if i < self.n:
-                o.convt1d_up(self.hH[i][:n], w, self.hA[i + 1][:n])
+                o.convt1d_up(self.hH[i][:n], self.w1[i], self.hA[i + 1][:n])
             else:
-                o.convt1d_up(self.hH[i][:n], w, self.pos[:n], self.act_id)
+                o.convt1d_up(self.hH[i][:n], self.w1[i], self.pos[:n], self.act_id)
         return self.sites[:n].view(n, 1, self.data, self.data), self.pos[:n]

@@ -113,6 +113,13 @@ def test_optimizer_takes_torchs_state_and_refuses_what_it_cannot_do():
         sd = ref.state_dict()
         sd["param_groups"][0]["state_bits"] = 8
         eight.load_state_dict(sd)
+    had = snapshot(opt, [p])[0]
+    with pytest.raises(ValueError):
+        sd = ref.state_dict()
+        del sd["state"][0]["exp_avg_sq"]
+        opt.load_state_dict(sd)
+    has = snapshot(opt, [p])[0]                      # as it was
+    assert torch.equal(has[1], had[1]) and torch.equal(has[2], had[2]) and has[3] == had[3] == 3
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16)):
         with pytest.raises(ValueError):
             AdamW([p], **bad)
@@ -486,13 +493,15 @@ def test_optimizer_follows_its_parameters_and_counter():
     opt = AdamW([p], capturable=True)
     p.grad = torch.ones_like(p)
     opt.step()
-    opt.load_state_dict(opt.state_dict())            # its counter on the device is made by the next eager step
+    late = AdamW([p], weight_decay=0.0)
+    late.step()
+    late.param_groups[0]["capturable"] = True        # the counter on the device is made by the next eager step
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="before the capture"):
         with torch.cuda.graph(graph):
-            opt.step()
-    opt.step()
-    assert int(opt.param_groups[0]["counter"][0]) == 2
+            late.step()
+    late.step()
+    assert int(late.param_groups[0]["counter"][0]) == 2
     p.data = p.data.t()                              # the same memory in another order
     p.grad = torch.ones_like(p)
     with pytest.raises(PganError):
@@ -521,3 +530,95 @@ def test_draw_slab_needs_its_folder(tmp_path):
     import train_wgan_v2
     with pytest.raises(SystemExit, match="no folder"):
         train_wgan_v2.main(["--use_cuda", "--idir", str(tmp_path), "--odir", str(tmp_path), "--draw_n", "4", "--draw_slab", str(tmp_path / "none" / "x.slab")])
+
+
+@pytest.mark.gpu
+def test_a_captured_draw_follows_refresh():
+    """Weights and statistics change under a sampler: draws stay those of the last refresh(), a captured one's replays too."""
+    from pgan_hip import HipOps
+    from pgan_sampler import Sampler8
+    P, Bf = generator(21)
+    s = Sampler8(HipOps(DEV, max_samples=8), P, Bf, 8)
+    z = torch.randn(4, 128, device=DEV)
+    first = [t.clone() for t in s.draw(z)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.draw(z)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    for t in list(P.values()) + [v for k, v in Bf.items() if "running" in k]:
+        t.mul_(1 + 0.2 * torch.rand(t.shape, device=DEV, generator=gen))
+    assert all(torch.equal(a, b) for a, b in zip(s.draw(z), first))
+    graph.replay()
+    assert torch.equal(s.pos[:4], first[1])
+    s.refresh()
+    keep = [torch.full((1 << 16,), float("nan"), device=DEV) for _ in range(64)]      # what a freed buffer would hold
+    for _ in range(3):
+        s.draw(torch.zeros_like(z))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = s.sites[:4].clone(), s.pos[:4].clone()
+        want = s.draw(z)
+        assert torch.equal(got[0].view(4, 1, 64, 64), want[0]) and torch.equal(got[1], want[1])
+        assert not torch.equal(want[0], first[0]) and not torch.equal(want[1], first[1])
+    near(want[0], *eval64(P, Bf, z, s.n, "twod", "sigmoid"))
+    pos, _ = eval64(P, Bf, z, s.n, "oned", "sigmoid")
+    assert float((want[1].double().cpu() - pos).abs().max()) < 1e-4
+    del keep
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_trainer_in_a_graph_takes_the_eager_steps(bits):
+    a, b = make_trainer(optimizer="adamw", state_bits=bits), make_trainer(optimizer="adamw", state_bits=bits)
+    b.capture()                                      # makes one iteration
+    a.iteration()
+    for _ in range(3):
+        a.iteration()
+        b.replay()
+    torch.cuda.synchronize()
+    for x, y in ((a.eng.D, b.eng.D), (a.eng.G, b.eng.G)):
+        assert torch.equal(x.flat, y.flat) and torch.equal(x.adamw[4], y.adamw[4])
+        for n in x.p:
+            assert torch.equal(x.m[n].view(torch.uint8), y.m[n].view(torch.uint8))
+            assert torch.equal(x.v[n].view(torch.uint8), y.v[n].view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_follows_load_state_dict(bits):
+    from pgan_optim import AdamW
+    torch.manual_seed(4)
+    start = torch.randn(700, device=DEV)
+    grads = [torch.randn(700, device=DEV) for _ in range(6)]
+
+    def run(captured):
+        p = torch.nn.Parameter(start.clone())
+        p.grad = torch.zeros_like(p)
+        opt = AdamW([p], lr=1e-2, betas=(B1, B2), eps=EPS, state_bits=bits, seed=3, capturable=True)
+
+        def step(g, how):
+            p.grad.copy_(g)
+            how()
+        step(grads[0], opt.step)
+        step(grads[1], opt.step)
+        saved, at = copy.deepcopy(opt.state_dict()), p.detach().clone()
+        how = opt.step
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+            how = graph.replay
+        step(grads[2], how)
+        step(grads[3], how)
+        mid = p.detach().clone()
+        p.data.copy_(at)
+        opt.load_state_dict(saved)
+        junk = [torch.full((700,), float("nan"), device=DEV) for _ in range(16)]
+        step(grads[4], how)
+        step(grads[5], how)
+        torch.cuda.synchronize()
+        del junk
+        assert opt.state_dict()["state"][0]["step"] == 4
+        return [mid, p.detach().clone()] + [t.view(torch.uint8) for k, t in opt.state[p].items() if k != "step"]
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)

@@ -110,6 +110,7 @@ class AdamW(torch.optim.Optimizer):
                 with torch.cuda.device(members[0].device):
                     plan.step(grads, made + 1, float(group["lr"]), group["betas"][0], group["betas"][1], group["eps"],
                               group["weight_decay"], seed=group["seed"] + gi, step_dev=counter)
+                torch.autograd.graph.increment_version(members)      # a backward pass that saved them says so
                 if counter is None:
                     for p in members:
                         self.state[p]["step"] = made + 1

@@ -622,3 +622,15 @@ def test_a_captured_step_follows_load_state_dict(bits):
         return [mid, p.detach().clone()] + [t.view(torch.uint8) for k, t in opt.state[p].items() if k != "step"]
     for a, b in zip(run(False), run(True)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_over_stepped_weights_is_refused():
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.randn(30, device=DEV))
+    opt = AdamW([p])
+    loss = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

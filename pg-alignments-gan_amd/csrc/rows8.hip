@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
             };
             if (whole) {
 #pragma unroll
-                for (int r = 0; r < 32 * JO; r += 64 / LANES) *reinterpret_cast<i32x4*>(to + r * a.ldy) = piece(r);
+                for (int r = 0; r < 32 * JO; r += 64 / LANES) __builtin_nontemporal_store(piece(r), reinterpret_cast<i32x4*>(to + r * a.ldy));
             } else {
                 for (int r = 0; r < 32 * JO; r += 64 / LANES)
                     if (tr + r + lane / LANES < trows) put16(to + r * a.ldy, piece(r), nrows - wc0 - lane % LANES * PER, a.align);

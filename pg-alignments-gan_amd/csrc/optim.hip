@@ -15,8 +15,8 @@
 //
 // One launch for all tensors, as most of a network's are tiny: a block takes 2048 elements of one of them (a wave two blocks
 // of 256 with 8-bit states, the second's reads under way while the first is computed).  Bound by HBM: 28 bytes an element
-// with fp32 states (36 M elements: 191 us, 5.25 TB/s; a copy makes 4.86), 10 in bf16 with 8-bit ones (46 M elements: 98 us,
-// 4.7 TB/s, hash and codes take almost as long), 26 tensors of 2.8 M elements 13 us.
+// with fp32 states (36 M elements: 172 us, 5.8 TB/s; a copy makes 4.86), 10 in bf16 with 8-bit ones (46 M elements: 94 us,
+// 4.9 TB/s, hash and codes take almost as long), 26 tensors of 2.8 M elements 13 us.
 #include <algorithm>
 #include <vector>
 
@@ -73,14 +73,27 @@ __device__ __forceinline__ uint16_t to16(float x, int type) {
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <bool NT, class V>
+__device__ __forceinline__ V get(const void* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(static_cast<const V*>(p));
+    else return *static_cast<const V*>(p);
+}
+template <bool NT, class V>
+__device__ __forceinline__ void put(void* p, V v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, static_cast<V*>(p));
+    else *static_cast<V*>(p) = v;
+}
+
 // Four elements of a tensor: o (a lane's) past b, which is the same for the whole wave and stays in scalar registers.  VEC: one
 // access, else those below n one by one.
-template <int TYPE, bool VEC>
+template <int TYPE, bool VEC, bool NT>
 __device__ __forceinline__ void load4(const void* src, long long b, int o, long long n, float (&v)[4]) {
     if constexpr (TYPE == 0) {
         const float* s = static_cast<const float*>(src) + b;
         if constexpr (VEC) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(s + o);
+            const f32x4 x = get<NT, f32x4>(s + o);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = x[e];
         } else {
@@ -90,7 +103,7 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
     } else {
         const uint16_t* s = static_cast<const uint16_t*>(src) + b;
         if constexpr (VEC) {
-            const uint2 x = *reinterpret_cast<const uint2*>(s + o);
+            const u32x2 x = get<NT, u32x2>(s + o);
             if constexpr (TYPE == 1) {
                 v[0] = __builtin_bit_cast(float, x.x << 16);
                 v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
@@ -108,12 +121,12 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
         }
     }
 }
-template <int TYPE, bool VEC>
+template <int TYPE, bool VEC, bool NT>
 __device__ __forceinline__ void store4(void* dst, long long b, int o, long long n, const float (&v)[4]) {
     if constexpr (TYPE == 0) {
         float* d = static_cast<float*>(dst) + b;
         if constexpr (VEC) {
-            *reinterpret_cast<f32x4*>(d + o) = f32x4{v[0], v[1], v[2], v[3]};
+            put<NT>(d + o, f32x4{v[0], v[1], v[2], v[3]});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -124,8 +137,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
         if constexpr (VEC) {
             using H = std::conditional_t<TYPE == 1, __bf16, _Float16>;
             typedef H h2 __attribute__((ext_vector_type(2)));
-            *reinterpret_cast<uint2*>(d + o) =
-                uint2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})};
+            put<NT>(d + o, u32x2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -133,21 +145,21 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
         }
     }
 }
-template <bool VEC>
+template <bool VEC, bool NT>
 __device__ __forceinline__ uint32_t load_codes(const void* src, long long b, int o, long long n) {
     const uint8_t* s = static_cast<const uint8_t*>(src) + b;
-    if constexpr (VEC) return *reinterpret_cast<const uint32_t*>(s + o);
+    if constexpr (VEC) return get<NT, uint32_t>(s + o);
     uint32_t u = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (b + o + e < n) u |= (uint32_t)s[o + e] << (8 * e);
     return u;
 }
-template <bool VEC>
+template <bool VEC, bool NT>
 __device__ __forceinline__ void store_codes(void* dst, long long b, int o, long long n, uint32_t u) {
     uint8_t* d = static_cast<uint8_t*>(dst) + b;
     if constexpr (VEC) {
-        *reinterpret_cast<uint32_t*>(d + o) = u;
+        put<NT>(d + o, u);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -190,18 +202,18 @@ __device__ __forceinline__ void update(const AwStep& s, float& p, float g, float
     p = __builtin_fmaf(-(m * s.size), __builtin_amdgcn_rcpf(__builtin_fmaf(root, s.inv2, s.eps)), p * s.keep);
 }
 
-template <int PT, int GT, bool VEC>
+template <int PT, int GT, bool VEC, bool NT>
 __device__ __forceinline__ void body32(const AwTensor& t, const AwStep& s, long long b, int o) {
     float p[4], g[4], m[4], v[4], root;
-    load4<PT, VEC>(t.p, b, o, t.n, p);
-    load4<GT, VEC>(t.g, b, o, t.n, g);
-    load4<0, VEC>(t.m, b, o, t.n, m);
-    load4<0, VEC>(t.v, b, o, t.n, v);
+    load4<PT, VEC, NT>(t.p, b, o, t.n, p);
+    load4<GT, VEC, NT>(t.g, b, o, t.n, g);
+    load4<0, VEC, NT>(t.m, b, o, t.n, m);
+    load4<0, VEC, NT>(t.v, b, o, t.n, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) update(s, p[e], g[e], m[e], v[e], root);
-    store4<PT, VEC>(t.p, b, o, t.n, p);
-    store4<0, VEC>(t.m, b, o, t.n, m);
-    store4<0, VEC>(t.v, b, o, t.n, v);
+    store4<PT, VEC, NT>(t.p, b, o, t.n, p);
+    store4<0, VEC, NT>(t.m, b, o, t.n, m);
+    store4<0, VEC, NT>(t.v, b, o, t.n, v);
 }
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
@@ -215,15 +227,15 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 }
 
 // one block of 256 elements by one wave, four elements a lane from i on
-template <int PT, int GT, bool VEC>
+template <int PT, int GT, bool VEC, bool NT>
 struct Block8 {
     float p[4], g[4], ms, rs;
     uint32_t cm, cv;
     __device__ __forceinline__ void load(const AwTensor& t, long long i, int o) {
-        load4<PT, VEC>(t.p, i, o, t.n, p);
-        load4<GT, VEC>(t.g, i, o, t.n, g);
-        cm = load_codes<VEC>(t.m, i, o, t.n);
-        cv = load_codes<VEC>(t.v, i, o, t.n);
+        load4<PT, VEC, NT>(t.p, i, o, t.n, p);
+        load4<GT, VEC, NT>(t.g, i, o, t.n, g);
+        cm = load_codes<VEC, NT>(t.m, i, o, t.n);
+        cv = load_codes<VEC, NT>(t.v, i, o, t.n);
         ms = t.ms[i / AW_BLOCK];
         rs = t.rs[i / AW_BLOCK];
     }
@@ -246,7 +258,7 @@ struct Block8 {
             mmax = max(mmax, __builtin_bit_cast(uint32_t, m[e]) & 0x7fffffffu);
             vmax = max(vmax, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
         }
-        store4<PT, VEC>(t.p, i, o, t.n, p);
+        store4<PT, VEC, NT>(t.p, i, o, t.n, p);
         mmax = wave_max(mmax);
         vmax = wave_max(vmax);
         const bool odd = __builtin_amdgcn_readfirstlane(max(mmax, vmax)) >= 0x7f800000;
@@ -280,8 +292,8 @@ struct Block8 {
             nm |= (a | ((__builtin_bit_cast(uint32_t, m[e]) >> 24) & 0x80u)) << (8 * e);
             nr |= b << (8 * e);
         }
-        store_codes<VEC>(t.m, i, o, t.n, nm);
-        store_codes<VEC>(t.v, i, o, t.n, nr);
+        store_codes<VEC, NT>(t.m, i, o, t.n, nm);
+        store_codes<VEC, NT>(t.v, i, o, t.n, nr);
         if ((threadIdx.x & 63) == 0) {
             t.ms[i / AW_BLOCK] = pow2(em);
             t.rs[i / AW_BLOCK] = pow2(er);
@@ -289,7 +301,7 @@ struct Block8 {
     }
 };
 
-template <int BITS, int PT, int GT>
+template <int BITS, bool NT, int PT, int GT>
 __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long long at, bool vec, uint32_t key) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (BITS == 32) {
@@ -297,16 +309,16 @@ __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long l
         for (int u = 0; u < AW_CHUNK / 1024; ++u) {
             const long long b = at + u * 1024 + wave * 256;
             if (vec && b + 256 <= t.n) {
-                body32<PT, GT, true>(t, s, b, lane * 4);
+                body32<PT, GT, true, NT>(t, s, b, lane * 4);
             } else if (b + lane * 4 < t.n) {
-                body32<PT, GT, false>(t, s, b, lane * 4);
+                body32<PT, GT, false, NT>(t, s, b, lane * 4);
             }
         }
     } else {
         // two blocks of 256 a wave, the second one's reads under way while the first is computed
         const long long b = at + wave * (2 * AW_BLOCK);
         if (vec && b + 2 * AW_BLOCK <= t.n) {
-            Block8<PT, GT, true> x, y;
+            Block8<PT, GT, true, NT> x, y;
             x.load(t, b, lane * 4);
             y.load(t, b + AW_BLOCK, lane * 4);
             x.step(t, s, b, lane * 4, key);
@@ -315,7 +327,7 @@ __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long l
             for (int u = 0; u < 2; ++u) {
                 const long long i = b + u * AW_BLOCK;
                 if (i >= t.n) break;
-                Block8<PT, GT, false> x;
+                Block8<PT, GT, false, NT> x;
                 x.load(t, i, lane * 4);
                 x.step(t, s, i, lane * 4, key);
             }
@@ -323,7 +335,7 @@ __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long l
     }
 }
 
-template <int BITS>
+template <int BITS, bool NT>
 __global__ __launch_bounds__(256) void adamw_kernel(const AwArgs a) {
     // the block's tensor: the lanes compare it with every tensor's first chunk at once
     const int lane = threadIdx.x & 63;
@@ -341,15 +353,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwArgs a) {
     const uint32_t key = BITS == 8 ? mix(a.seed + step * 0xA54FF53Bu + (uint32_t)t.index * 0x3C6EF373u) : 0u;
     const bool vec = t.types >= 16;
     switch (t.types & 15) {
-        case 0: chunk<BITS, 0, 0>(t, s, at, vec, key); break;
-        case 1: chunk<BITS, 1, 0>(t, s, at, vec, key); break;
-        case 2: chunk<BITS, 2, 0>(t, s, at, vec, key); break;
-        case 3: chunk<BITS, 0, 1>(t, s, at, vec, key); break;
-        case 4: chunk<BITS, 1, 1>(t, s, at, vec, key); break;
-        case 5: chunk<BITS, 2, 1>(t, s, at, vec, key); break;
-        case 6: chunk<BITS, 0, 2>(t, s, at, vec, key); break;
-        case 7: chunk<BITS, 1, 2>(t, s, at, vec, key); break;
-        default: chunk<BITS, 2, 2>(t, s, at, vec, key); break;
+        case 0: chunk<BITS, NT, 0, 0>(t, s, at, vec, key); break;
+        case 1: chunk<BITS, NT, 1, 0>(t, s, at, vec, key); break;
+        case 2: chunk<BITS, NT, 2, 0>(t, s, at, vec, key); break;
+        case 3: chunk<BITS, NT, 0, 1>(t, s, at, vec, key); break;
+        case 4: chunk<BITS, NT, 1, 1>(t, s, at, vec, key); break;
+        case 5: chunk<BITS, NT, 2, 1>(t, s, at, vec, key); break;
+        case 6: chunk<BITS, NT, 0, 2>(t, s, at, vec, key); break;
+        case 7: chunk<BITS, NT, 1, 2>(t, s, at, vec, key); break;
+        default: chunk<BITS, NT, 2, 2>(t, s, at, vec, key); break;
     }
 }
 
@@ -380,6 +392,7 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
     if (n > 0 && (!p || !g || !m || !v || !numel || !types || !lr || !decay)) return PGAN_EINVAL;
     if (bits == 8 && n > 0 && (!m_scale || !r_scale)) return PGAN_EINVAL;
     const int size_of[3] = {4, 2, 2};
+    long long bytes = 0;
     try {
         // what is written: no two of these may share memory (the same tensor twice in the lists, a state for two of them)
         std::vector<Span> out, in;
@@ -396,6 +409,7 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
             const int ps = size_of[types[i] % 3], gsz = size_of[types[i] / 3];
             if (!aligned(p[i], ps) || !aligned(g[i], gsz)) return PGAN_EINVAL;
             if (bits == 32 && (!aligned(m[i], 4) || !aligned(v[i], 4))) return PGAN_EINVAL;
+            bytes += numel[i] * (2 * ps + gsz + bits / 2);
             add(in, g[i], numel[i] * gsz);
             add(out, p[i], numel[i] * ps);
             add(out, m[i], numel[i] * (bits / 8));
@@ -418,6 +432,13 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
     } catch (...) {
         return PGAN_EINVAL;
     }
+    // Steps of more than one and a half times the memory-side cache go past the caches: what passes between two steps leaves
+    // little of them there.  us with ordinary accesses and past the caches, after 1 GB of other writes: 240 MB 58 and 46 (fp32,
+    // 32 bits), 63 and 46 (fp32, 8), 64 and 54 (bf16, 8); 450 MB 102 and 81, 105 and 79, 107 and 92; step after step with
+    // nothing between: 240 MB 37 and 41, 40 and 42, 49 and 50; 450 MB 67 and 77, 72 and 76, 94 and 90; 1200 MB 232 and 218, 222
+    // and 192, 246 and 241.  Smaller steps do not: an iteration of the trainer (78 MB a step, the weights read again at once)
+    // takes 6.17 ms and 6.18.
+    const bool past = bytes > (384LL << 20);
     if (step_dev) adamw_tick_kernel<<<1, 1, 0, st>>>(step_dev, b1, b2);
     AwArgs a;
     a.step_dev = step_dev;
@@ -449,8 +470,8 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
             ++a.n;
         }
         if (a.n == 0) break;
-        if (bits == 32) adamw_kernel<32><<<(unsigned)chunks, 256, 0, st>>>(a);
-        else adamw_kernel<8><<<(unsigned)chunks, 256, 0, st>>>(a);
+        auto* const kernel = bits == 32 ? (past ? adamw_kernel<32, true> : adamw_kernel<32, false>) : past ? adamw_kernel<8, true> : adamw_kernel<8, false>;
+        kernel<<<(unsigned)chunks, 256, 0, st>>>(a);
     }
     return pgan_launch_status();
 }

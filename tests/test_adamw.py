@@ -463,3 +463,49 @@ def test_elements_past_31_bits(hip, monkeypatch):
         assert torch.equal(ms[lo // BLOCK:-(-hi // BLOCK)].cpu(), sm) and torch.equal(rs[lo // BLOCK:-(-hi // BLOCK)].cpu(), sr)
     monkeypatch.undo()
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,pt,gt,n", [(32, "float32", "float32", 20_000_003), (8, "float32", "bfloat16", 40_000_001), (8, "bfloat16", "bfloat16", 60_000_003),
+                                          (32, "float16", "float32", 26_000_000)])
+def test_steps_past_the_caches_equal_small_ones(hip, bits, pt, gt, n):
+    """A step of more than 384 MB reads and writes past the caches: bit for bit what its tensors' steps give in two parts.  (A
+    tensor's random bits depend on its number in the list and the place in it: the parts keep both.)"""
+    pt, gt = getattr(torch, pt), getattr(torch, gt)
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    rnd = lambda n, dt, s: torch.randn(n, device=DEV, generator=gen).mul_(s).to(dt)
+    sizes = [n, 5000, 255]
+
+    def held(k):
+        if bits == 32:
+            return [torch.zeros(k, device=DEV), torch.zeros(k, device=DEV)], None
+        return ([torch.zeros(k, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)],
+                [torch.zeros(-(-k // BLOCK), device=DEV) for _ in range(2)])
+    p, g = [rnd(k, pt, 0.1) for k in sizes], [rnd(k, gt, 1e-2) for k in sizes]
+    whole, st = [t.clone() for t in p], [held(k) for k in sizes]
+    for t in (1, 2):
+        hip.adamw(whole, g, [s[0][0] for s in st], [s[0][1] for s in st], t, 1e-3, B1, B2, EPS, 0.01, seed=9,
+                  scales=None if bits == 32 else ([s[1][0] for s in st], [s[1][1] for s in st]))
+    half = n // 2 // 2048 * 2048
+    # the same tensor's first part alone, in a list in which it has the same number and place
+    part, sp = p[0][:half].clone(), held(half)
+    for t in (1, 2):
+        hip.adamw([part], [g[0][:half]], [sp[0][0]], [sp[0][1]], t, 1e-3, B1, B2, EPS, 0.01, seed=9,
+                  scales=None if bits == 32 else ([sp[1][0]], [sp[1][1]]))
+    raw = lambda t: t.view(torch.uint8)
+    assert torch.equal(raw(whole[0][:half]), raw(part))
+    assert all(torch.equal(raw(a[:half]), raw(b)) for a, b in zip(st[0][0], sp[0]))
+    if bits == 8:
+        assert all(torch.equal(a[:half // BLOCK], b) for a, b in zip(st[0][1], sp[1]))
+    # its end against the definition (32 bits: no random bits in it)
+    if bits == 32:
+        e = slice(n - 5000, n)
+        m = v = torch.zeros(5000)
+        q = p[0][e].cpu()
+        for t in (1, 2):
+            want, _, _, _, tol = step64(q, g[0][e].cpu(), m, v, t, 1e-3, 0.01)
+            m, v = states32(m, v, g[0][e].cpu().float())
+            if t == 1:
+                q = want.float().to(pt)
+        within("m", st[0][0][0][e], m.double(), 4 * U * m.abs().double() + 1e-12)
+        within("p", whole[0][e], want, 2 * tol + 3 * half_step(want.abs() + tol, pt))

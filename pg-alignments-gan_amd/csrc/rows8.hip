@@ -88,20 +88,22 @@ __device__ __forceinline__ void no_row(float (&v)[N], float inv) {
 // LeakyReLU: of x and its tenth the larger
 __device__ __forceinline__ float slope(float x, bool lrelu) { return lrelu ? __builtin_fmaxf(x, x * PGAN_SLOPE) : x; }
 
-// eight elements from p on, which lies on a multiple of 4 bytes
-template <int TYPE>
+// eight elements from p on, which lies on a multiple of 4 bytes; NT: read once, past the caches
+template <int TYPE, bool NT = false>
 __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float (&v)[8]) {
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
     if constexpr (TYPE == 0) {
-        const f32x4 a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
+        const f32x4u* x = reinterpret_cast<const f32x4u*>(p);
+        const f32x4 a = NT ? __builtin_nontemporal_load(x) : x[0], b = NT ? __builtin_nontemporal_load(x + 1) : x[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v[e] = a[e];
             v[4 + e] = b[e];
         }
     } else {
-        const i32x4 a = *reinterpret_cast<const i32x4u*>(p);
+        const i32x4u* x = reinterpret_cast<const i32x4u*>(p);
+        const i32x4 a = NT ? __builtin_nontemporal_load(x) : *x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (TYPE == 1) {
@@ -735,7 +737,8 @@ struct FoldArgs {
 
 // 2^log lanes an output pixel, eight channels each: neighbouring ones (VEC: every tap and row of results on a 16-byte
 // border), else every 2^log-th.  Every input value goes to exactly one output: nothing is read twice.  Bound by HBM
-// (codes of 1000 x 16 x 16 x 64: 594 MB in 109 us, 5.4 TB/s).
+// (codes of 1000 x 16 x 16 x 64: 594 MB in 108 us, 5.5 TB/s; the codes past the caches too: 104, but the next product then
+// waits for them, a thousand alignments drawn 600 us for 590).
 template <int TYPE, bool VEC, bool Q8>
 __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned pix = blockIdx.x * (256u >> a.log) + (threadIdx.x >> a.log);
@@ -752,7 +755,7 @@ __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>:
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) p[i][j][e] = 0.f;
-                if (c < C && t.at[i][j] >= 0) load8<TYPE>(y + t.at[i][j] + c, p[i][j]);
+                if (c < C && t.at[i][j] >= 0) load8<TYPE, true>(y + t.at[i][j] + c, p[i][j]);
             }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sh[e] = a.shift && c < C ? a.shift[c + e] : 0.f;

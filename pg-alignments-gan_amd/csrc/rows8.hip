@@ -262,10 +262,11 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
 // A wave waits for its own reads of a stage by their count and meets the others at a barrier, once a stage; the operands of
 // a step of 32 are read from LDS between the products of the step before.
 // Bound by the matrix instructions and the power they draw where K is long (8192 x 8192 x 8192: 458 us, 2400 Top/s, the
-// rate of the library's product; 4096 x 4096 x 4096: 67 us, 2040 Top/s), by the results' way out where it is short (256000 x
-// 128 x 1024: 115 us, 4.8 TB/s).  With stages that went through registers into one place of LDS 4096 x 4096 x 4096 took 77
+// rate of the library's product; 4096 x 4096 x 4096: 64 us, 2150 Top/s), by the results' way out where it is short (256000 x
+// 128 x 1024: 95 us, 5.9 TB/s).  With stages that went through registers into one place of LDS 4096 x 4096 x 4096 took 77
 // us and 2048 x 2048 x 2048 21 for 14; with all of a step's LDS reads before its products, and so the next stage's reads
-// from memory waited for at once, 74 and 15.
+// from memory waited for at once, 74 and 15; with results that stay in the caches 16000 x 512 x 4096 61 for 50 and
+// 256000 x 128 x 1024 115 for 95: the kernel ends when they have left.
 __device__ __forceinline__ i32x4 below(i32x4 v, int left) {        // the first `left` of 16 bytes, zero behind them
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -1052,19 +1053,21 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
         // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
         // behind another's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight waves, one block
-        // a CU), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
-        //   4096 x 4096 x 4096     64   86   84    -       16000 x 512 x 4096     66   61   75   85
-        //   3000 x 4000 x 3000     52   66   65   77       64000 x 256 x 2048     98   84  107  113
-        //   2000 x 8000 x 2000     81   64   51   65      256000 x 128 x 1024    147  118  187  257
-        //   5000 x 2048 x 2000     31   31   31   39        8000 x 1024 x 1024    17   15   17   20
-        //   2048 x 2048 x 2048     23   16   15   16         777 x 1001 x 1234    17    9    8    8
-        //   4000 x 1000 x 2000     22   18   19   21         600 x 2000 x 1000    24   14    9    8
+        // a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
+        //   4096 x 4096 x 4096     64   77   86   84    -      16000 x 512 x 4096     57   50   52   62   83
+        //   4096 x 2048 x 4096     36   40   45   45   58       4000 x 512 x 4096     17   14   15   19   23
+        //   3000 x 4000 x 3000     52   71   66   65   77      64000 x 256 x 2048     80   70   66   85  116
+        //   5000 x 2048 x 2000     29   33   30   30   39    256000 x 128 x 1024     122  108   95  130  175
+        //   2000 x 8000 x 2000     81   60   64   51   65      8000 x 1024 x 1024     16   17   13   16   19
+        //   2048 x 2048 x 2048     23   18   16   15   17       777 x 1001 x 1234     17   10    9    8    8
+        //   4000 x 1000 x 2000     20   17   18   19   21       600 x 2000 x 1000     24   17   14    9    8
         // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
         // shares K among the waves of a block of 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0,
         // 64 x 4096 x 1024 7.6 against 14.9, but 777 x 1001 x 1234 10 against 8.
         if (T <= FEW || tiles(64, 64) <= 128) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
         else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
         else if (K >= 1024 && tiles(256, 256) >= (K < 2048 ? 256 : 144)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
+        else if (K >= 512 && tiles(128, 256) >= 512) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
         else if (tiles(128, 128) >= 448) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
         else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
         else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);

@@ -20,6 +20,12 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+// Global memory takes wide accesses on any border; these say so.
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef int i32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef int i32x2_1 __attribute__((ext_vector_type(2), aligned(1)));
 
 template <int TYPE>
 struct Elem {
@@ -88,13 +94,11 @@ __device__ __forceinline__ void no_row(float (&v)[N], float inv) {
 // LeakyReLU: of x and its tenth the larger
 __device__ __forceinline__ float slope(float x, bool lrelu) { return lrelu ? __builtin_fmaxf(x, x * PGAN_SLOPE) : x; }
 
-// eight elements from p on, which lies on a multiple of 4 bytes; NT: read once, past the caches
+// eight elements from p on; NT: read once, past the caches
 template <int TYPE, bool NT = false>
 __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float (&v)[8]) {
-    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-    typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
     if constexpr (TYPE == 0) {
-        const f32x4u* x = reinterpret_cast<const f32x4u*>(p);
+        const f32x4_4* x = reinterpret_cast<const f32x4_4*>(p);
         const f32x4 a = NT ? __builtin_nontemporal_load(x) : x[0], b = NT ? __builtin_nontemporal_load(x + 1) : x[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -102,7 +106,7 @@ __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float 
             v[4 + e] = b[e];
         }
     } else {
-        const i32x4u* x = reinterpret_cast<const i32x4u*>(p);
+        const i32x4_2* x = reinterpret_cast<const i32x4_2*>(p);
         const i32x4 a = NT ? __builtin_nontemporal_load(x) : *x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -116,12 +120,22 @@ __device__ __forceinline__ void load8(const typename Elem<TYPE>::type* p, float 
         }
     }
 }
+// as load8 of fewer than eight elements in a row, zeros behind them
+template <int TYPE>
+__device__ __forceinline__ void load_few(const typename Elem<TYPE>::type* p, int n, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? to_f32<TYPE>(p[e]) : 0.f;
+}
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[8], float inv) {
+    *reinterpret_cast<i32x2_1*>(p) = i32x2_1{(int)four_codes(v[0], v[1], v[2], v[3], inv), (int)four_codes(v[4], v[5], v[6], v[7], inv)};
+}
+
 // ---- rows to codes ------------------------------------------------------------------------------------------------
 // 2^log lanes a row, whose values stay in their registers between the maximum and the codes: 8 NIT each, K <= 8 NIT 2^log; a
-// lane has R rows, to have more bytes on their way.  VEC: eight neighbouring elements at a time, in rows that start on
-// 4-byte borders (codes on 8); else every 2^log-th.  Bound by HBM (2 + 1 bytes an element of 16 bits;
-// 16000 x 512 from memory: 8.3 us, 3 TB/s, launch and one trip to memory half of it).
-template <int TYPE, bool VEC, int NIT, int R>
+// lane has R rows, to have more bytes on their way.  A lane takes eight neighbouring elements at a time, the one at the row's
+// end its last eight, some of them its neighbour's too.  Bound by HBM (2 + 1 bytes an element of 16 bits; 16000 x 512 from
+// memory: 8.3 us, 3 TB/s, launch and one trip to memory half of it).
+template <int TYPE, int NIT, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                          int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                                                          long long rows, int K, int lrelu, int log) {
@@ -134,24 +148,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYP
         const typename Elem<TYPE>::type* xr = x + (row0 + r < rows ? row0 + r : row0) * ldx;
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
-            if constexpr (VEC) {
-                const int k = ((it << log) + l) * 8;
+            const int k = ((it << log) + l) * 8;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[r][it][e] = 0.f;
-                if (k + 8 <= K) {
-                    load8<TYPE>(xr + k, v[r][it]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (k + e < K) v[r][it][e] = to_f32<TYPE>(xr[k + e]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int k = ((it * 8 + e) << log) + l;
-                    v[r][it][e] = k < K ? to_f32<TYPE>(xr[k]) : 0.f;
-                }
-            }
+            for (int e = 0; e < 8; ++e) v[r][it][e] = 0.f;
+            if (K < 8) load_few<TYPE>(xr, K, v[r][it]);
+            else if (k < K) load8<TYPE>(xr + min(k, K - 8), v[r][it]);
         }
     }
 #pragma unroll
@@ -171,32 +172,21 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYP
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
             no_row(v[r][it], rs.inv);
-            if constexpr (VEC) {
-                const int k = ((it << log) + l) * 8;
-                uint2 u;
-                u.x = four_codes(v[r][it][0], v[r][it][1], v[r][it][2], v[r][it][3], rs.inv);
-                u.y = four_codes(v[r][it][4], v[r][it][5], v[r][it][6], v[r][it][7], rs.inv);
-                if (k + 8 <= K) {
-                    *reinterpret_cast<uint2*>(qr + k) = u;
-                } else {
+            const int k = ((it << log) + l) * 8;
+            if (K < 8) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (k + e < K) qr[k + e] = (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3)));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int k = ((it * 8 + e) << log) + l;
-                    if (k < K) qr[k] = (int8_t)code_of(v[r][it][e], rs.inv);
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (e < K) qr[e] = (int8_t)code_of(v[r][it][e], rs.inv);
+            } else if (k < K) {
+                store_codes(qr + min(k, K - 8), v[r][it], rs.inv);
             }
         }
     }
 }
 
-// Longer rows: one a block.  NIT > 0: the values stay in registers, 8 NIT of a thread (K <= 2048 NIT, VEC); 0: rows are read
-// twice, the second time from the L1 or L2.  8192 x 8192 in bf16, from memory: 42.5 us, 4.7 TB/s (read twice: 49).
-template <int TYPE, bool VEC, int NIT>
+// Longer rows: one a block.  NIT > 0: the values stay in registers, 8 NIT of a thread (K <= 2048 NIT); 0: rows are read twice,
+// the second time from the L1 or L2.  8192 x 8192 in bf16, from memory: 42.5 us, 4.7 TB/s (read twice: 49).
+template <int TYPE, int NIT>
 __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                               int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                                                               long long rows, int K, int lrelu) {
@@ -204,7 +194,6 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
     const long long row = blockIdx.x;
     const typename Elem<TYPE>::type* xr = x + row * ldx;
     int8_t* qr = q + row * ldq;
-    const int whole = VEC ? K / 8 * 8 : 0;          // elements that are read eight at a time
     uint32_t mx = 0;
     const auto top = [&](float (&v)[8]) {
 #pragma unroll
@@ -217,41 +206,39 @@ __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Ele
     if constexpr (NIT > 0) {
 #pragma unroll
         for (int i = 0; i < NIT; ++i)
-            if (threadIdx.x * 8 + 2048 * i < whole) load8<TYPE>(xr + threadIdx.x * 8 + 2048 * i, kept[i]);
+            if (threadIdx.x * 8 + 2048 * i < K) load8<TYPE>(xr + min((int)threadIdx.x * 8 + 2048 * i, K - 8), kept[i]);
 #pragma unroll
         for (int i = 0; i < NIT; ++i)
-            if (threadIdx.x * 8 + 2048 * i < whole) top(kept[i]);
+            if (threadIdx.x * 8 + 2048 * i < K) top(kept[i]);
     } else {
-        for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+        for (int k = threadIdx.x * 8; k < K; k += 2048) {
             float v[8];
-            load8<TYPE>(xr + k, v);
+            load8<TYPE>(xr + min(k, K - 8), v);
             top(v);
         }
     }
-    for (int k = whole + threadIdx.x; k < K; k += 256) mx = max(mx, magnitude(slope(to_f32<TYPE>(xr[k]), lrelu)));
     mx = group_max(mx, 6);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = mx;
     __syncthreads();
     const RowScale rs = row_scale(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
     if (threadIdx.x == 0) scale[row] = rs.scale;
-    const auto put = [&](int k, float (&v)[8]) {
-        no_row(v, rs.inv);
-        *reinterpret_cast<uint2*>(qr + k) = uint2{four_codes(v[0], v[1], v[2], v[3], rs.inv), four_codes(v[4], v[5], v[6], v[7], rs.inv)};
-    };
     if constexpr (NIT > 0) {
 #pragma unroll
         for (int i = 0; i < NIT; ++i)
-            if (threadIdx.x * 8 + 2048 * i < whole) put(threadIdx.x * 8 + 2048 * i, kept[i]);
+            if (threadIdx.x * 8 + 2048 * i < K) {
+                no_row(kept[i], rs.inv);
+                store_codes(qr + min((int)threadIdx.x * 8 + 2048 * i, K - 8), kept[i], rs.inv);
+            }
     } else {
-        for (int k = threadIdx.x * 8; k < whole; k += 2048) {
+        for (int k = threadIdx.x * 8; k < K; k += 2048) {
             float v[8];
-            load8<TYPE>(xr + k, v);
+            load8<TYPE>(xr + min(k, K - 8), v);
+            no_row(v, rs.inv);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = slope(v[e], lrelu);
-            put(k, v);
+            store_codes(qr + min(k, K - 8), v, rs.inv);
         }
     }
-    for (int k = whole + threadIdx.x; k < K; k += 256) qr[k] = rs.inv == 0.f ? 0 : (int8_t)code_of(slope(to_f32<TYPE>(xr[k]), lrelu), rs.inv);
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
@@ -282,25 +269,13 @@ __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
     typedef H h2 __attribute__((ext_vector_type(2)));
     return uint2{__builtin_bit_cast(uint32_t, h2{(H)a, (H)b}), __builtin_bit_cast(uint32_t, h2{(H)c, (H)d})};
 }
-// 16 bytes of a row, of which `left` elements lie inside it; align: bytes that every row starts on a multiple of
+// 16 bytes of a row, of which `left` elements lie inside it
 template <class Y>
-__device__ __forceinline__ void put16(Y* to, i32x4 v, int left, int align) {
+__device__ __forceinline__ void put16(Y* to, i32x4 v, int left) {
     constexpr int PER = 16 / (int)sizeof(Y);
     if (left >= PER) {
-        if (align == 16) {
-            *reinterpret_cast<i32x4*>(to) = v;
-            return;
-        }
-        if (align == 8) {
-            reinterpret_cast<int2*>(to)[0] = int2{v[0], v[1]};
-            reinterpret_cast<int2*>(to)[1] = int2{v[2], v[3]};
-            return;
-        }
-        if (align == 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<int*>(to)[e] = v[e];
-            return;
-        }
+        *reinterpret_cast<i32x4_2*>(to) = v;
+        return;
     }
     const Y* h = reinterpret_cast<const Y*>(&v);
 #pragma unroll
@@ -325,7 +300,6 @@ struct GemmArgs {
     long long ldq, ldw, ldy, T;
     int N, K;
     unsigned tt, tn, band;      // tiles along the tokens and along the channels, channel tiles of a band
-    int align;                  // bytes (16, 8, 4, 2) that every row of y starts on a multiple of
 };
 
 // Tile of a block: blocks go round the eight dies, each of which gets a run of neighbouring tiles -- bands of eight channel
@@ -480,7 +454,7 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
     // channel (within 32): e % 4 + 8 (e / 4) + 4 (lane / 32); token: lane % 32
     char* own = mem + wave * 32 * JO * YROW;
     constexpr int PER = 16 / (int)sizeof(Y), LANES = 32 * FO / PER;      // channels and lanes of a 16-byte row stretch
-    const bool whole = trows == BT && nrows == BN && a.align == 16;
+    const bool whole = trows == BT && nrows == BN;
 #pragma unroll
     for (int io = 0; io < FN; io += FO) {
         const int wc0 = (wn * FN + io) * 32;
@@ -516,10 +490,10 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
             };
             if (whole) {
 #pragma unroll
-                for (int r = 0; r < 32 * JO; r += 64 / LANES) __builtin_nontemporal_store(piece(r), reinterpret_cast<i32x4*>(to + r * a.ldy));
+                for (int r = 0; r < 32 * JO; r += 64 / LANES) __builtin_nontemporal_store(i32x4_2(piece(r)), reinterpret_cast<i32x4_2*>(to + r * a.ldy));
             } else {
                 for (int r = 0; r < 32 * JO; r += 64 / LANES)
-                    if (tr + r + lane / LANES < trows) put16(to + r * a.ldy, piece(r), nrows - wc0 - lane % LANES * PER, a.align);
+                    if (tr + r + lane / LANES < trows) put16(to + r * a.ldy, piece(r), nrows - wc0 - lane % LANES * PER);
             }
             wave_sync();
         }
@@ -536,7 +510,7 @@ struct FewArgs {
     GemmArgs g;
     const void* x;
     long long ldx;
-    int lrelu, vec;         // vec: rows of x start on 4-byte borders
+    int lrelu, log;         // 2^log lanes make a row's codes, 512 elements at a time
 };
 template <int X, int WV, int RW, int TYPE>
 __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
@@ -584,22 +558,17 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
         uint32_t mx[RW];
 #pragma unroll
         for (int r = 0; r < RW; ++r) mx[r] = 0;
-        const auto part = [&](int k0) {     // 512 elements of each of the wave's rows
+        const int l8 = (lane & ((1 << f.log) - 1)) * 8;
+        const auto row_of = [&](int r) { return ((wave + WV * r) << (6 - f.log)) + (lane >> f.log); };
+        const auto part = [&](int k0) {     // up to 512 elements of each of the wave's rows, a row's last eight at its end
 #pragma unroll
             for (int r = 0; r < RW; ++r) {
-                const int row = wave + WV * r;
-                const XE* xr = x + (long long)row * f.ldx;
+                const XE* xr = x + (long long)row_of(r) * f.ldx;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
-                if (row >= T) continue;
-                const int k = k0 + lane * 8;
-                if (f.vec && k + 8 <= K) {
-                    load8<X < 0 ? 0 : X>(xr + k, v[r]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (k + e < K) v[r][e] = to_f32<X < 0 ? 0 : X>(xr[k + e]);
-                }
+                if (row_of(r) >= T || k0 + l8 >= K) continue;
+                if (K < 8) load_few<X < 0 ? 0 : X>(xr, K, v[r]);
+                else load8<X < 0 ? 0 : X>(xr + min(k0 + l8, K - 8), v[r]);
             }
 #pragma unroll
             for (int r = 0; r < RW; ++r)
@@ -616,20 +585,17 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
         float inv[RW];
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
-            if (wave + WV * r >= T) continue;
-            const RowScale rs = row_scale(group_max(mx[r], 6));
+            const RowScale rs = row_scale(group_max(mx[r], f.log));
             inv[r] = rs.inv;
-            if (lane == 0) scales[wave + WV * r] = rs.scale;
+            if (l8 == 0 && row_of(r) < T) scales[row_of(r)] = rs.scale;
         }
         for (int k0 = 0; k0 < K; k0 += 512) {
             if (K > 512) part(k0);
-            const int k = k0 + lane * 8;
 #pragma unroll
             for (int r = 0; r < RW; ++r)
-                if (wave + WV * r < T && k < K) {
+                if (row_of(r) < T && k0 + l8 < K) {
                     no_row(v[r], inv[r]);
-                    *reinterpret_cast<uint2*>(few + (wave + WV * r) * stride + k) =
-                        uint2{four_codes(v[r][0], v[r][1], v[r][2], v[r][3], inv[r]), four_codes(v[r][4], v[r][5], v[r][6], v[r][7], inv[r])};
+                    store_codes(reinterpret_cast<int8_t*>(few) + row_of(r) * stride + (K < 8 ? 0 : min(k0 + l8, K - 8)), v[r], inv[r]);
                 }
         }
     } else {
@@ -681,9 +647,9 @@ __global__ __launch_bounds__(64 * WV) void gemm_few_kernel(const FewArgs f) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)sum[e] * st, ws[e], bs[e]);
     Y* to = static_cast<Y*>(a.y) + (t0 + t) * a.ldy + ch;
-    if (a.align >= 4 * (int)sizeof(Y) && ch + 4 <= N) {
-        if constexpr (TYPE == 0) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-        else *reinterpret_cast<uint2*>(to) = pack4<TYPE>(v[0], v[1], v[2], v[3]);
+    if (ch + 4 <= N) {
+        if constexpr (TYPE == 0) *reinterpret_cast<f32x4_4*>(to) = f32x4_4{v[0], v[1], v[2], v[3]};
+        else *reinterpret_cast<i32x2_2*>(to) = __builtin_bit_cast(i32x2_2, pack4<TYPE>(v[0], v[1], v[2], v[3]));
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -714,11 +680,29 @@ __device__ __forceinline__ Taps taps_of(unsigned pix, int H, int W, int C) {
     t.at[1][1] = hok && wok ? ((rb + w2) * 16 + kb * 4 + lb) * C : -1;
     return t;
 }
+// of the eight channels from c on, or of the only n < 8
 template <int TYPE>
-__device__ __forceinline__ float folded(const typename Elem<TYPE>::type* y, const Taps& t, int c, const float* shift) {
-    const auto get = [&](int i, int j) { return t.at[i][j] < 0 ? 0.f : to_f32<TYPE>(y[t.at[i][j] + c]); };
-    const float o = (get(0, 0) + get(1, 0)) + (get(0, 1) + get(1, 1));
-    return shift ? o + shift[c] : o;
+__device__ __forceinline__ void fold8(const typename Elem<TYPE>::type* y, const Taps& t, int c, int n, const float* shift, float (&v)[8]) {
+    float p[2][2][8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[i][j][e] = 0.f;
+            if (t.at[i][j] < 0) continue;
+            if (n < 8) load_few<TYPE>(y + t.at[i][j], n, p[i][j]);
+            else load8<TYPE, true>(y + t.at[i][j] + c, p[i][j]);
+        }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (p[0][0][e] + p[1][0][e]) + (p[0][1][e] + p[1][1][e]);
+    if (shift) {
+        float sh[8];
+        if (n < 8) load_few<0>(shift, n, sh);
+        else load8<0>(shift + c, sh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += sh[e];
+    }
 }
 __device__ __forceinline__ float activate(float o, int act) {
     if (act == 1) return 1.f / (1.f + expf(-o));
@@ -736,42 +720,18 @@ struct FoldArgs {
     int H, W, C, act, log;
 };
 
-// 2^log lanes an output pixel, eight channels each: neighbouring ones (VEC: every tap and row of results on a 16-byte
-// border), else every 2^log-th.  Every input value goes to exactly one output: nothing is read twice.  Bound by HBM
-// (codes of 1000 x 16 x 16 x 64: 594 MB in 108 us, 5.5 TB/s; the codes past the caches too: 104, but the next product then
-// waits for them, a thousand alignments drawn 600 us for 590).
-template <int TYPE, bool VEC, bool Q8>
+// 2^log lanes an output pixel, eight neighbouring channels each, the last lane the pixel's last eight.  Every input value goes
+// to exactly one output: nothing is read twice.  Bound by HBM (codes of 1000 x 16 x 16 x 64: 594 MB in 108 us, 5.5 TB/s; the
+// codes past the caches too: 104, but the next product then waits for them, a thousand alignments drawn 600 us for 590).
+template <int TYPE, bool Q8>
 __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned pix = blockIdx.x * (256u >> a.log) + (threadIdx.x >> a.log);
-    const int l = threadIdx.x & ((1 << a.log) - 1), C = a.C;
+    const int l = threadIdx.x & ((1 << a.log) - 1), C = a.C, c = C < 8 ? 0 : min(l * 8, C - 8);
     if (pix >= a.pixels) return;        // whole groups of 2^log lanes
     const Taps t = taps_of(pix, a.H, a.W, C);
-    float v[8];
-    if constexpr (VEC) {
-        const int c = l * 8;
-        float p[2][2][8], sh[8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[i][j][e] = 0.f;
-                if (c < C && t.at[i][j] >= 0) load8<TYPE, true>(y + t.at[i][j] + c, p[i][j]);
-            }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sh[e] = a.shift && c < C ? a.shift[c + e] : 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float o = (p[0][0][e] + p[1][0][e]) + (p[0][1][e] + p[1][1][e]);
-            v[e] = a.shift ? o + sh[e] : o;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = (e << a.log) + l;
-            v[e] = c < C ? folded<TYPE>(y, t, c, a.shift) : 0.f;
-        }
-    }
+    const bool some = l * 8 < C;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (some) fold8<TYPE>(y, t, c, C, a.shift, v);
     if constexpr (Q8) {
         uint32_t mx = 0;
 #pragma unroll
@@ -779,35 +739,28 @@ __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>:
             v[e] = slope(v[e], true);
             mx = max(mx, magnitude(v[e]));
         }
-        if constexpr (VEC) mx = l * 8 < C ? mx : 0u;
         const RowScale rs = row_scale(group_max(mx, a.log));
         if (l == 0) a.scale[pix] = rs.scale;
         no_row(v, rs.inv);
         int8_t* qr = a.q + (long long)pix * a.ldq;
-        if constexpr (VEC) {
-            if (l * 8 < C)
-                *reinterpret_cast<uint2*>(qr + l * 8) = uint2{four_codes(v[0], v[1], v[2], v[3], rs.inv), four_codes(v[4], v[5], v[6], v[7], rs.inv)};
-        } else {
+        if (C < 8) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = (e << a.log) + l;
-                if (c < C) qr[c] = (int8_t)code_of(v[e], rs.inv);
-            }
+            for (int e = 0; e < 8; ++e)
+                if (e < C) qr[e] = (int8_t)code_of(v[e], rs.inv);
+        } else if (some) {
+            store_codes(qr + c, v, rs.inv);
         }
     } else {
         float* o = a.out + (long long)pix * C;
-        if constexpr (VEC) {
-            if (l * 8 < C) {
+        if (C < 8) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 4)
-                    *reinterpret_cast<f32x4*>(o + l * 8 + e) = f32x4{activate(v[e], a.act), activate(v[e + 1], a.act), activate(v[e + 2], a.act), activate(v[e + 3], a.act)};
-            }
-        } else {
+            for (int e = 0; e < 8; ++e)
+                if (e < C) o[e] = activate(v[e], a.act);
+        } else if (some) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = (e << a.log) + l;
-                if (c < C) o[c] = activate(v[e], a.act);
-            }
+            for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<f32x4_4*>(o + c + e) =
+                    f32x4_4{activate(v[e], a.act), activate(v[e + 1], a.act), activate(v[e + 2], a.act), activate(v[e + 3], a.act)};
         }
     }
 }
@@ -816,43 +769,54 @@ __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>:
 template <int TYPE, bool Q8>
 __global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned pix = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    const int l8 = (threadIdx.x & 63) * 8, C = a.C;
     if (pix >= a.pixels) return;
-    const Taps t = taps_of(pix, a.H, a.W, a.C);
+    const Taps t = taps_of(pix, a.H, a.W, C);
+    float v[8];
     if constexpr (Q8) {
         uint32_t mx = 0;
-        for (int c = lane; c < a.C; c += 64) mx = max(mx, magnitude(slope(folded<TYPE>(y, t, c, a.shift), true)));
+        for (int c = l8; c < C; c += 512) {
+            fold8<TYPE>(y, t, min(c, C - 8), C, a.shift, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = max(mx, magnitude(slope(v[e], true)));
+        }
         const RowScale rs = row_scale(group_max(mx, 6));
-        for (int c = lane; c < a.C; c += 64)
-            a.q[(long long)pix * a.ldq + c] = rs.inv == 0.f ? 0 : (int8_t)code_of(slope(folded<TYPE>(y, t, c, a.shift), true), rs.inv);
-        if (lane == 0) a.scale[pix] = rs.scale;
+        for (int c = l8; c < C; c += 512) {
+            fold8<TYPE>(y, t, min(c, C - 8), C, a.shift, v);
+            no_row(v, rs.inv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = slope(v[e], true);
+            store_codes(a.q + (long long)pix * a.ldq + min(c, C - 8), v, rs.inv);
+        }
+        if (l8 == 0) a.scale[pix] = rs.scale;
     } else {
-        for (int c = lane; c < a.C; c += 64) a.out[(long long)pix * a.C + c] = activate(folded<TYPE>(y, t, c, a.shift), a.act);
+        for (int c = l8; c < C; c += 512) {
+            fold8<TYPE>(y, t, min(c, C - 8), C, a.shift, v);
+            float* o = a.out + (long long)pix * C + min(c, C - 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = activate(v[e], a.act);
+        }
     }
 }
 
 // One channel: a lane an input pixel, for the 2 x 2 output pixels on it.  It reads what its column gives them -- taps of row 3
-// from the pixel above, 1 and 2 of its own, 0 of the one below, four at a time (VEC: y starts on a multiple of four
-// elements) -- sums them along the column, and takes from its left and right neighbours their sums of column 3 and 0.  The
+// from the pixel above, 1 and 2 of its own, 0 of the one below, four at a time -- sums them along the column, and takes from its left and right neighbours their sums of column 3 and 0.  The
 // first and last lane of a wave, whose neighbour is in another wave, make that neighbour's sums themselves.  Bound by HBM
 // (1000 x 32 x 32: 49 MB in 11 us; tap by tap 32).
-template <int TYPE, bool VEC>
+template <int TYPE>
 __device__ __forceinline__ void load_taps(const typename Elem<TYPE>::type* p, float (&v)[4]) {
-    if constexpr (VEC && TYPE == 0) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(p);
+    if constexpr (TYPE == 0) {
+        const f32x4 x = *reinterpret_cast<const f32x4_4*>(p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = x[e];
-    } else if constexpr (VEC) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        const uint16_t h[4] = {(uint16_t)x.x, (uint16_t)(x.x >> 16), (uint16_t)x.y, (uint16_t)(x.y >> 16)};
+    } else {
+        const i32x2_2 x = *reinterpret_cast<const i32x2_2*>(p);
+        const uint16_t h[4] = {(uint16_t)x[0], (uint16_t)((uint32_t)x[0] >> 16), (uint16_t)x[1], (uint16_t)((uint32_t)x[1] >> 16)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = to_f32<TYPE>(__builtin_bit_cast(typename Elem<TYPE>::type, h[e]));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = to_f32<TYPE>(p[e]);
     }
 }
-template <int TYPE, bool VEC>
+template <int TYPE>
 __global__ __launch_bounds__(256) void up_fold_one_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned i = blockIdx.x * 256 + threadIdx.x, n = a.pixels / 4, at = min(i, n - 1);
     const int H = a.H, W = a.W, lane = threadIdx.x & 63;
@@ -861,10 +825,10 @@ __global__ __launch_bounds__(256) void up_fold_one_kernel(const typename Elem<TY
     const bool up = ih > 0, down = ih + 1 < H;
     const auto* t = y + (long long)at * 16;
     float r1[4], r2[4], r3[4] = {0.f, 0.f, 0.f, 0.f}, r0[4] = {0.f, 0.f, 0.f, 0.f};
-    load_taps<TYPE, VEC>(t + 4, r1);
-    load_taps<TYPE, VEC>(t + 8, r2);
-    if (up) load_taps<TYPE, VEC>(t + 12 - 16 * (long long)W, r3);
-    if (down) load_taps<TYPE, VEC>(t + 16 * (long long)W, r0);
+    load_taps<TYPE>(t + 4, r1);
+    load_taps<TYPE>(t + 8, r2);
+    if (up) load_taps<TYPE>(t + 12 - 16 * (long long)W, r3);
+    if (down) load_taps<TYPE>(t + 16 * (long long)W, r0);
     float e[4], o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -884,9 +848,8 @@ __global__ __launch_bounds__(256) void up_fold_one_kernel(const typename Elem<TY
     const float sh = a.shift ? a.shift[0] : 0.f;
     const auto end = [&](float x) { return activate(a.shift ? x + sh : x, a.act); };
     float* to = a.out + ((long long)line * 4 * W + 2 * iw);
-    typedef float f32x2 __attribute__((ext_vector_type(2), aligned(4)));
-    *reinterpret_cast<f32x2*>(to) = f32x2{end(e[1] + le), end(e[2] + re)};
-    *reinterpret_cast<f32x2*>(to + 2 * W) = f32x2{end(o[1] + lo), end(o[2] + ro)};
+    *reinterpret_cast<f32x2_4*>(to) = f32x2_4{end(e[1] + le), end(e[2] + re)};
+    *reinterpret_cast<f32x2_4*>(to + 2 * W) = f32x2_4{end(o[1] + lo), end(o[2] + ro)};
 }
 
 // threads of one launch stay below 2^32
@@ -896,11 +859,6 @@ inline int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 constexpr long long MAX_STRIDE = 1 << 22;      // offsets of a tile's rows fit 31 bits
 constexpr int MAX_ROW = 1 << 30;               // elements, so that a place in a row plus a block's stride does too
-
-inline int row_align(const void* p, long long stride) {
-    const uintptr_t u = reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride;
-    return u % 16 == 0 ? 16 : u % 8 == 0 ? 8 : u % 4 == 0 ? 4 : 2;
-}
 
 constexpr int FEW = 32, FEW_ELEMENTS = 32768;
 
@@ -953,14 +911,13 @@ inline bool fold_fits(int type, int B, int H, int W, int C) {
     return B <= ((MAX_BLOCKS * 256) >> lanes_log(C)) / (4LL * H * W);
 }
 template <bool Q8>
-int launch_fold(const void* y, int type, FoldArgs a, bool vec, hipStream_t st) {
+int launch_fold(const void* y, int type, FoldArgs a, hipStream_t st) {
     a.log = lanes_log(a.C);
     const unsigned per = 256u >> a.log, blocks = a.pixels / per + (a.pixels % per != 0);
     return by_type(type, [&](auto t) {
         const auto* p = static_cast<const typename Elem<t.value>::type*>(y);
         if (a.C > 512) up_fold_wide_kernel<t.value, Q8><<<blocks, 256, 0, st>>>(p, a);
-        else if (vec) up_fold_kernel<t.value, true, Q8><<<blocks, 256, 0, st>>>(p, a);
-        else up_fold_kernel<t.value, false, Q8><<<blocks, 256, 0, st>>>(p, a);
+        else up_fold_kernel<t.value, Q8><<<blocks, 256, 0, st>>>(p, a);
     });
 }
 
@@ -983,8 +940,10 @@ void launch_few(const FewArgs& f, hipStream_t st) {
         if (f.g.T <= 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
         else go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
     } else {
-        if (f.g.T <= 4) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-        else if (f.g.T <= 16) go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+        const int rows = 4 << (6 - f.log);      // that the four waves take at a time
+        if (f.g.T <= rows) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        else if (f.g.T <= 2 * rows) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+        else if (f.g.T <= 4 * rows) go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
         else go(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     }
 }
@@ -1015,10 +974,9 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
     if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4) || ldx < K || ldq < K) return PGAN_EINVAL;
     if (!apart({rows_of(x, rows, K, ldx, type_bytes(x_type)), rows_of(q, rows, K, ldq, 1, true), rows_of(scale, 1, rows, 0, 4, true)}))
         return PGAN_EINVAL;
-    const bool vec = row_align(x, ldx * type_bytes(x_type)) >= 4 && row_align(q, ldq) >= 8;
     const int log = lanes_log(K);    // lanes a row
     // Rows of more than 1024 elements by a block: in a wave's registers 4096 x 4096 in bf16 took 14.9 us for 12.9, 8192 x 2048
-    // 15.0 for 12.8, 300 x 2048 4.2 for 2.8, 3000 x 3001 (borders of 2 bytes) 50 for 21, though 4000 x 1024 6.0 for 6.4.
+    // 15.0 for 12.8, 300 x 2048 4.2 for 2.8, though 4000 x 1024 6.0 for 6.4.
     constexpr int LONG_ROW = 1024;
     // Rows a lane: two where there are enough of them (16000 x 512 in bf16: 9.3 us with one, 6.7 with two)
     const int R = K <= 1024 && rows >= 8192 ? 2 : 1;
@@ -1030,15 +988,12 @@ int pgan_quant_rows(const void* x, int x_type, long long ldx, void* q, long long
             kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const typename Elem<X>::type*>(x), ldx, static_cast<int8_t*>(q), ldq,
                                                       scale, rows, K, lrelu, more...);
         };
-        if (K > LONG_ROW && !vec) go(quant_long_rows_kernel<X, false, 0>);
-        else if (K > 8192) go(quant_long_rows_kernel<X, true, 0>);
-        else if (K > 4096) go(quant_long_rows_kernel<X, true, 4>);
-        else if (K > 2048) go(quant_long_rows_kernel<X, true, 2>);
-        else if (K > LONG_ROW) go(quant_long_rows_kernel<X, true, 1>);
-        else if (K > 512 && R == 2) vec ? go(quant_rows_kernel<X, true, 2, 2>, log) : go(quant_rows_kernel<X, false, 2, 2>, log);
-        else if (K > 512) vec ? go(quant_rows_kernel<X, true, 2, 1>, log) : go(quant_rows_kernel<X, false, 2, 1>, log);
-        else if (R == 2) vec ? go(quant_rows_kernel<X, true, 1, 2>, log) : go(quant_rows_kernel<X, false, 1, 2>, log);
-        else vec ? go(quant_rows_kernel<X, true, 1, 1>, log) : go(quant_rows_kernel<X, false, 1, 1>, log);
+        if (K > 8192) go(quant_long_rows_kernel<X, 0>);
+        else if (K > 4096) go(quant_long_rows_kernel<X, 4>);
+        else if (K > 2048) go(quant_long_rows_kernel<X, 2>);
+        else if (K > LONG_ROW) go(quant_long_rows_kernel<X, 1>);
+        else if (K > 512) R == 2 ? go(quant_rows_kernel<X, 2, 2>, log) : go(quant_rows_kernel<X, 2, 1>, log);
+        else R == 2 ? go(quant_rows_kernel<X, 1, 2>, log) : go(quant_rows_kernel<X, 1, 1>, log);
     });
 }
 
@@ -1048,8 +1003,7 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
     if (rc || T == 0) return rc;
     return by_type(y_type, [&](auto t) {
         constexpr int Y = t.value;
-        GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0,
-                   row_align(y, ldy * type_bytes(y_type))};
+        GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0};
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
         // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
         // behind another's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight waves, one block
@@ -1086,9 +1040,8 @@ int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long 
     if (T <= FEW && T * K <= FEW_ELEMENTS)
         return by_type(x_type, [&](auto xt) {
             (void)by_type(y_type, [&](auto t) {
-                const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0,
-                                 row_align(y, ldy * type_bytes(y_type))};
-                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, row_align(x, ldx * type_bytes(x_type)) >= 4}, st);
+                const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0};
+                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, lanes_log(K)}, st);
             });
         });
     const int rc = pgan_quant_rows(x, x_type, ldx, q, ldq, q_scale, T, K, lrelu, st);
@@ -1105,7 +1058,7 @@ int pgan_up_fold_q8(const void* y, int y_type, const float* shift, void* q, long
                 rows_of(scale, 1, pixels, 0, 4, true)}))
         return PGAN_EINVAL;
     FoldArgs a{shift, static_cast<int8_t*>(q), scale, nullptr, ldq, (unsigned)pixels, H, W, C, 0, 0};
-    return launch_fold<true>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && row_align(q, ldq) >= 8, st);
+    return launch_fold<true>(y, y_type, a, st);
 }
 
 int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int B, int H, int W, int C, int act,
@@ -1120,10 +1073,9 @@ int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int 
     if (C == 1)
         return by_type(y_type, [&](auto t) {
             const auto* p = static_cast<const typename Elem<t.value>::type*>(y);
-            if (aligned(y, 4 * type_bytes(y_type))) up_fold_one_kernel<t.value, true><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(p, a);
-            else up_fold_one_kernel<t.value, false><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(p, a);
+            up_fold_one_kernel<t.value><<<(a.pixels / 4 + 255) / 256, 256, 0, st>>>(p, a);
         });
-    return launch_fold<false>(y, y_type, a, C % 8 == 0 && aligned(y, 16) && aligned(out, 16), st);
+    return launch_fold<false>(y, y_type, a, st);
 }
 
 }  // extern "C"

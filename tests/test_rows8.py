@@ -478,3 +478,44 @@ def test_quant_rows_of_more_than_a_wave(hip, K, dtype):
             assert torch.equal(q.cpu(), want)
             same(s.cpu(), ws)
             rest_kept(q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_operand_on_borders_of_one_element(hip, dtype):
+    """Rows of x and y that start anywhere in memory, with odd strides; what lies between and around y's rows stays."""
+    rng = np.random.default_rng(12)
+    for T, K, N in ((1, 5, 3), (7, 200, 90), (30, 700, 130), (21, 300, 1000), (70, 1001, 257), (300, 129, 640), (5000, 65, 33), (6500, 70, 1301)):
+        x = (rnd(rng, T, K) * torch.exp(rnd(rng, T, 1))).to(dtype)
+        _, w, _, ws, bias = product_case(T, 1, K, N)
+        ldx, ldy = K + 1 + K % 2 * 2, N + 3 - N % 2
+        assert ldy % 2 == 1 or N % 2 == 0
+        xb = torch.full((T * ldx + 1,), float("nan"), dtype=dtype, device=DEV)
+        xv = xb[1:].view(T, ldx)[:, :K]
+        xv.copy_(x.to(DEV))
+        yb = torch.full((T * ldy + 1,), 7.0, dtype=dtype, device=DEV)
+        yv = yb[1:].view(T, ldy)[:, :N]
+        q, s = rows8(torch.zeros(T, K, dtype=torch.int8)), torch.zeros(T, device=DEV)
+        hip.linear_q8(xv, rows8(w), ws.to(DEV), yv, q, s, bias.to(DEV), lrelu=True)
+        want, tol = product64(*codes_of(lrelu(x.float())), w, ws, bias)
+        check_product(yv, want, tol, dtype)
+        assert float(yb[0]) == 7 and bool((yb[1:].view(T, ldy)[:, N:] == 7).all())
+        q2, s2 = rows8(torch.zeros(T, K, dtype=torch.int8)), torch.zeros(T, device=DEV)
+        hip.quant_rows(xv, q2, s2, lrelu=True)
+        qw, sw = codes_of(lrelu(x.float()))
+        assert torch.equal(q2.cpu(), qw) and torch.equal(s2.cpu(), sw)
+        rest_kept(q2)
+    for B, H, W, C in ((2, 3, 5, 1), (1, 4, 3, 5), (2, 2, 2, 13), (1, 3, 2, 64), (1, 2, 2, 333), (1, 1, 2, 700)):
+        y, shift = rnd(rng, B, H, W, 16 * C).to(dtype), rnd(rng, C)
+        yb = torch.full((y.numel() + 2,), float("nan"), dtype=dtype, device=DEV)
+        yv = yb[1:-1].view(y.shape)
+        yv.copy_(y.to(DEV))
+        ob = torch.full((4 * B * H * W * C + 2,), 7.0, device=DEV)
+        ov = ob[1:-1].view(B, 2 * H, 2 * W, C)
+        hip.up_fold(yv, shift.to(DEV), ov)
+        assert torch.equal(ov.cpu(), fold32(y, shift)) and float(ob[0]) == 7 and float(ob[-1]) == 7
+        q, s = rows8(torch.zeros(4 * B * H * W, C, dtype=torch.int8)), torch.zeros(4 * B * H * W, device=DEV)
+        hip.up_fold_q8(yv, shift.to(DEV), q, s)
+        qw, sw = codes_of(lrelu(fold32(y, shift)).view(-1, C))
+        assert torch.equal(q.cpu(), qw) and torch.equal(s.cpu(), sw)
+        rest_kept(q)

@@ -503,8 +503,8 @@ __global__ __launch_bounds__(64 * WT * WN, MW) void gemm_q8_kernel(const GemmArg
 // ---- the product for few tiles ------------------------------------------------------------------------------------
 // A block makes 32 tokens x 32 channels, its WV waves share K and add up their sums (whole numbers: any order) in LDS.
 // Channels come straight from memory into the matrix instruction's registers, every line of them by one wave.  X >= 0: the
-// block makes the tokens' codes itself, a wave RW rows -- every block all of them, which for up to 32768 elements takes less
-// time than a launch of its own -- while its first channels are on their way; X < 0: it reads codes.  Bound by the launch
+// block makes the tokens' codes itself, a lane parts of RW rows -- every block all of them, which for few of them takes less time
+// than a launch of its own -- while its first channels are on their way; X < 0: it reads codes.  Bound by the launch
 // (1 x 128 x 8192: 3.7 us in a graph), then by the channels' bytes (1 x 8192 x 8192: 15 us, 4.5 TB/s).
 struct FewArgs {
     GemmArgs g;
@@ -860,7 +860,17 @@ inline int type_bytes(int type) { return type == 0 ? 4 : 2; }
 constexpr long long MAX_STRIDE = 1 << 22;      // offsets of a tile's rows fit 31 bits
 constexpr int MAX_ROW = 1 << 30;               // elements, so that a place in a row plus a block's stride does too
 
-constexpr int FEW = 32, FEW_ELEMENTS = 32768;
+// lanes a row or an output pixel (as a power of two): eight elements each, all 64 for more than 256
+inline int lanes_log(int C) {
+    int log = 0;
+    while (log < 6 && (8 << log) < C) ++log;
+    return log;
+}
+
+constexpr int FEW = 32;
+// waves of a block of a product of few tiles, and rows that they make the codes of at a time (512 elements of each)
+inline int few_waves(int K) { return K >= 1024 ? 8 : 4; }
+inline int few_rows(int K) { return few_waves(K) << (6 - lanes_log(K)); }
 
 template <int FT, int FN, int WT, int WN, int GK, int D, int MW, int TYPE>
 void launch_gemm(GemmArgs a, hipStream_t st) {
@@ -900,12 +910,6 @@ bool apart(const Span (&s)[N]) {
     return true;
 }
 
-// lanes a row or an output pixel (as a power of two): eight elements each, all 64 for more than 256
-inline int lanes_log(int C) {
-    int log = 0;
-    while (log < 6 && (8 << log) < C) ++log;
-    return log;
-}
 inline bool fold_fits(int type, int B, int H, int W, int C) {
     if (B < 0 || H < 1 || W < 1 || C < 1 || C > MAX_ROW || type < 0 || type > 2 || H > 32768 || W > 32768) return false;
     return B <= ((MAX_BLOCKS * 256) >> lanes_log(C)) / (4LL * H * W);
@@ -934,17 +938,15 @@ void launch_few(const FewArgs& f, hipStream_t st) {
     };
     using std::integral_constant;
     if constexpr (X < 0) {
-        if (K >= 1024) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        if (few_waves(K) == 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
         else go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     } else if (K >= 1024) {
-        if (f.g.T <= 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-        else go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+        go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
     } else {
-        const int rows = 4 << (6 - f.log);      // that the four waves take at a time
+        const int rows = few_rows(K);
         if (f.g.T <= rows) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
         else if (f.g.T <= 2 * rows) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-        else if (f.g.T <= 4 * rows) go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-        else go(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+        else go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
     }
 }
 
@@ -1037,7 +1039,10 @@ int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long 
         || !apart({rows_of(x, T, K, ldx, type_bytes(x_type)), rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1, true),
                    rows_of(q_scale, 1, T, 0, 4, true), rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
-    if (T <= FEW && T * K <= FEW_ELEMENTS)
+    // The product's blocks make the codes where that takes a wave four loads a lane at most: us in one launch and in two,
+    // 16 x 512 x 1024 6.2 and 6.2, 8 x 700 x 1024 7.1 and 7.2, 8 x 2048 x 1024 7.3 and 7.5, 32 x 128 x 8192 4.9 and 6.2; past that
+    // 32 x 512 x 1024 9.1 and 6.2, 16 x 700 x 1024 10.2 and 7.2, 1 x 4096 x 1024 10.2 and 9.1.
+    if (T <= FEW && (T + few_rows(K) - 1) / few_rows(K) * ((K + 511) / 512) <= 4)
         return by_type(x_type, [&](auto xt) {
             (void)by_type(y_type, [&](auto t) {
                 const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0};

@@ -1018,14 +1018,19 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         //   2048 x 2048 x 2048     23   18   16   15   17       777 x 1001 x 1234     17   10    9    8    8
         //   4000 x 1000 x 2000     20   17   18   19   21       600 x 2000 x 1000     24   17   14    9    8
         // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
-        // shares K among the waves of a block of 32 x 32 instead: 1024 x 1024 x 512 (128 tiles of 64 x 64) 4.8 us against 6.0,
-        // 64 x 4096 x 1024 7.6 against 14.9, but 777 x 1001 x 1234 10 against 8.
-        if (T <= FEW || tiles(64, 64) <= 128) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
+        // shares K among the waves of a block of 32 x 32 instead, one of somewhat more takes tiles of 64 x 32 (two waves): us in
+        // 32 x 32, 64 x 32, 64 x 64
+        //   64 x 4096 x 1024      7.3   9.3  11.1         704 x 4096 x 688     12.8  10.7  12.2
+        //   512 x 4096 x 512      8.7   9.5  11.1        1024 x 4096 x 512     13.1  10.3  11.7
+        //   512 x 512 x 512       3.9   4.2   4.3        1024 x 1024 x 512      5.6   5.0   5.3
+        //                                                1024 x 2048 x 1024    12.4   8.1   7.6
+        if (T <= FEW || tiles(64, 64) <= 64) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
         else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
         else if (K >= 1024 && tiles(256, 256) >= (K < 2048 ? 256 : 144)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
         else if (K >= 512 && tiles(128, 256) >= 512) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
         else if (tiles(128, 128) >= 448) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
         else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
+        else if (tiles(64, 64) <= 160) launch_gemm<1, 1, 2, 1, 128, 4, 2, Y>(a, st);
         else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);
     });
 }

@@ -142,8 +142,9 @@ def test_gemm_q8(hip, T, K, N, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,N,Ks", [(4097, 4100, (1024, 1030)), (7300, 1025, (512, 1001)), (7300, 2100, (512, 577, 1001)), (6500, 1300, (1, 64, 65, 128, 190, 200, 256, 500)),
-                                    (5000, 1100, (1, 128, 129, 256, 300, 513, 700)), (1000, 700, (1, 127, 129, 300, 385, 2000)),
+@pytest.mark.parametrize("T,N,Ks", [(4097, 4100, (1024, 1030)), (7300, 1025, (512, 1001)), (7300, 2100, (512, 577, 1001)),
+                                    (6500, 1300, (1, 64, 65, 128, 190, 200, 256, 500)),
+                                    (5000, 1100, (1, 128, 129, 256, 300, 513, 700)), (1000, 700, (1, 127, 129, 300, 385, 2000)), (650, 600, (1, 128, 129, 512, 520, 900)),
                                     (100000, 30, (1, 64, 70, 129, 200)), (9000, 32, (33, 4096))])
 def test_gemm_q8_of_every_tile(hip, T, N, Ks):
     """Each tile size with K of one stage of its ring, of a few, of more than it holds, and with a rest.  (The sums of the oracle

@@ -1007,16 +1007,21 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         constexpr int Y = t.value;
         GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0};
         const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
+        // how many in a hundred of the CUs that the last round of tiles takes along have one
+        const auto fill = [&](long long bt, long long bn) { return tiles(bt, bn) * 100 / ((tiles(bt, bn) + 255) / 256 * 256); };
         // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
-        // behind another's products; and each of the 256 CUs wants a tile.  us in tiles of 256 x 256 (eight waves, one block
-        // a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64, 64 x 64, results in bf16:
-        //   4096 x 4096 x 4096     64   77   86   84    -      16000 x 512 x 4096     57   50   52   62   83
-        //   4096 x 2048 x 4096     36   40   45   45   58       4000 x 512 x 4096     17   14   15   19   23
-        //   3000 x 4000 x 3000     52   71   66   65   77      64000 x 256 x 2048     80   70   66   85  116
-        //   5000 x 2048 x 2000     29   33   30   30   39    256000 x 128 x 1024     122  108   95  130  175
-        //   2000 x 8000 x 2000     81   60   64   51   65      8000 x 1024 x 1024     16   17   13   16   19
-        //   2048 x 2048 x 2048     23   18   16   15   17       777 x 1001 x 1234     17   10    9    8    8
-        //   4000 x 1000 x 2000     20   17   18   19   21       600 x 2000 x 1000     24   17   14    9    8
+        // behind another's products; and the last round of tiles should find a tile for most of the 256 CUs.  us in tiles of
+        // 256 x 256 (eight waves, one block a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64,
+        // 64 x 64, results in bf16:
+        //   4096 x 4096 x 4096     63   74   83   82  102      16000 x 512 x 4096     53   47   50   62   86
+        //   4096 x 2048 x 4096     36   40   45   45   58       4000 x 512 x 4096     15   14   15   17   21
+        //   3000 x 4000 x 3000     43   59   51   51   59      64000 x 256 x 2048     82   69   65   85  116
+        //   5000 x 2048 x 2000     28   31   28   29   36    256000 x 128 x 1024     118  106   96  127  173
+        //   6000 x 1200 x 6000     68   59   63   71   94       9493 x 422 x 7069     82   75   83  111  107
+        //   2500 x 2500 x 2500     31   25   25   33   31      10000 x 1000 x 1000    19   20   18   20   22
+        //   1037 x 2288 x 5552     27   21   23   28   25       4000 x 2000 x 1000    24   17   17   14   17
+        //   2000 x 8000 x 2000     73   54   55   42   54       2048 x 2048 x 2048    24   18   17   13   17
+        //   1500 x 4000 x 1500     40   29   28   22   21       1944 x 1575 x 1304    21   14   15   12   12
         // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
         // shares K among the waves of a block of 32 x 32 instead, one of somewhat more takes tiles of 64 x 32 (two waves): us in
         // 32 x 32, 64 x 32, 64 x 64
@@ -1026,11 +1031,11 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
         //                                                1024 x 2048 x 1024    12.4   8.1   7.6
         if (T <= FEW || tiles(64, 64) <= 64) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
         else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
-        else if (K >= 1024 && tiles(256, 256) >= (K < 2048 ? 256 : 144)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
-        else if (K >= 512 && tiles(128, 256) >= 512) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
+        else if (K >= 1024 && fill(256, 256) >= (K < 2048 ? 90 : 55)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
+        else if (K > 256 && fill(128, 256) >= 70) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
         else if (tiles(128, 128) >= 448) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
         else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
-        else if (tiles(64, 64) <= 160) launch_gemm<1, 1, 2, 1, 128, 4, 2, Y>(a, st);
+        else if (tiles(64, 64) <= 128) launch_gemm<1, 1, 2, 1, 128, 4, 2, Y>(a, st);
         else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);
     });
 }

@@ -418,8 +418,10 @@ ADAMW_BLOCK = 256      # elements of an 8-bit AdamW state that share a scale
 
 
 def rows8(rows: int, cols: int, device) -> torch.Tensor:
-    """[rows, cols] int8 buffer for the codes of quant_rows / gemm_q8: rows start on 16-byte borders."""
-    return torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :cols]
+    """[rows, cols] int8 buffer for the codes of quant_rows / gemm_q8: rows start on 16-byte borders, from 128 columns on on
+    those of 128-byte lines (a product of 2048 x 4080 x 2048 takes 24 us with such rows, 32 with rows of 4080 bytes)."""
+    step = 128 if cols >= 128 else 16
+    return torch.zeros(rows, (cols + step - 1) // step * step, dtype=torch.int8, device=device)[:, :cols]
 
 
 class AdamWPlan:

@@ -520,3 +520,17 @@ def test_every_operand_on_borders_of_one_element(hip, dtype):
         qw, sw = codes_of(lrelu(fold32(y, shift)).view(-1, C))
         assert torch.equal(q.cpu(), qw) and torch.equal(s.cpu(), sw)
         rest_kept(q)
+
+
+@pytest.mark.gpu
+def test_rows8_buffers(hip):
+    """What pgan_hip.rows8 gives: zeros, rows that a product takes, from 128 columns on one to a run of 128-byte lines."""
+    from pgan_hip import rows8 as buffer
+    for T, K in ((3, 1), (2, 16), (5, 127), (1, 128), (4, 129), (3, 1000), (0, 40)):
+        b = buffer(T, K, DEV)
+        assert b.shape == (T, K) and b.dtype == torch.int8 and b.stride(0) % (128 if K >= 128 else 16) == 0 and not bool(b.any())
+        s, w, ws, y = torch.ones(max(T, 1), device=DEV), buffer(6, K, DEV), torch.ones(6, device=DEV), torch.ones(T, 6, device=DEV)
+        w.fill_(1)
+        b.fill_(2)
+        hip.gemm_q8(b, s, w, ws, y)
+        assert torch.equal(y, torch.full_like(y, 2.0 * K))

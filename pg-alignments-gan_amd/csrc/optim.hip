@@ -44,7 +44,7 @@ struct AwTensor {
     long long n;
     float size;                     // lr / (1 - b1^t); lr alone where the step count lives on the device
     float keep;                     // 1 - lr wd
-    int types;                      // p type + 3 * g type, + 16 where every pointer allows vector accesses
+    int types;                      // p type + 3 * g type
     int index;                      // number of the tensor in the caller's list
 };
 struct AwArgs {
@@ -73,17 +73,20 @@ __device__ __forceinline__ uint16_t to16(float x, int type) {
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
+// Global memory takes wide accesses on any border; these types say so.
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_1 __attribute__((aligned(1)));
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <bool NT, class V>
-__device__ __forceinline__ V get(const void* p) {
-    if constexpr (NT) return __builtin_nontemporal_load(static_cast<const V*>(p));
-    else return *static_cast<const V*>(p);
+template <bool NT, class P>
+__device__ __forceinline__ auto get(const P* p) {
+    return NT ? __builtin_nontemporal_load(p) : *p;
 }
-template <bool NT, class V>
-__device__ __forceinline__ void put(void* p, V v) {
-    if constexpr (NT) __builtin_nontemporal_store(v, static_cast<V*>(p));
-    else *static_cast<V*>(p) = v;
+template <bool NT, class P, class V>
+__device__ __forceinline__ void put(P* p, V v) {
+    if constexpr (NT) __builtin_nontemporal_store(P(v), p);
+    else *p = v;
 }
 
 // Four elements of a tensor: o (a lane's) past b, which is the same for the whole wave and stays in scalar registers.  VEC: one
@@ -93,7 +96,7 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
     if constexpr (TYPE == 0) {
         const float* s = static_cast<const float*>(src) + b;
         if constexpr (VEC) {
-            const f32x4 x = get<NT, f32x4>(s + o);
+            const f32x4 x = get<NT>(reinterpret_cast<const f32x4_4*>(s + o));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = x[e];
         } else {
@@ -103,7 +106,7 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
     } else {
         const uint16_t* s = static_cast<const uint16_t*>(src) + b;
         if constexpr (VEC) {
-            const u32x2 x = get<NT, u32x2>(s + o);
+            const u32x2 x = get<NT>(reinterpret_cast<const u32x2_2*>(s + o));
             if constexpr (TYPE == 1) {
                 v[0] = __builtin_bit_cast(float, x.x << 16);
                 v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
@@ -126,7 +129,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
     if constexpr (TYPE == 0) {
         float* d = static_cast<float*>(dst) + b;
         if constexpr (VEC) {
-            put<NT>(d + o, f32x4{v[0], v[1], v[2], v[3]});
+            put<NT>(reinterpret_cast<f32x4_4*>(d + o), f32x4{v[0], v[1], v[2], v[3]});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -137,7 +140,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
         if constexpr (VEC) {
             using H = std::conditional_t<TYPE == 1, __bf16, _Float16>;
             typedef H h2 __attribute__((ext_vector_type(2)));
-            put<NT>(d + o, u32x2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})});
+            put<NT>(reinterpret_cast<u32x2_2*>(d + o), u32x2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -148,7 +151,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
 template <bool VEC, bool NT>
 __device__ __forceinline__ uint32_t load_codes(const void* src, long long b, int o, long long n) {
     const uint8_t* s = static_cast<const uint8_t*>(src) + b;
-    if constexpr (VEC) return get<NT, uint32_t>(s + o);
+    if constexpr (VEC) return get<NT>(reinterpret_cast<const u32_1*>(s + o));
     uint32_t u = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -159,7 +162,7 @@ template <bool VEC, bool NT>
 __device__ __forceinline__ void store_codes(void* dst, long long b, int o, long long n, uint32_t u) {
     uint8_t* d = static_cast<uint8_t*>(dst) + b;
     if constexpr (VEC) {
-        put<NT>(d + o, u);
+        put<NT>(reinterpret_cast<u32_1*>(d + o), u);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -302,13 +305,13 @@ struct Block8 {
 };
 
 template <int BITS, bool NT, int PT, int GT>
-__device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long long at, bool vec, uint32_t key) {
+__device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long long at, uint32_t key) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (BITS == 32) {
 #pragma unroll
         for (int u = 0; u < AW_CHUNK / 1024; ++u) {
             const long long b = at + u * 1024 + wave * 256;
-            if (vec && b + 256 <= t.n) {
+            if (b + 256 <= t.n) {
                 body32<PT, GT, true, NT>(t, s, b, lane * 4);
             } else if (b + lane * 4 < t.n) {
                 body32<PT, GT, false, NT>(t, s, b, lane * 4);
@@ -317,7 +320,7 @@ __device__ __forceinline__ void chunk(const AwTensor& t, const AwStep& s, long l
     } else {
         // two blocks of 256 a wave, the second one's reads under way while the first is computed
         const long long b = at + wave * (2 * AW_BLOCK);
-        if (vec && b + 2 * AW_BLOCK <= t.n) {
+        if (b + 2 * AW_BLOCK <= t.n) {
             Block8<PT, GT, true, NT> x, y;
             x.load(t, b, lane * 4);
             y.load(t, b + AW_BLOCK, lane * 4);
@@ -351,17 +354,16 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwArgs a) {
         s.inv2 = __builtin_bit_cast(float, a.step_dev[2]);
     }
     const uint32_t key = BITS == 8 ? mix(a.seed + step * 0xA54FF53Bu + (uint32_t)t.index * 0x3C6EF373u) : 0u;
-    const bool vec = t.types >= 16;
-    switch (t.types & 15) {
-        case 0: chunk<BITS, NT, 0, 0>(t, s, at, vec, key); break;
-        case 1: chunk<BITS, NT, 1, 0>(t, s, at, vec, key); break;
-        case 2: chunk<BITS, NT, 2, 0>(t, s, at, vec, key); break;
-        case 3: chunk<BITS, NT, 0, 1>(t, s, at, vec, key); break;
-        case 4: chunk<BITS, NT, 1, 1>(t, s, at, vec, key); break;
-        case 5: chunk<BITS, NT, 2, 1>(t, s, at, vec, key); break;
-        case 6: chunk<BITS, NT, 0, 2>(t, s, at, vec, key); break;
-        case 7: chunk<BITS, NT, 1, 2>(t, s, at, vec, key); break;
-        default: chunk<BITS, NT, 2, 2>(t, s, at, vec, key); break;
+    switch (t.types) {
+        case 0: chunk<BITS, NT, 0, 0>(t, s, at, key); break;
+        case 1: chunk<BITS, NT, 1, 0>(t, s, at, key); break;
+        case 2: chunk<BITS, NT, 2, 0>(t, s, at, key); break;
+        case 3: chunk<BITS, NT, 0, 1>(t, s, at, key); break;
+        case 4: chunk<BITS, NT, 1, 1>(t, s, at, key); break;
+        case 5: chunk<BITS, NT, 2, 1>(t, s, at, key); break;
+        case 6: chunk<BITS, NT, 0, 2>(t, s, at, key); break;
+        case 7: chunk<BITS, NT, 1, 2>(t, s, at, key); break;
+        default: chunk<BITS, NT, 2, 2>(t, s, at, key); break;
     }
 }
 
@@ -460,12 +462,9 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
             if (numel[i] == 0) continue;
             const long long c = (numel[i] + AW_CHUNK - 1) / AW_CHUNK;
             if (chunks + c > AW_MOST) break;
-            const int pt = types[i] % 3, gt = types[i] / 3;
-            const bool vec = aligned(p[i], 4 * size_of[pt]) && aligned(g[i], 4 * size_of[gt])
-                             && aligned(m[i], bits / 2) && aligned(v[i], bits / 2);
             a.first[a.n] = (unsigned)chunks;
             a.t[a.n] = AwTensor{p[i], g[i], m[i], v[i], bits == 8 ? m_scale[i] : nullptr, bits == 8 ? r_scale[i] : nullptr,
-                                numel[i], (float)(lr[i] / bc1), (float)(1.0 - lr[i] * decay[i]), types[i] + (vec ? 16 : 0), i};
+                                numel[i], (float)(lr[i] / bc1), (float)(1.0 - lr[i] * decay[i]), types[i], i};
             chunks += c;
             ++a.n;
         }

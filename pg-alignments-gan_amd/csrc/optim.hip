@@ -73,20 +73,44 @@ __device__ __forceinline__ uint16_t to16(float x, int type) {
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// Global memory takes wide accesses on any border; these types say so.
+// Four elements in one access, on any border (global memory takes them so); NT: past the caches.
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32_1 __attribute__((aligned(1)));
 typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <bool NT, class P>
-__device__ __forceinline__ auto get(const P* p) {
-    return NT ? __builtin_nontemporal_load(p) : *p;
+template <bool NT>
+__device__ __forceinline__ f32x4 get(const float* p) {
+    const f32x4_4* q = reinterpret_cast<const f32x4_4*>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
 }
-template <bool NT, class P, class V>
-__device__ __forceinline__ void put(P* p, V v) {
-    if constexpr (NT) __builtin_nontemporal_store(P(v), p);
-    else *p = v;
+template <bool NT>
+__device__ __forceinline__ u32x2 get(const uint16_t* p) {
+    const u32x2_2* q = reinterpret_cast<const u32x2_2*>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool NT>
+__device__ __forceinline__ uint32_t get(const uint8_t* p) {
+    const u32_1* q = reinterpret_cast<const u32_1*>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool NT>
+__device__ __forceinline__ void put(float* p, f32x4_4 v) {
+    f32x4_4* q = reinterpret_cast<f32x4_4*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(v, q);
+    else *q = v;
+}
+template <bool NT>
+__device__ __forceinline__ void put(uint16_t* p, u32x2_2 v) {
+    u32x2_2* q = reinterpret_cast<u32x2_2*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(v, q);
+    else *q = v;
+}
+template <bool NT>
+__device__ __forceinline__ void put(uint8_t* p, uint32_t v) {
+    u32_1* q = reinterpret_cast<u32_1*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(v, q);
+    else *q = v;
 }
 
 // Four elements of a tensor: o (a lane's) past b, which is the same for the whole wave and stays in scalar registers.  VEC: one
@@ -96,7 +120,7 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
     if constexpr (TYPE == 0) {
         const float* s = static_cast<const float*>(src) + b;
         if constexpr (VEC) {
-            const f32x4 x = get<NT>(reinterpret_cast<const f32x4_4*>(s + o));
+            const f32x4 x = get<NT>(s + o);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = x[e];
         } else {
@@ -106,7 +130,7 @@ __device__ __forceinline__ void load4(const void* src, long long b, int o, long 
     } else {
         const uint16_t* s = static_cast<const uint16_t*>(src) + b;
         if constexpr (VEC) {
-            const u32x2 x = get<NT>(reinterpret_cast<const u32x2_2*>(s + o));
+            const u32x2 x = get<NT>(s + o);
             if constexpr (TYPE == 1) {
                 v[0] = __builtin_bit_cast(float, x.x << 16);
                 v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
@@ -129,7 +153,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
     if constexpr (TYPE == 0) {
         float* d = static_cast<float*>(dst) + b;
         if constexpr (VEC) {
-            put<NT>(reinterpret_cast<f32x4_4*>(d + o), f32x4{v[0], v[1], v[2], v[3]});
+            put<NT>(d + o, f32x4_4{v[0], v[1], v[2], v[3]});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -140,7 +164,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
         if constexpr (VEC) {
             using H = std::conditional_t<TYPE == 1, __bf16, _Float16>;
             typedef H h2 __attribute__((ext_vector_type(2)));
-            put<NT>(reinterpret_cast<u32x2_2*>(d + o), u32x2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})});
+            put<NT>(d + o, u32x2_2{__builtin_bit_cast(uint32_t, h2{(H)v[0], (H)v[1]}), __builtin_bit_cast(uint32_t, h2{(H)v[2], (H)v[3]})});
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -151,7 +175,7 @@ __device__ __forceinline__ void store4(void* dst, long long b, int o, long long 
 template <bool VEC, bool NT>
 __device__ __forceinline__ uint32_t load_codes(const void* src, long long b, int o, long long n) {
     const uint8_t* s = static_cast<const uint8_t*>(src) + b;
-    if constexpr (VEC) return get<NT>(reinterpret_cast<const u32_1*>(s + o));
+    if constexpr (VEC) return get<NT>(s + o);
     uint32_t u = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -162,7 +186,7 @@ template <bool VEC, bool NT>
 __device__ __forceinline__ void store_codes(void* dst, long long b, int o, long long n, uint32_t u) {
     uint8_t* d = static_cast<uint8_t*>(dst) + b;
     if constexpr (VEC) {
-        put<NT>(reinterpret_cast<u32_1*>(d + o), u);
+        put<NT>(d + o, u);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)

@@ -634,3 +634,55 @@ def test_a_backward_pass_over_stepped_weights_is_refused():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Each operator on two streams beside each other, with buffers of their own, gives what it gives alone."""
+    from pgan_hip import HipOps, rows8
+    hip = HipOps(DEV, ws_floats=4, max_samples=1)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+
+    def lane(T, K, N, n):
+        x, w, ws, y = rnd(T, K).bfloat16(), rows8(N, K, DEV), torch.zeros(N, device=DEV), torch.zeros(T, N, device=DEV)
+        hip.quant_rows(rnd(N, K), w, ws)
+        q, qs, taps = rows8(T, K, DEV), torch.zeros(T, device=DEV), rnd(n, 6, 6, 16 * 24).half()
+        fq, fs = rows8(n * 144, 24, DEV), torch.zeros(n * 144, device=DEV)
+        p, g = [rnd(n * 1000), rnd(300)], [rnd(n * 1000), rnd(300)]
+        m, v = ([torch.zeros(t.numel(), dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for t in p] for _ in range(2))
+        sc = [[torch.zeros(-(-t.numel() // 256), device=DEV) for t in p] for _ in range(2)]
+        start = [t.clone() for t in p]
+        plan = hip.adamw_plan(p, m, v, sc)
+
+        def reset():
+            for t, s in zip(p, start):
+                t.copy_(s)
+            for t in m + v + sc[0] + sc[1] + [y, fs]:
+                t.view(torch.uint8).zero_()
+
+        def work():
+            for t in range(1, 9):
+                hip.linear_q8(x, w, ws, y, q, qs, lrelu=True)
+                plan.step(g, t, 1e-2, B1, B2, EPS, 0.01, seed=4)
+                hip.up_fold_q8(taps, None, fq, fs)
+        results = lambda: [t.view(torch.uint8).clone() for t in [y, fq.contiguous(), fs] + p + m + v + sc[0] + sc[1]]
+        return reset, work, results
+    lanes = [lane(700, 640, 900, 40), lane(20, 300, 70, 7)]
+    want = []
+    for reset, work, results in lanes:
+        reset()
+        work()
+        torch.cuda.synchronize()
+        want.append(results())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for reset, _, _ in lanes:
+            reset()
+        torch.cuda.synchronize()
+        for s, (_, work, _) in zip(streams, lanes):
+            with torch.cuda.stream(s):
+                work()
+        torch.cuda.synchronize()
+        for (_, _, results), w in zip(lanes, want):
+            assert all(torch.equal(a, b) for a, b in zip(results(), w))

@@ -349,6 +349,8 @@ int pgan_gemm(const float* A, const float* B, float* C, int M, int N, int K, int
  *   and w start on 16-byte borders (base and stride) and are readable up to the next multiple of 16 past K; what stands
  *   there does not matter.
  * pgan_linear_q8: both, through the caller's q (T rows of stride ldq) and q_scale.
+ * pgan_linear_q8_rows (no launch): 0 where pgan_linear_q8 makes the codes of T rows of K elements in a launch of its own;
+ *   else it is one launch, and this the number of rows (at least T) whose codes each of its blocks can make.
  * pgan_up_fold_q8 / pgan_up_fold: the end of ConvTranspose2d(k 4, stride 2, padding 1) (src/layers.py:97-115) made as a
  *   product whose channels are (kh, kw, c): y[B][H][W][4][4][C] -> [B][2H][2W][C] = sum of the up to four taps + shift[c]
  *   (NULL: none); then LeakyReLU(0.1) and pgan_quant_rows' codes (one row a pixel), or fp32 through act 0 none, 1 sigmoid,
@@ -360,6 +362,7 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
 int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long ldq, float* q_scale, const void* w,
                    long long ldw, const float* w_scale, const float* bias, void* y, int y_type, long long ldy, long long T,
                    int N, int K, int lrelu, hipStream_t st);
+int pgan_linear_q8_rows(long long T, int K);
 int pgan_up_fold_q8(const void* y, int y_type, const float* shift, void* q, long long ldq, float* scale, int B, int H, int W,
                     int C, hipStream_t st);
 int pgan_up_fold(const void* y, int y_type, const float* shift, float* out, int B, int H, int W, int C, int act,

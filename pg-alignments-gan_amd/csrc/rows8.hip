@@ -871,6 +871,18 @@ constexpr int FEW = 32;
 // waves of a block of a product of few tiles, and rows that they make the codes of at a time (512 elements of each)
 inline int few_waves(int K) { return K >= 1024 ? 8 : 4; }
 inline int few_rows(int K) { return few_waves(K) << (6 - lanes_log(K)); }
+// Where the product's blocks make the codes themselves, each wave does so for RW times its share of few_rows(K); 0: rows to
+// codes is a launch of its own.  launch_few takes RW from here, so that RW few_rows(K) >= T holds for what is launched.  They do
+// where that takes a wave four loads a lane at most: us in one launch and in two, 16 x 512 x 1024 6.2 and 6.2, 8 x 700 x 1024 7.1
+// and 7.2, 8 x 2048 x 1024 7.3 and 7.5, 32 x 128 x 8192 4.9 and 6.2, in a graph 8 x 1024 x 512 4.6 and 6.0, 12 x 1024 x 4096 5.8 and
+// 5.8, 16 x 1024 x 4096 6.4 and 5.8 (called from a program, that is a launch less); past that 32 x 512 x 1024 9.1 and 6.2, 16 x 700
+// x 1024 10.2 and 7.2, 1 x 4096 x 1024 10.2 and 9.1.
+inline int few_coded(long long T, int K) {
+    if (T < 1 || T > FEW || K < 1) return 0;
+    for (int rw = 1; rw <= 4 && rw * ((K - 1) / 512 + 1) <= 4; rw *= 2)
+        if (T <= rw * few_rows(K)) return rw;
+    return 0;
+}
 
 template <int FT, int FN, int WT, int WN, int GK, int D, int MW, int TYPE>
 void launch_gemm(GemmArgs a, hipStream_t st) {
@@ -925,9 +937,9 @@ int launch_fold(const void* y, int type, FoldArgs a, hipStream_t st) {
     });
 }
 
-// up to 32 tokens x (of type X), or codes of any number (X < 0)
+// up to 32 tokens x (of type X), or codes of any number (X < 0); false: no kernel makes the codes of so many
 template <int X, int Y>
-void launch_few(const FewArgs& f, hipStream_t st) {
+bool launch_few(const FewArgs& f, hipStream_t st) {
     const int K = f.g.K, codes = X < 0 ? 0 : (int)f.g.T * ((K + 31) / 32 * 32 + 16);
     const dim3 blocks((unsigned)((f.g.N + 31) / 32), X < 0 ? (unsigned)((f.g.T + 31) / 32) : 1u);
     // eight waves from K = 1024 on (us with 4, 8, 16: 1 x 8192 x 8192 16, 15, 15; 96 x 2048 x 2048 5.4, 4.8, 4.8; 64 x 4096 x
@@ -935,18 +947,23 @@ void launch_few(const FewArgs& f, hipStream_t st) {
     const auto go = [&](auto waves, auto rows) {
         constexpr int WV = waves.value;
         gemm_few_kernel<X, WV, rows.value, Y><<<blocks, 64 * WV, std::max(codes, WV * 4096), st>>>(f);
+        return true;
     };
     using std::integral_constant;
+    constexpr integral_constant<int, 4> four;
+    constexpr integral_constant<int, 8> eight;
+    constexpr integral_constant<int, 1> one;
     if constexpr (X < 0) {
-        if (few_waves(K) == 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-        else go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    } else if (K >= 1024) {
-        go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        return few_waves(K) == 8 ? go(eight, one) : go(four, one);
     } else {
-        const int rows = few_rows(K);
-        if (f.g.T <= rows) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-        else if (f.g.T <= 2 * rows) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-        else go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+        switch (few_waves(K) * 8 + few_coded(f.g.T, K)) {
+            case 4 * 8 + 1: return go(four, one);
+            case 4 * 8 + 2: return go(four, integral_constant<int, 2>{});
+            case 4 * 8 + 4: return go(four, integral_constant<int, 4>{});
+            case 8 * 8 + 1: return go(eight, one);
+            case 8 * 8 + 2: return go(eight, integral_constant<int, 2>{});
+            default: return false;
+        }
     }
 }
 
@@ -1040,6 +1057,8 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
     });
 }
 
+int pgan_linear_q8_rows(long long T, int K) { return few_coded(T, K) * few_rows(K < 1 ? 1 : K); }
+
 int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long ldq, float* q_scale, const void* w,
                    long long ldw, const float* w_scale, const float* bias, void* y, int y_type, long long ldy, long long T,
                    int N, int K, int lrelu, hipStream_t st) {
@@ -1049,16 +1068,16 @@ int pgan_linear_q8(const void* x, int x_type, long long ldx, void* q, long long 
         || !apart({rows_of(x, T, K, ldx, type_bytes(x_type)), rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1, true),
                    rows_of(q_scale, 1, T, 0, 4, true), rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
-    // The product's blocks make the codes where that takes a wave four loads a lane at most: us in one launch and in two,
-    // 16 x 512 x 1024 6.2 and 6.2, 8 x 700 x 1024 7.1 and 7.2, 8 x 2048 x 1024 7.3 and 7.5, 32 x 128 x 8192 4.9 and 6.2; past that
-    // 32 x 512 x 1024 9.1 and 6.2, 16 x 700 x 1024 10.2 and 7.2, 1 x 4096 x 1024 10.2 and 9.1.
-    if (T <= FEW && (T + few_rows(K) - 1) / few_rows(K) * ((K + 511) / 512) <= 4)
-        return by_type(x_type, [&](auto xt) {
+    if (few_coded(T, K)) {
+        bool launched = false;
+        const int rc = by_type(x_type, [&](auto xt) {
             (void)by_type(y_type, [&](auto t) {
                 const GemmArgs a{nullptr, nullptr, static_cast<const int8_t*>(w), w_scale, bias, y, 0, ldw, ldy, T, N, K, 0, 0, 0};
-                launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, lanes_log(K)}, st);
+                launched = launch_few<xt.value, t.value>(FewArgs{a, x, ldx, lrelu, lanes_log(K)}, st);
             });
         });
+        return launched ? rc : PGAN_EINVAL;
+    }
     const int rc = pgan_quant_rows(x, x_type, ldx, q, ldq, q_scale, T, K, lrelu, st);
     return rc ? rc : pgan_gemm_q8(q, ldq, q_scale, w, ldw, w_scale, bias, y, y_type, ldy, T, N, K, st);
 }

@@ -98,6 +98,7 @@ _SIGS = {
     "pgan_quant_rows": [P, I, L, P, L, P, L, I, I, P],
     "pgan_gemm_q8": [P, L, P, P, L, P, P, P, I, L, L, I, I, P],
     "pgan_linear_q8": [P, I, L, P, L, P, P, L, P, P, P, I, L, L, I, I, I, P],
+    "pgan_linear_q8_rows": [L, I],
     "pgan_up_fold_q8": [P, I, P, P, L, P, I, I, I, I, P],
     "pgan_up_fold": [P, I, P, P, I, I, I, I, I, P],
     "pgan_philox": [P, L, P, I, P],
@@ -204,7 +205,7 @@ class _Lib:
              "pgan_step_graph_destroy", "pgan_event_create", "pgan_event_destroy", "pgan_tape_destroy", "pgan_tape_arg_count",
              "pgan_tape_append", "pgan_tape_length", "pgan_tape_replay", "pgan_gn_onepass_workspace_bytes",
              "pgan_gn_onepass_workspace_init", "pgan_gn_onepass_workspace_error", "pgan_conv_down_h2_adds",
-             "pgan_conv_down_x3_adds")
+             "pgan_conv_down_x3_adds", "pgan_linear_q8_rows")
 
     def __init__(self, lib):
         self._real = lib

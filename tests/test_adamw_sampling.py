@@ -686,3 +686,28 @@ def test_calls_on_two_streams_at_once():
         torch.cuda.synchronize()
         for (_, _, results), w in zip(lanes, want):
             assert all(torch.equal(a, b) for a, b in zip(results(), w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("latent,n", [(1024, 12), (1024, 16), (1024, 8), (512, 16), (2048, 7), (16, 3)])
+def test_sampler_of_other_latent_sizes(latent, n):
+    """Draws of a few alignments from latent vectors of any multiple of 16: the first product from its definition, the sites
+    within the spread of the roundings."""
+    from pgan_engine import gen_buffer_shapes, gen_param_shapes
+    from pgan_hip import HipOps
+    from pgan_sampler import Sampler8
+    P = {k: v.to(DEV) for k, v in orc.make_params(gen_param_shapes(latent, 64), 31).items()}
+    rng = np.random.default_rng(31)
+    Bf = {}
+    for k, shape in gen_buffer_shapes(latent, 64).items():
+        x = torch.from_numpy(rng.standard_normal(shape).astype(np.float32))
+        Bf[k] = (x * 0.2 if k.endswith("mean") else 0.3 + x.abs()).to(DEV)
+    s = Sampler8(HipOps(DEV, max_samples=64), P, Bf, n, "sigmoid", latent)
+    z = torch.randn(n, latent, generator=torch.Generator().manual_seed(n))
+    sites, pos = s.draw(z.to(DEV))
+    q, qs = codes_of(z)
+    want = (q.double() @ s.w[0].cpu().double().t()) * (qs.double()[:, None] * s.ws[0].cpu().double()) + s.bias0.cpu().double()
+    tol = 4 * U * (want.abs() + 2 * s.bias0.cpu().double().abs())
+    within("y0", s.y[0][:n], want, tol + half_step(want.abs() + tol, torch.bfloat16))
+    near(sites, *eval64(P, Bf, z, s.n, "twod", "sigmoid"))
+    assert bool(torch.isfinite(pos).all())

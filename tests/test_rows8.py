@@ -534,3 +534,48 @@ def test_rows8_buffers(hip):
         b.fill_(2)
         hip.gemm_q8(b, s, w, ws, y)
         assert torch.equal(y, torch.full_like(y, 2.0 * K))
+
+
+def test_one_launch_codes_every_token():
+    """Where linear_q8 is one launch, each block's waves make the codes of at least as many rows as there are tokens (no GPU
+    needed: the rule that the launch is made by, over every K that a product takes and every T that it can hold)."""
+    import pgan_hip
+    rows = pgan_hip._lib.pgan_linear_q8_rows
+    one = set()
+    for K in list(range(1, 4200)) + [k for b in range(4096, 131072, 512) for k in (b + 511, b + 512, b + 513) if k <= 131072]:
+        for T in range(1, 41):
+            n = rows(T, K)
+            assert n == 0 or n >= T, (T, K, n)
+            if n:
+                one.add((T, K))
+    # both sides of each border are there
+    for T, K in ((1, 1), (32, 256), (16, 257), (16, 512), (8, 513), (8, 1023), (8, 1024), (8, 1025), (8, 2048)):
+        assert (T, K) in one, (T, K)
+    for T, K in ((33, 16), (17, 257), (17, 512), (9, 513), (9, 1023), (17, 1024), (9, 1025), (9, 2048), (1, 2049), (1, 131072)):
+        assert (T, K) not in one, (T, K)
+    assert rows(0, 16) == rows(-1, 16) == rows(1, 0) == rows(1, -5) == rows(1 << 40, 16) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [8, 16, 256, 257, 512, 513, 1000, 1023, 1024, 1025, 1536, 2048, 2049])
+@pytest.mark.parametrize("xt,yt", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_linear_q8_at_the_borders_of_one_launch(hip, K, xt, yt):
+    """Every number of tokens next to a border of the rule, bit for bit what rows to codes and the product give one after the
+    other, and that of the definition; what a block's LDS held before is other rows' codes and scales."""
+    rng = np.random.default_rng(K)
+    N = 70
+    _, w, _, ws, bias = product_case(K, 1, K, N)
+    w8, wsg, bg = rows8(w), ws.to(DEV), bias.to(DEV)
+    for T in (1, 4, 5, 7, 8, 9, 12, 15, 16, 17, 31, 32):
+        x = (rnd(rng, T, K) * torch.exp(2 * rnd(rng, T, 1))).to(xt)
+        xg, neg = x.to(DEV), T % 2 == 1
+        q, s = rows8(torch.zeros(T, K, dtype=torch.int8)), torch.zeros(T, device=DEV)
+        two, one = (torch.full((T + 1, N), 7.0, dtype=yt, device=DEV) for _ in range(2))
+        hip.quant_rows(xg, q, s, lrelu=neg)
+        hip.gemm_q8(q, s, w8, wsg, two[:T], bg)
+        hip.linear_q8(torch.full((32, K), 1e4, dtype=xt, device=DEV), w8, wsg, torch.empty(32, N, dtype=yt, device=DEV),
+                      rows8(torch.zeros(32, K, dtype=torch.int8)), torch.zeros(32, device=DEV))
+        hip.linear_q8(xg, w8, wsg, one[:T], rows8(torch.zeros(T, K, dtype=torch.int8)), torch.zeros(T, device=DEV), bg, lrelu=neg)
+        assert torch.equal(one, two), (T, K)
+        want, tol = product64(*codes_of(lrelu(x.float()) if neg else x.float()), w, ws, bias)
+        check_product(one[:T], want, tol, yt)

@@ -509,3 +509,46 @@ def test_steps_past_the_caches_equal_small_ones(hip, bits, pt, gt, n):
                 q = want.float().to(pt)
         within("m", st[0][0][0][e], m.double(), 4 * U * m.abs().double() + 1e-12)
         within("p", whole[0][e], want, 2 * tol + 3 * half_step(want.abs() + tol, pt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-20])
+def test_second_moments_among_the_denormals(hip, eps):
+    """Gradients whose squares leave fp32's normal range, an epsilon that does not hide it.  p starts at zero, so that what is
+    left is -size m / (sqrt(v) inv + eps) of the m and v that the GPU holds: 1 u each for size, its product, the root, inv, the
+    denominator, eps and the result, 2 u for the reciprocal (one unit off at most): 9 u, 10 are used."""
+    n, lr = 600, 1e-3
+    g = torch.from_numpy(np.exp(np.random.default_rng(5).uniform(math.log(1e-20), math.log(1e-15), n)).astype(np.float32))
+    g[::2] *= -1
+    d = dict(p=[torch.zeros(n)], g=[g], m=[torch.zeros(n)], v=[torch.zeros(n)], ms=[], rs=[])
+    gpu = {k: [t.to(DEV) for t in d[k]] for k in d}
+    for t in (1, 2):
+        gpu["p"][0].zero_()
+        hip.adamw(gpu["p"], gpu["g"], gpu["m"], gpu["v"], t, lr, B1, B2, eps, 0.0)
+        m, v = gpu["m"][0].cpu().double(), gpu["v"][0].cpu().double()
+        assert bool((v > 0).all()) and bool((v < 2.0 ** -126).any()) and bool((v > 2.0 ** -126).any())
+        # g^2, its product, v's product and their sum: half a denormal step each at most, and u of a normal one
+        within("v", v, (1 - B2) * (1 + (t - 1) * B2) * g.double() ** 2, 5 * U * v + t * 2.0 ** -148)
+        upd = lr / (1 - B1 ** t) * m / (v.sqrt() / math.sqrt(1 - B2 ** t) + eps)
+        within("p", gpu["p"][0], -upd, 10 * U * upd.abs())
+
+
+@pytest.mark.gpu
+def test_8_bit_roots_of_second_moments_among_the_denormals(hip):
+    """Blocks that hold nothing but such second moments: the codes are those of the format's definition, bit for bit."""
+    sizes = [256, 700, 2048]
+    rng = np.random.default_rng(9)
+    d = dict(p=[], g=[], m=[], v=[], ms=[], rs=[])
+    for n in sizes:
+        d["p"].append(torch.zeros(n))
+        d["g"].append(torch.from_numpy((rng.standard_normal(n) * 3e-19).astype(np.float32)))
+        for k in ("m", "v"):
+            d[k].append(torch.zeros(n, dtype=torch.uint8))
+        for k in ("ms", "rs"):
+            d[k].append(torch.zeros(-(-n // BLOCK)))
+    got = run(hip, d, 8, 1, seed=17)
+    for i, n in enumerate(sizes):
+        cm, cr, ms, rs = hold8(*states32(torch.zeros(n), torch.zeros(n), d["g"][i]), 17, 1, i)
+        assert torch.equal(got["ms"][i].cpu(), ms) and torch.equal(got["rs"][i].cpu(), rs)
+        assert torch.equal(got["m"][i].cpu(), cm) and torch.equal(got["v"][i].cpu(), cr)
+        assert len(set(cr.tolist())) > 20

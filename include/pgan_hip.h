@@ -265,7 +265,7 @@ int pgan_adam(float* p, const float* g, float* m, float* v, long long n, float l
  * m_scale / r_scale one power of two for every 256 elements (codes and scales of zeros are a fresh state); codes are rounded
  * stochastically from a hash of (seed, step, tensor's number, element).  Elements past a tensor's last one are left alone.
  * Refused (-1): a written buffer that shares memory with another one or with a gradient, pointers that are not aligned to
- * their element.
+ * their element, an eps that is neither 0 nor at least 2^-126 (fp32's normal numbers).
  * step_dev: NULL (step >= 1 is the number of this step), or 4 device ints: [0] is incremented and used, [1] and [2] get the
  * corrections 1 / (1 - b1^t) and 1 / sqrt(1 - b2^t) as fp32 -- a captured graph then counts on every replay.
  * grad_scale as in pgan_adam.  (src/train_wgan_v2.py:489-490,612,634 step torch.optim.Adam.) */

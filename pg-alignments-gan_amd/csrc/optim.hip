@@ -431,7 +431,8 @@ int pgan_adamw_multi(void* const* p, const void* const* g, void* const* m, void*
                      float* const* r_scale, const long long* numel, const int* types, const double* lr,
                      const double* decay, int n, int bits, double b1, double b2, float eps, float grad_scale, int seed,
                      int* step_dev, int step, hipStream_t st) {
-    if (n < 0 || (bits != 32 && bits != 8) || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1) || !(eps >= 0)) return PGAN_EINVAL;
+    if (n < 0 || (bits != 32 && bits != 8) || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1)) return PGAN_EINVAL;
+    if (!(eps == 0 || eps >= 0x1p-126f)) return PGAN_EINVAL;     // the hardware's reciprocal takes denormals for zero
     if (!step_dev && step < 1) return PGAN_EINVAL;
     if (n > 0 && (!p || !g || !m || !v || !numel || !types || !lr || !decay)) return PGAN_EINVAL;
     if (bits == 8 && n > 0 && (!m_scale || !r_scale)) return PGAN_EINVAL;

@@ -416,6 +416,7 @@ def _hw(t: torch.Tensor) -> int:
 
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # type codes of the C-ABI
 ADAMW_BLOCK = 256      # elements of an 8-bit AdamW state that share a scale
+ADAMW_LEAST_EPS = 2.0 ** -126      # besides zero: the hardware's reciprocal takes denormals for zero
 
 
 def rows8(rows: int, cols: int, device) -> torch.Tensor:
@@ -507,6 +508,8 @@ class AdamWPlan:
             sd = step_dev.data_ptr()
         elif step < 1:
             raise PganError(f"adamw: steps count from 1, got {step}")
+        if not (eps == 0 or eps >= ADAMW_LEAST_EPS):
+            raise PganError(f"adamw: eps must be 0 or at least {ADAMW_LEAST_EPS}, got {eps}")
         _check(_lib.pgan_adamw_multi(self._p, self._pt(*map(T.data_ptr, grads)), self._m, self._v, self._ms, self._rs, self._numel, self._types[1],
                                      self._rates[2], self._rates[3], self.n, self.bits, b1, b2, eps, grad_scale,
                                      (seed + (1 << 31)) % (1 << 32) - (1 << 31), sd, int(step), ops._own_stream()),

@@ -14,7 +14,7 @@ import copy
 
 import torch
 
-from pgan_hip import ADAMW_BLOCK, PganError
+from pgan_hip import ADAMW_BLOCK, ADAMW_LEAST_EPS, PganError
 
 _STATE = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
@@ -31,6 +31,8 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0, capturable=False):
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:
             raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps} and {weight_decay}")
+        if not (eps == 0 or eps >= ADAMW_LEAST_EPS):
+            raise ValueError(f"eps must be 0 or at least {ADAMW_LEAST_EPS}, got {eps}")
         if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         if state_bits not in _STATE:

@@ -552,3 +552,33 @@ def test_8_bit_roots_of_second_moments_among_the_denormals(hip):
         assert torch.equal(got["ms"][i].cpu(), ms) and torch.equal(got["rs"][i].cpu(), rs)
         assert torch.equal(got["m"][i].cpu(), cm) and torch.equal(got["v"][i].cpu(), cr)
         assert len(set(cr.tolist())) > 20
+
+
+def test_an_epsilon_among_the_denormals_is_refused():
+    """(No GPU needed.)  The reciprocal takes such a denominator for zero: an element without a gradient would become NaN."""
+    import pgan_hip
+    from pgan_optim import AdamW
+    P, LL, I, D = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_double
+    one = lambda t, x: (t * 1)(x)
+    for eps in (1e-45, 1e-39, 2.0 ** -127, math.inf * -1):
+        assert pgan_hip._lib._real.pgan_adamw_multi(one(P, 4096), one(P, 1 << 16), one(P, 1 << 20), one(P, 1 << 21), None, None, one(LL, 100), one(I, 0),
+                                                    one(D, 1e-3), one(D, 0.0), 1, 32, 0.5, 0.999, eps, 1.0, 0, None, 1, None) == -1
+        with pytest.raises(ValueError):
+            AdamW([torch.nn.Parameter(torch.zeros(3))], eps=eps)
+    AdamW([torch.nn.Parameter(torch.zeros(3))], eps=2.0 ** -126)
+
+
+@pytest.mark.gpu
+def test_the_least_epsilon(hip):
+    """Elements without a gradient stay where they are, at the smallest epsilon that is taken; at zero they are 0 / 0."""
+    from pgan_hip import PganError
+    g = torch.zeros(300, device=DEV)
+    g[::3] = 1e-3
+    for eps in (2.0 ** -126, 0.0):
+        p, m, v = torch.ones(300, device=DEV), torch.zeros(300, device=DEV), torch.zeros(300, device=DEV)
+        hip.adamw([p], [g], [m], [v], 1, 1e-3, B1, B2, eps, 0.0)
+        still = p.cpu()[g.cpu() == 0]
+        assert bool((still == 1).all()) if eps else bool(torch.isnan(still).all())
+        within("p", p.cpu()[::3], torch.full((100,), 1 - 1e-3, dtype=torch.float64), torch.full((100,), 16 * U * 1e-3 + 4 * U, dtype=torch.float64))
+    with pytest.raises(PganError):
+        hip.adamw([p], [g], [m], [v], 1, 1e-3, B1, B2, 1e-39, 0.0)

@@ -16,6 +16,15 @@ import torch
 
 from pgan_hip import ADAMW_BLOCK, ADAMW_LEAST_EPS, PganError
 
+def _honoured(group) -> None:
+    """Refuses a group's options (torch's names) that step() would have to pass over."""
+    for name in ("maximize", "amsgrad", "differentiable"):
+        if group.get(name):
+            raise ValueError(f"AdamW: {name} is not supported")
+    if group.get("decoupled_weight_decay") is False and group.get("weight_decay"):
+        raise ValueError("AdamW: the weight decay of these groups is part of the gradient (torch.optim.Adam's), here it is decoupled")
+
+
 _STATE = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
 
@@ -25,6 +34,7 @@ class AdamW(torch.optim.Optimizer):
 
     state: per parameter `step`, `exp_avg` and `exp_avg_sq` -- float32, or with state_bits=8 float8_e4m3fn codes of the first
     moment and of the root of the second, with their scales in `exp_avg_scale` and `exp_avg_sq_scale`.
+    torch's amsgrad, maximize, differentiable and a decay that is part of the gradient are refused, in groups and loaded states.
     capturable: the steps are counted on the device, so that a captured graph counts on every replay; every parameter of a
     group then needs a gradient in every step.  Without it a step refuses to be captured."""
 
@@ -44,6 +54,10 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plans = {}
+
+    def add_param_group(self, param_group):
+        _honoured(param_group)
+        super().add_param_group(param_group)
 
     @staticmethod
     def _layout(p, bits):
@@ -141,6 +155,7 @@ class AdamW(torch.optim.Optimizer):
         saved, held = state_dict["state"], dict(self.state)
         counters = [g.get("counter") for g in self.param_groups]
         for own, g in zip(self.param_groups, state_dict["param_groups"]):      # before anything is changed
+            _honoured(g)
             for i, p in zip(g["params"], own["params"]):
                 b = g.get("state_bits", self.defaults["state_bits"])
                 for name, (dtype, n) in self._layout(p, b).items() if i in saved else ():

@@ -711,3 +711,33 @@ def test_sampler_of_other_latent_sizes(latent, n):
     within("y0", s.y[0][:n], want, tol + half_step(want.abs() + tol, torch.bfloat16))
     near(sites, *eval64(P, Bf, z, s.n, "twod", "sigmoid"))
     assert bool(torch.isfinite(pos).all())
+
+
+@pytest.mark.parametrize("other,options", [("AdamW", dict(maximize=True)), ("AdamW", dict(amsgrad=True)), ("AdamW", dict(differentiable=True)),
+                                           ("Adam", dict(weight_decay=0.1)), ("Adam", dict(maximize=True))])
+def test_options_that_a_step_would_pass_over_are_refused(other, options):
+    """A state of torch's whose step would be another one here; nothing changes.  (No GPU needed.)"""
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5))
+    p.grad = torch.ones(5)
+    ref = getattr(torch.optim, other)([p], lr=0.125, **options)
+    if not options.get("differentiable"):
+        ref.step()
+    opt = AdamW([p], lr=0.25)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and len(opt.state) == 0 and "maximize" not in opt.param_groups[0]
+    if other == "AdamW":
+        with pytest.raises(ValueError):
+            AdamW([dict(params=[p], **options)])
+
+
+def test_states_of_adam_without_a_decay_are_taken():
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5))
+    p.grad = torch.ones(5)
+    ref = torch.optim.Adam([p], lr=0.125)
+    ref.step()
+    opt = AdamW([p])
+    opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.125 and opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], ref.state[p]["exp_avg"])

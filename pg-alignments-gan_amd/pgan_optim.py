@@ -166,6 +166,8 @@ class AdamW(torch.optim.Optimizer):
         for g in self.param_groups:     # options that another AdamW's groups do not have
             for k, v in self.defaults.items():
                 g.setdefault(k, v)
+            if "decoupled_weight_decay" in g:
+                g["decoupled_weight_decay"] = True
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ps = [p for g in self.param_groups for p in g["params"]]
         bits = [g["state_bits"] for g in self.param_groups for _ in g["params"]]

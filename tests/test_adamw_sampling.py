@@ -741,3 +741,18 @@ def test_states_of_adam_without_a_decay_are_taken():
     opt = AdamW([p])
     opt.load_state_dict(ref.state_dict())
     assert opt.param_groups[0]["lr"] == 0.125 and opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], ref.state[p]["exp_avg"])
+
+
+def test_a_decay_given_after_adams_states_were_taken():
+    """Its own saved state goes back in.  (No GPU needed.)"""
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5))
+    p.grad = torch.ones(5)
+    ref = torch.optim.Adam([p], lr=0.125)
+    ref.step()
+    opt = AdamW([p])
+    opt.load_state_dict(ref.state_dict())
+    opt.param_groups[0]["weight_decay"] = 0.25
+    again = AdamW([p])
+    again.load_state_dict(opt.state_dict())
+    assert again.param_groups[0]["weight_decay"] == 0.25

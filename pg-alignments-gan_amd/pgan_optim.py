@@ -10,11 +10,12 @@ All tensors of a group are stepped in one launch per forty tensors (HipOps.adamw
 """
 from __future__ import annotations
 
-import copy
-
 import torch
 
 from pgan_hip import ADAMW_BLOCK, ADAMW_LEAST_EPS, PganError
+
+_STATE = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
+
 
 def _honoured(group) -> None:
     """Refuses a group's options (torch's names) that step() would have to pass over."""
@@ -23,9 +24,6 @@ def _honoured(group) -> None:
             raise ValueError(f"AdamW: {name} is not supported")
     if group.get("decoupled_weight_decay") is False and group.get("weight_decay"):
         raise ValueError("AdamW: the weight decay of these groups is part of the gradient (torch.optim.Adam's), here it is decoupled")
-
-
-_STATE = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
 
 class AdamW(torch.optim.Optimizer):
@@ -151,10 +149,26 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """States keep the types they are held in (torch's own loading would cast codes and scales to the parameter's) and, where
         they are there already, their memory: a captured step goes on from what was loaded."""
-        state_dict = copy.copy(state_dict)
-        saved, held = state_dict["state"], dict(self.state)
-        counters = [g.get("counter") for g in self.param_groups]
-        for own, g in zip(self.param_groups, state_dict["param_groups"]):      # before anything is changed
+        had = {}
+
+        def take(_, state_dict):        # the last of the hooks before: torch loads the groups alone
+            had.update(saved=self._checked(state_dict), held=dict(self.state), counters=[g.get("counter") for g in self.param_groups],
+                       ids=[i for g in state_dict["param_groups"] for i in g["params"]])
+            return {**state_dict, "state": {}}
+
+        def give(_):                    # the first of those after
+            self._take_over(**had)
+        hooks = [self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(give, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _checked(self, state_dict):
+        """The saved states, refused before anything is changed if they do not fit."""
+        saved = state_dict["state"]
+        for own, g in zip(self.param_groups, state_dict["param_groups"]):
             _honoured(g)
             for i, p in zip(g["params"], own["params"]):
                 b = g.get("state_bits", self.defaults["state_bits"])
@@ -162,13 +176,14 @@ class AdamW(torch.optim.Optimizer):
                     t = saved[i].get(name)
                     if t is None or t.dtype != dtype or t.numel() != n:
                         raise ValueError(f"AdamW: the saved state holds no {name} of {n} elements in {dtype}")
-        super().load_state_dict({**state_dict, "state": {}})
+        return saved
+
+    def _take_over(self, saved, held, counters, ids):
         for g in self.param_groups:     # options that another AdamW's groups do not have
             for k, v in self.defaults.items():
                 g.setdefault(k, v)
             if "decoupled_weight_decay" in g:
                 g["decoupled_weight_decay"] = True
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ps = [p for g in self.param_groups for p in g["params"]]
         bits = [g["state_bits"] for g in self.param_groups for _ in g["params"]]
         loaded = {}

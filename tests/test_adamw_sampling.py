@@ -756,3 +756,34 @@ def test_a_decay_given_after_adams_states_were_taken():
     again = AdamW([p])
     again.load_state_dict(opt.state_dict())
     assert again.param_groups[0]["weight_decay"] == 0.25
+
+
+def test_load_hooks_see_and_may_change_the_states():
+    """torch's hooks around load_state_dict: the one before gets the saved states and what it makes of them is loaded, the one
+    after finds them in place.  (No GPU needed.)"""
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5))
+    p.grad = torch.ones(5)
+    ref = torch.optim.AdamW([p], lr=0.125)
+    ref.step()
+    opt, seen = AdamW([p]), []
+
+    def before(o, sd):
+        seen.append(sorted(sd["state"][0]))
+        st = {0: {**sd["state"][0], "exp_avg": sd["state"][0]["exp_avg"] * 2}}
+        return {**sd, "state": st}
+
+    def after(o):
+        seen.append((o.state[p]["step"], o.state[p]["exp_avg"].clone()))
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(after)
+    saved = ref.state_dict()
+    opt.load_state_dict(saved)
+    opt.load_state_dict(saved)                       # once each time
+    assert seen[0] == seen[2] == ["exp_avg", "exp_avg_sq", "step"] and seen[1][0] == 1 and len(seen) == 4
+    assert torch.equal(seen[1][1], 2 * ref.state[p]["exp_avg"]) and torch.equal(opt.state[p]["exp_avg"], 2 * ref.state[p]["exp_avg"])
+    with pytest.raises(ValueError):                  # a hook's states are checked as any
+        bad = AdamW([p])
+        bad.register_load_state_dict_pre_hook(lambda o, sd: {**sd, "state": {0: {"step": 1}}})
+        bad.load_state_dict(saved)
+    assert len(bad.state) == 0

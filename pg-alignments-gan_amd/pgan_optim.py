@@ -153,6 +153,7 @@ class AdamW(torch.optim.Optimizer):
 
         def take(_, state_dict):        # the last of the hooks before: torch loads the groups alone
             had.update(saved=self._checked(state_dict), held=dict(self.state), counters=[g.get("counter") for g in self.param_groups],
+                       own=[{k: g[k] for k in self.defaults} for g in self.param_groups],
                        ids=[i for g in state_dict["param_groups"] for i in g["params"]])
             return {**state_dict, "state": {}}
 
@@ -171,16 +172,16 @@ class AdamW(torch.optim.Optimizer):
         for own, g in zip(self.param_groups, state_dict["param_groups"]):
             _honoured(g)
             for i, p in zip(g["params"], own["params"]):
-                b = g.get("state_bits", self.defaults["state_bits"])
+                b = g.get("state_bits", own["state_bits"])
                 for name, (dtype, n) in self._layout(p, b).items() if i in saved else ():
                     t = saved[i].get(name)
                     if t is None or t.dtype != dtype or t.numel() != n:
                         raise ValueError(f"AdamW: the saved state holds no {name} of {n} elements in {dtype}")
         return saved
 
-    def _take_over(self, saved, held, counters, ids):
-        for g in self.param_groups:     # options that another AdamW's groups do not have
-            for k, v in self.defaults.items():
+    def _take_over(self, saved, held, counters, own, ids):
+        for g, options in zip(self.param_groups, own):      # those that another AdamW's groups do not have stay
+            for k, v in options.items():
                 g.setdefault(k, v)
             if "decoupled_weight_decay" in g:
                 g["decoupled_weight_decay"] = True

@@ -787,3 +787,22 @@ def test_load_hooks_see_and_may_change_the_states():
         bad.register_load_state_dict_pre_hook(lambda o, sd: {**sd, "state": {0: {"step": 1}}})
         bad.load_state_dict(saved)
     assert len(bad.state) == 0
+
+
+def test_groups_keep_options_that_a_loaded_state_does_not_name():
+    """torch's states know neither bits nor seeds: each group's own stay, not the constructor's.  (No GPU needed.)"""
+    from pgan_optim import AdamW
+    a, b = torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(6))
+    a.grad, b.grad = torch.ones(5), torch.ones(6)
+    ref = torch.optim.AdamW([dict(params=[a]), dict(params=[b])], lr=0.125)
+    ref.step()
+    opt = AdamW([dict(params=[a], seed=5), dict(params=[b])], seed=9)
+    opt.load_state_dict(ref.state_dict())
+    assert [g["seed"] for g in opt.param_groups] == [5, 9] and [g["lr"] for g in opt.param_groups] == [0.125, 0.125]
+    opt = AdamW([dict(params=[a], state_bits=8), dict(params=[b])])
+    with pytest.raises(ValueError):                  # states of 32 bits for a group that holds 8
+        opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["state_bits"] == 8
+    opt = AdamW([dict(params=[a], state_bits=32), dict(params=[b], state_bits=32)], state_bits=8)
+    opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["state_bits"] == 32 and opt.state[a]["exp_avg"].dtype == torch.float32

@@ -48,10 +48,11 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       seed=seed, capturable=capturable))
         self._plans = {}                # (group, steps made): plan and what it was made of
+        self._recorded = []             # plans and counters of captured steps: their graphs write to this memory
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans = {}
+        self._plans, self._recorded = {}, getattr(self, "_recorded", [])
 
     def add_param_group(self, param_group):
         _honoured(param_group)
@@ -120,6 +121,8 @@ class AdamW(torch.optim.Optimizer):
                     counter = group["counter"] = torch.tensor([next(iter(by_step)), 0, 0, 0], dtype=torch.int32, device=ps[0].device)
             for k, (made, members) in enumerate(sorted(by_step.items(), key=lambda kv: kv[0])):
                 plan = self._plan((gi, k), members, group["state_bits"])
+                if capturing:
+                    self._recorded.append((plan, counter))
                 grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in members]
                 with torch.cuda.device(members[0].device):
                     plan.step(grads, made + 1, float(group["lr"]), group["betas"][0], group["betas"][1], group["eps"],
@@ -202,11 +205,11 @@ class AdamW(torch.optim.Optimizer):
             self.state[p][name].view(torch.uint8).copy_(t.contiguous().view(torch.uint8))
         for group, counter in zip(self.param_groups, counters):
             steps = {self.state[p]["step"] for p in group["params"] if p in self.state}
-            if counter is not None and len(steps) == 1 and group["capturable"]:
+            group.pop("counter", None)
+            if counter is not None and len(steps) == 1:         # a captured step reads it, whatever these groups say
                 counter.copy_(torch.tensor([steps.pop(), 0, 0, 0], dtype=torch.int32))
-                group["counter"] = counter
-            else:
-                group.pop("counter", None)
+                if group["capturable"]:
+                    group["counter"] = counter
         self._plans = {}
 
 

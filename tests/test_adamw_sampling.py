@@ -806,3 +806,71 @@ def test_groups_keep_options_that_a_loaded_state_does_not_name():
     opt = AdamW([dict(params=[a], state_bits=32), dict(params=[b], state_bits=32)], state_bits=8)
     opt.load_state_dict(ref.state_dict())
     assert opt.param_groups[0]["state_bits"] == 32 and opt.state[a]["exp_avg"].dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_after_loading_a_state_that_is_not_capturable(bits):
+    """Its counter and states stay allocated, and it counts on from what was loaded: replays equal numbered steps, and what is
+    allocated after the load is left alone."""
+    from pgan_optim import AdamW
+    torch.manual_seed(6)
+    start = torch.randn(700, device=DEV)
+    grads = [torch.randn(700, device=DEV) for _ in range(6)]
+    p = torch.nn.Parameter(start.clone())
+    p.grad = torch.zeros_like(p)
+    kw = dict(lr=1e-2, betas=(B1, B2), eps=EPS, state_bits=bits, seed=3)
+    plain = AdamW([p], **kw)
+    for g in grads[:3]:
+        p.grad.copy_(g)
+        plain.step()
+    saved, at = copy.deepcopy(plain.state_dict()), p.detach().clone()
+    for g in grads[3:5]:
+        p.grad.copy_(g)
+        plain.step()
+    want = [p.detach().clone()] + [t.clone() for k, t in plain.state[p].items() if k != "step"]
+    p.data.copy_(start)
+    opt = AdamW([p], capturable=True, **kw)
+    p.grad.copy_(grads[0])
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(saved)
+    assert not opt.param_groups[0]["capturable"]
+    p.data.copy_(at)
+    torch.cuda.synchronize()
+    junk = [torch.full((4,), 7, dtype=torch.int32, device=DEV) for _ in range(512)] + [torch.full((700,), 7, dtype=torch.int32, device=DEV) for _ in range(32)]
+    for g in grads[3:5]:
+        p.grad.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in junk)
+    got = [p.detach()] + [t for k, t in opt.state[p].items() if k != "step"]
+    if bits == 8:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got[1:], want[1:]))
+    # the corrections pass through fp32 on the device: two roundings of each update, |update| < 8 lr here
+    assert float((got[0] - want[0]).abs().max()) <= 2 * (1e-2 * 8 * 8 * U + 4 * U * 5)
+
+
+@pytest.mark.gpu
+def test_states_of_a_captured_step_stay_allocated():
+    """A load that brings no states takes the optimizer's away, not the memory that the captured step writes to."""
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.randn(900, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], capturable=True)
+    none = copy.deepcopy(opt.state_dict())
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(none)
+    assert len(opt.state) == 0
+    torch.cuda.synchronize()
+    junk = [torch.full((900,), 7, dtype=torch.int32, device=DEV) for _ in range(64)] + [torch.full((4,), 7, dtype=torch.int32, device=DEV) for _ in range(512)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in junk)
+    opt.step()                                       # starts anew
+    assert int(opt.param_groups[0]["counter"][0]) == 1

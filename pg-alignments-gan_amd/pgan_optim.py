@@ -97,6 +97,9 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError("AdamW: a captured step needs capturable=True (the step's number would be recorded)")
             if group["capturable"] and len(ps) != len(group["params"]):
                 raise RuntimeError("AdamW: with capturable=True every parameter of a group needs a gradient in every step")
+            if group.get("counter") is not None and not group["capturable"]:
+                self._read_counters()   # numbered steps from here on
+                group.pop("counter")
             by_step = {}                # parameters that have been stepped equally often
             for p in ps:
                 if p.grad.is_sparse:

@@ -874,3 +874,20 @@ def test_states_of_a_captured_step_stay_allocated():
     assert all(bool((t == 7).all()) for t in junk)
     opt.step()                                       # starts anew
     assert int(opt.param_groups[0]["counter"][0]) == 1
+
+
+@pytest.mark.gpu
+def test_a_group_that_stops_counting_on_the_device():
+    """The steps made so far count on, in numbered steps and, after another change, on the device again."""
+    from pgan_optim import AdamW
+    p = torch.nn.Parameter(torch.randn(300, device=DEV))
+    opt = AdamW([p], lr=1e-2, betas=(B1, B2), eps=EPS, weight_decay=0.0, capturable=True)
+    for k in range(6):
+        opt.param_groups[0]["capturable"] = k not in (3, 4)
+        p.grad = torch.randn(300, device=DEV)
+        m, v = (opt.state[p][n].cpu().clone() if k else torch.zeros(300) for n in ("exp_avg", "exp_avg_sq"))
+        p0 = p.detach().cpu().clone()
+        opt.step()
+        want, _, _, _, tol = step64(p0, p.grad.cpu(), m, v, k + 1, 1e-2, 0.0)
+        within(f"step {k + 1}", p.detach(), want, tol)
+    assert opt.state_dict()["state"][0]["step"] == 6

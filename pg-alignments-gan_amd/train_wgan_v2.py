@@ -394,12 +394,17 @@ def plotting_forward(trainer, normalize, n=1000):
 
 def draw_alignments(trainer, n, normalize, batch=250):
     """n genotyped alignments of the generator as it stands, in evaluation and with 8-bit products (pgan_sampler), as
-    packed bits [n, 512] and positions [n, 64] (alignment_slab's format)."""
+    packed bits [n, 512] and positions [n, 64] (alignment_slab's format).  The latent vectors come from a generator of the
+    trainer's own, seeded from the run's seed; further calls go on in it."""
     import alignment_slab
+    gen = getattr(trainer, "_draw_gen", None)
+    if gen is None:
+        gen = trainer._draw_gen = torch.Generator(device=trainer.dev)
+        gen.manual_seed(trainer.seed + 7)
     sampler = trainer.sampler8(min(n, batch))
     bits, pos = [], []
     for lo in range(0, n, batch):
-        s, p = sampler.draw(torch.randn(min(batch, n - lo), trainer.eng.latent, device=trainer.dev))
+        s, p = sampler.draw(torch.randn(min(batch, n - lo), trainer.eng.latent, device=trainer.dev, generator=gen))
         if normalize:
             s, p = s / 2 + 0.5, p / 2 + 0.5
         g = sample_genotypes_bernoulli(s.clamp(0, 1))

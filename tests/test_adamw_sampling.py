@@ -891,3 +891,26 @@ def test_a_group_that_stops_counting_on_the_device():
         want, _, _, _, tol = step64(p0, p.grad.cpu(), m, v, k + 1, 1e-2, 0.0)
         within(f"step {k + 1}", p.detach(), want, tol)
     assert opt.state_dict()["state"][0]["step"] == 6
+
+
+@pytest.mark.gpu
+def test_drawn_alignments_follow_the_runs_seed():
+    """Whatever the global generator went through before; a second draw of the same trainer is another one."""
+    import train_wgan_v2 as tw
+
+    def draws(seed, before):
+        tr = make_trainer()
+        tr.seed = seed
+        tw.set_genotype_sampler(tr.ops, seed + 6)
+        torch.manual_seed(before)
+        torch.randn(before, device=DEV)
+        first = tw.draw_alignments(tr, 21, False, batch=8)
+        torch.manual_seed(before)
+        return first, tw.draw_alignments(tr, 21, False, batch=8)
+    try:
+        a, b, c = draws(77, 5), draws(77, 900), draws(78, 5)
+    finally:
+        tw._GENOTYPE_RNG.clear()
+    for x, y in zip(a, b):
+        assert np.array_equal(x[0], y[0]) and np.array_equal(x[1], y[1])
+    assert not np.array_equal(a[0][1], a[1][1]) and not np.array_equal(a[0][1], c[0][1])

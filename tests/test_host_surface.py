@@ -184,3 +184,12 @@ def test_library_states_its_build():
     lib = ctypes.CDLL(pgan_hip.LIB_PATH)
     lib.pgan_build_info.restype = ctypes.c_char_p
     assert b"packed-fp32-ops=off" in lib.pgan_build_info()
+
+
+def test_build_takes_its_former_argument():
+    """build(force=True) and `__graft_entry__.py --force` (tools/ab_pk.sh): every call compiles everything either way."""
+    import inspect
+    import __graft_entry__ as entry
+    inspect.signature(entry.build).bind()
+    inspect.signature(entry.build).bind(True)
+    inspect.signature(entry.build).bind(force=True)

@@ -680,8 +680,8 @@ __device__ __forceinline__ Taps taps_of(unsigned pix, int H, int W, int C) {
     t.at[1][1] = hok && wok ? ((rb + w2) * 16 + kb * 4 + lb) * C : -1;
     return t;
 }
-// of the eight channels from c on, or of the only n < 8
-template <int TYPE>
+// of the eight channels from c on, or of the only n < 8; NT: taps read past the caches
+template <int TYPE, bool NT = true>
 __device__ __forceinline__ void fold8(const typename Elem<TYPE>::type* y, const Taps& t, int c, int n, const float* shift, float (&v)[8]) {
     float p[2][2][8];
 #pragma unroll
@@ -692,7 +692,7 @@ __device__ __forceinline__ void fold8(const typename Elem<TYPE>::type* y, const 
             for (int e = 0; e < 8; ++e) p[i][j][e] = 0.f;
             if (t.at[i][j] < 0) continue;
             if (n < 8) load_few<TYPE>(y + t.at[i][j], n, p[i][j]);
-            else load8<TYPE, true>(y + t.at[i][j] + c, p[i][j]);
+            else load8<TYPE, NT>(y + t.at[i][j] + c, p[i][j]);
         }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (p[0][0][e] + p[1][0][e]) + (p[0][1][e] + p[1][1][e]);
@@ -765,7 +765,9 @@ __global__ __launch_bounds__(256) void up_fold_kernel(const typename Elem<TYPE>:
     }
 }
 
-// more than 512 channels: one output pixel a wave, codes in two passes
+// More than 512 channels: one output pixel a wave, codes in two passes, of which only the second reads past the caches: 200 x 8 x
+// 8 x 700 in bf16 101 us (133 with both past them, 103 with neither), in fp32 157 (249, 146), 16 x 16 x 16 x 8000 in bf16 402 (446,
+// 457).  HBM and the second read of the taps: 3.2 TB/s of needed bytes where 400 x 8 x 8 x 512 in one pass makes 5.5.
 template <int TYPE, bool Q8>
 __global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<TYPE>::type* __restrict__ y, const FoldArgs a) {
     const unsigned pix = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -776,7 +778,7 @@ __global__ __launch_bounds__(256) void up_fold_wide_kernel(const typename Elem<T
     if constexpr (Q8) {
         uint32_t mx = 0;
         for (int c = l8; c < C; c += 512) {
-            fold8<TYPE>(y, t, min(c, C - 8), C, a.shift, v);
+            fold8<TYPE, false>(y, t, min(c, C - 8), C, a.shift, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) mx = max(mx, magnitude(slope(v[e], true)));
         }

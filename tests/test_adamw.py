@@ -582,3 +582,27 @@ def test_the_least_epsilon(hip):
         within("p", p.cpu()[::3], torch.full((100,), 1 - 1e-3, dtype=torch.float64), torch.full((100,), 16 * U * 1e-3 + 4 * U, dtype=torch.float64))
     with pytest.raises(PganError):
         hip.adamw([p], [g], [m], [v], 1, 1e-3, B1, B2, 1e-39, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b2,steps", [(0.9, 120), (0.99, 900)])
+def test_the_8_bit_second_moment_over_many_steps(hip, b2, steps):
+    """Gradients of variance 1: the mean V of the held root's square, which is what the next step starts from.  A rounding that is
+    unbiased in the root adds its variance to the square, so V is no less than what 32 bits give, 1 - b2^t.  Nor is it much more:
+    a rounded root stands on a code, the next step moves it by d = |sqrt(b2 r^2 + c2 g^2) - r| <= c2 |g^2 - r^2| / (2 r) (1 + c2),
+    two neighbouring codes are at most s <= r / 8 apart, and rounding between them has a variance of at most d s, in the mean at
+    most c2 (1 + c2) (1 + V) / 16.  With V = b2 V + c2 + that, k = (1 + c2) / 16: V <= (1 + k) / (1 - k), that is 1.16 for b2 =
+    0.9 and 1.14 for 0.99.  Over n elements the mean is off by five times spread / sqrt(n) at most, a root that spreads by a
+    half of itself and so a square by its whole included."""
+    n = 1 << 16
+    z = lambda k, dt: torch.zeros(k, dtype=dt, device=DEV)
+    p, m, v, ms, rs = z(n, torch.float32), z(n, torch.uint8), z(n, torch.uint8), z(n // BLOCK, torch.float32), z(n // BLOCK, torch.float32)
+    f8 = lambda x: x.view(torch.float8_e4m3fn)
+    plan = hip.adamw_plan([p], [f8(m)], [f8(v)], scales=([ms], [rs]))
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    for t in range(1, steps + 1):
+        plan.step([torch.randn(n, device=DEV, generator=gen)], t, 1e-3, 0.9, b2, EPS, 0.0, seed=21)
+    mean = float(values8(v.cpu(), rs.cpu()).double().square().mean())
+    k, slack = (2 - b2) / 16, 5 / math.sqrt(n)
+    print("second moment", mean)
+    assert (1 - b2 ** steps) - slack <= mean <= (1 + k) / (1 - k) + slack

@@ -348,7 +348,8 @@ int pgan_gemm(const float* A, const float* B, float* C, int M, int N, int K, int
  * pgan_gemm_q8: y[t][n] = q_scale[t] w_scale[n] sum_k q[t][k] w[n][k] + bias[n] (bias may be NULL), K <= 131072.  Rows of q
  *   and w start on 16-byte borders (base and stride) and are readable up to the next multiple of 16 past K; what stands
  *   there does not matter.
- * pgan_linear_q8: both, through the caller's q (T rows of stride ldq) and q_scale.
+ * pgan_linear_q8: both.  q (T rows of stride ldq) and q_scale are scratch of the caller: what they hold afterwards is not
+ *   specified (one launch for few tokens leaves them as they were).
  * pgan_linear_q8_rows (no launch): 0 where pgan_linear_q8 makes the codes of T rows of K elements in a launch of its own;
  *   else it is one launch, and this the number of rows (at least T) whose codes each of its blocks can make.
  * pgan_up_fold_q8 / pgan_up_fold: the end of ConvTranspose2d(k 4, stride 2, padding 1) (src/layers.py:97-115) made as a

@@ -133,8 +133,9 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[8], floa
 // ---- rows to codes ------------------------------------------------------------------------------------------------
 // 2^log lanes a row, whose values stay in their registers between the maximum and the codes: 8 NIT each, K <= 8 NIT 2^log; a
 // lane has R rows, to have more bytes on their way.  A lane takes eight neighbouring elements at a time, the one at the row's
-// end its last eight, some of them its neighbour's too.  Bound by HBM (2 + 1 bytes an element of 16 bits; 16000 x 512 from
-// memory: 8.3 us, 3 TB/s, launch and one trip to memory half of it).
+// end its last eight, some of them its neighbour's too.  Bound by HBM (2 + 1 bytes an element of 16 bits; 16000 x 512: 6.2 us where
+// the same rows are taken again, 7.1 in front of its product, 8.8 out of 650 MB of rows in turn, 2.8 TB/s; launch and one trip to
+// memory are half of it).
 template <int TYPE, int NIT, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                          int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
@@ -185,7 +186,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const typename Elem<TYP
 }
 
 // Longer rows: one a block.  NIT > 0: the values stay in registers, 8 NIT of a thread (K <= 2048 NIT); 0: rows are read twice,
-// the second time from the L1 or L2.  8192 x 8192 in bf16, from memory: 42.5 us, 4.7 TB/s (read twice: 49).
+// the second time from the L2 or the memory-side cache.  From memory: 8192 x 8192 in bf16 43 us, 4.6 TB/s (read twice: 49), in fp32
+// 65 us, 5.1 TB/s; read twice 8192 x 11008 in bf16 71 us, 3.8 TB/s, in fp32 125 us, 3.6 TB/s, 4096 x 28672 in bf16 102 us, 3.5 TB/s.
 template <int TYPE, int NIT>
 __global__ __launch_bounds__(256) void quant_long_rows_kernel(const typename Elem<TYPE>::type* __restrict__ x, long long ldx,
                                                               int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
@@ -979,7 +981,8 @@ inline int gemm_args(const void* q, long long ldq, const float* q_scale, const v
     if (!apart({rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1), rows_of(q_scale, 1, T, 0, 4),
                 rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
-    // fewer than 2^32 threads in every tiling: 512 for 256 x 256, and for the 32 channels of a product of few tiles
+    // Fewer than 2^32 threads: 512 for 256 x 256, and for the 32 channels of a product of few tiles.  (Smaller tiles of as many
+    // results take more; past 2^32 those would fill more than the card's 288 GB, and the launch's error comes back.)
     if ((N + 31LL) / 32 > MAX_BLOCKS / 2) return PGAN_EINVAL;
     return (T + 255) / 256 * ((N + 255LL) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
 }

@@ -34,7 +34,8 @@ class AdamW(torch.optim.Optimizer):
     moment and of the root of the second, with their scales in `exp_avg_scale` and `exp_avg_sq_scale`.
     torch's amsgrad, maximize, differentiable and a decay that is part of the gradient are refused, in groups and loaded states.
     capturable: the steps are counted on the device, so that a captured graph counts on every replay; every parameter of a
-    group then needs a gradient in every step.  Without it a step refuses to be captured."""
+    group then needs a gradient in every step; rates, decay, betas and eps are those of the capture.  Without it a step refuses
+    to be captured."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0, capturable=False):
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:

@@ -971,6 +971,55 @@ bool launch_few(const FewArgs& f, hipStream_t st) {
     }
 }
 
+// Tiles of a product, tokens x channels; few: blocks of 32 x 32 whose waves share K
+enum class Tiling { few, t128x32, t256x256, t128x256, t128x128, t128x64, t64x32, t64x64 };
+inline Tiling tiling_of(long long T, int N, int K) {
+    const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
+    // how many in a hundred of the CUs that the last round of tiles takes along have one
+    const auto fill = [&](long long bt, long long bn) { return tiles(bt, bn) * 100 / ((tiles(bt, bn) + 255) / 256 * 256); };
+    // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
+    // behind another's products; and the last round of tiles should find a tile for most of the 256 CUs.  us in tiles of
+    // 256 x 256 (eight waves, one block a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64,
+    // 64 x 64, results in bf16:
+    //   4096 x 4096 x 4096     63   74   83   82  102      16000 x 512 x 4096     53   47   50   62   86
+    //   4096 x 2048 x 4096     36   40   45   45   58       4000 x 512 x 4096     15   14   15   17   21
+    //   3000 x 4000 x 3000     43   59   51   51   59      64000 x 256 x 2048     82   69   65   85  116
+    //   5000 x 2048 x 2000     28   31   28   29   36    256000 x 128 x 1024     118  106   96  127  173
+    //   6000 x 1200 x 6000     68   59   63   71   94       9493 x 422 x 7069     82   75   83  111  107
+    //   2500 x 2500 x 2500     31   25   25   33   31      10000 x 1000 x 1000    19   20   18   20   22
+    //   1037 x 2288 x 5552     27   21   23   28   25       4000 x 2000 x 1000    24   17   17   14   17
+    //   2000 x 8000 x 2000     73   54   55   42   54       2048 x 2048 x 2048    24   18   17   13   17
+    //   1500 x 4000 x 1500     40   29   28   22   21       1944 x 1575 x 1304    21   14   15   12   12
+    // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
+    // shares K among the waves of a block of 32 x 32 instead, one of somewhat more takes tiles of 64 x 32 (two waves): us in
+    // 32 x 32, 64 x 32, 64 x 64
+    //   64 x 4096 x 1024      7.3   9.3  11.1         704 x 4096 x 688     12.8  10.7  12.2
+    //   512 x 4096 x 512      8.7   9.5  11.1        1024 x 4096 x 512     13.1  10.3  11.7
+    //   512 x 512 x 512       3.9   4.2   4.3        1024 x 1024 x 512      5.6   5.0   5.3
+    //                                                1024 x 2048 x 1024    12.4   8.1   7.6
+    if (T <= FEW || tiles(64, 64) <= 64) return Tiling::few;
+    if (N <= 32) return Tiling::t128x32;
+    if (K >= 1024 && fill(256, 256) >= (K < 2048 ? 90 : 55)) return Tiling::t256x256;
+    if (K > 256 && fill(128, 256) >= 70) return Tiling::t128x256;
+    if (tiles(128, 128) >= 448) return Tiling::t128x128;
+    if (tiles(128, 64) >= 320) return Tiling::t128x64;
+    return tiles(64, 64) <= 128 ? Tiling::t64x32 : Tiling::t64x64;
+}
+// whether its launch has fewer than 2^32 threads
+inline bool launch_holds(long long T, int N, int K) {
+    const auto threads = [&](long long bt, long long bn, long long of) { return (T + bt - 1) / bt * ((N + bn - 1) / bn) * of < 1LL << 32; };
+    switch (tiling_of(T, N, K)) {
+        case Tiling::few: return threads(1LL << 40, 32, 512);       // along the channels; tokens are another dimension
+        case Tiling::t128x32: return threads(128, 32, 128);
+        case Tiling::t256x256: return threads(256, 256, 512);
+        case Tiling::t128x256: return threads(128, 256, 512);
+        case Tiling::t128x128: return threads(128, 128, 256);
+        case Tiling::t128x64: return threads(128, 64, 256);
+        case Tiling::t64x32: return threads(64, 32, 128);
+        default: return threads(64, 64, 256);
+    }
+}
+
 inline int gemm_args(const void* q, long long ldq, const float* q_scale, const void* w, long long ldw, const float* w_scale,
                      const float* bias, const void* y, int y_type, long long ldy, long long T, int N, int K) {
     if (T < 0 || N < 1 || K < 1 || K > 131072 || y_type < 0 || y_type > 2) return PGAN_EINVAL;
@@ -981,10 +1030,9 @@ inline int gemm_args(const void* q, long long ldq, const float* q_scale, const v
     if (!apart({rows_of(y, T, N, ldy, type_bytes(y_type), true), rows_of(q, T, K, ldq, 1), rows_of(q_scale, 1, T, 0, 4),
                 rows_of(w, N, K, ldw, 1), rows_of(w_scale, 1, N, 0, 4), rows_of(bias, 1, N, 0, 4)}))
         return PGAN_EINVAL;
-    // Fewer than 2^32 threads: 512 for 256 x 256, and for the 32 channels of a product of few tiles.  (Smaller tiles of as many
-    // results take more; past 2^32 those would fill more than the card's 288 GB, and the launch's error comes back.)
-    if ((N + 31LL) / 32 > MAX_BLOCKS / 2) return PGAN_EINVAL;
-    return (T + 255) / 256 * ((N + 255LL) / 256) > MAX_BLOCKS / 2 ? PGAN_EINVAL : PGAN_OK;
+    // fewer than 2^31 tokens and 2^28 channels, which keeps the counts of tiles inside 64 bits, and a launch that holds them
+    if ((N + 31LL) / 32 > MAX_BLOCKS / 2 || T > MAX_BLOCKS / 2 * 256) return PGAN_EINVAL;
+    return launch_holds(T, N, K) ? PGAN_OK : PGAN_EINVAL;
 }
 
 }  // namespace
@@ -1028,37 +1076,16 @@ int pgan_gemm_q8(const void* q, long long ldq, const float* q_scale, const void*
     return by_type(y_type, [&](auto t) {
         constexpr int Y = t.value;
         GemmArgs a{static_cast<const int8_t*>(q), q_scale, static_cast<const int8_t*>(w), w_scale, bias, y, ldq, ldw, ldy, T, N, K, 0, 0, 0};
-        const auto tiles = [&](long long bt, long long bn) { return (T + bt - 1) / bt * ((N + bn - 1) / bn); };
-        // how many in a hundred of the CUs that the last round of tiles takes along have one
-        const auto fill = [&](long long bt, long long bn) { return tiles(bt, bn) * 100 / ((tiles(bt, bn) + 255) / 256 * 256); };
-        // The larger the tile the fewer LDS reads a product takes; the smaller, the more blocks a CU has to hide one's results
-        // behind another's products; and the last round of tiles should find a tile for most of the 256 CUs.  us in tiles of
-        // 256 x 256 (eight waves, one block a CU), 128 x 256 (eight waves, two blocks), 128 x 128 (four blocks), 128 x 64,
-        // 64 x 64, results in bf16:
-        //   4096 x 4096 x 4096     63   74   83   82  102      16000 x 512 x 4096     53   47   50   62   86
-        //   4096 x 2048 x 4096     36   40   45   45   58       4000 x 512 x 4096     15   14   15   17   21
-        //   3000 x 4000 x 3000     43   59   51   51   59      64000 x 256 x 2048     82   69   65   85  116
-        //   5000 x 2048 x 2000     28   31   28   29   36    256000 x 128 x 1024     118  106   96  127  173
-        //   6000 x 1200 x 6000     68   59   63   71   94       9493 x 422 x 7069     82   75   83  111  107
-        //   2500 x 2500 x 2500     31   25   25   33   31      10000 x 1000 x 1000    19   20   18   20   22
-        //   1037 x 2288 x 5552     27   21   23   28   25       4000 x 2000 x 1000    24   17   17   14   17
-        //   2000 x 8000 x 2000     73   54   55   42   54       2048 x 2048 x 2048    24   18   17   13   17
-        //   1500 x 4000 x 1500     40   29   28   22   21       1944 x 1575 x 1304    21   14   15   12   12
-        // and 1024000 x 64 x 16 takes 21 us in tiles of 128 x 32 (two waves), 43 in tiles of 128 x 128.  A product of few tiles
-        // shares K among the waves of a block of 32 x 32 instead, one of somewhat more takes tiles of 64 x 32 (two waves): us in
-        // 32 x 32, 64 x 32, 64 x 64
-        //   64 x 4096 x 1024      7.3   9.3  11.1         704 x 4096 x 688     12.8  10.7  12.2
-        //   512 x 4096 x 512      8.7   9.5  11.1        1024 x 4096 x 512     13.1  10.3  11.7
-        //   512 x 512 x 512       3.9   4.2   4.3        1024 x 1024 x 512      5.6   5.0   5.3
-        //                                                1024 x 2048 x 1024    12.4   8.1   7.6
-        if (T <= FEW || tiles(64, 64) <= 64) launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st);
-        else if (N <= 32) launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st);
-        else if (K >= 1024 && fill(256, 256) >= (K < 2048 ? 90 : 55)) launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st);
-        else if (K > 256 && fill(128, 256) >= 70) launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st);
-        else if (tiles(128, 128) >= 448) launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st);
-        else if (tiles(128, 64) >= 320) launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st);
-        else if (tiles(64, 64) <= 128) launch_gemm<1, 1, 2, 1, 128, 4, 2, Y>(a, st);
-        else launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st);
+        switch (tiling_of(T, N, K)) {
+            case Tiling::few: launch_few<-1, Y>(FewArgs{a, nullptr, 0, 0, 0}, st); break;
+            case Tiling::t128x32: launch_gemm<2, 1, 2, 1, 64, 2, 4, Y>(a, st); break;
+            case Tiling::t256x256: launch_gemm<4, 2, 2, 4, 64, 4, 2, Y>(a, st); break;
+            case Tiling::t128x256: launch_gemm<2, 2, 2, 4, 64, 3, 4, Y>(a, st); break;
+            case Tiling::t128x128: launch_gemm<2, 2, 2, 2, 64, 2, 4, Y>(a, st); break;
+            case Tiling::t128x64: launch_gemm<2, 1, 2, 2, 128, 2, 3, Y>(a, st); break;
+            case Tiling::t64x32: launch_gemm<1, 1, 2, 1, 128, 4, 2, Y>(a, st); break;
+            case Tiling::t64x64: launch_gemm<1, 1, 2, 2, 128, 3, 3, Y>(a, st); break;
+        }
     });
 }
 

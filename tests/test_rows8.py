@@ -579,3 +579,13 @@ def test_linear_q8_at_the_borders_of_one_launch(hip, K, xt, yt):
         assert torch.equal(one, two), (T, K)
         want, tol = product64(*codes_of(lrelu(x.float()) if neg else x.float()), w, ws, bias)
         check_product(one[:T], want, tol, yt)
+
+
+def test_a_launch_of_too_many_threads_is_refused():
+    """Every tiling's launch stays below 2^32 threads (no GPU needed: refused before anything is launched)."""
+    import pgan_hip
+    lib = pgan_hip._lib._real
+    q, s, w, ws, y, x = 1 << 12, 1 << 40, 1 << 41, 1 << 42, 1 << 46, 1 << 44
+    for T, N in ((1 << 30, 129), (715827968, 257), ((1 << 31) - 256, 200)):
+        assert lib.pgan_gemm_q8(q, 16, s, w, 16, ws, None, y, 1, N, T, N, 16, None) == -1, (T, N)
+        assert lib.pgan_linear_q8(x, 1, 16, q, 16, s, w, 16, ws, None, y, 1, N, T, N, 16, 0, None) == -1, (T, N)
